@@ -1,0 +1,34 @@
+"""What the operators of a cache held in 4 bits refuse, without a GPU: the checks of the arguments alone."""
+
+import pytest
+
+from packed_plain import refusals
+
+
+def test_refused_before_anything_is_launched(monkeypatch):
+    from yalis_b200.ops import packed
+    from yalis_b200.ops._lib import KernelError
+
+    def launched():
+        raise AssertionError("an argument that should have been refused reached the library")
+
+    monkeypatch.setattr(packed, "_need_here", lambda *a: None)
+    monkeypatch.setattr(packed, "lib", launched)
+    for what, call in refusals("cpu"):
+        with pytest.raises(KernelError):
+            call()
+            pytest.fail(what)
+
+
+def test_tensors_on_the_cpu_are_refused():
+    import torch
+    from packed_plain import Cache
+    from yalis_b200.ops._lib import KernelError
+    from yalis_b200.ops.packed import evict_tokens, packed_kv_write
+    c = Cache([40], 2, 64, 16)
+    pages, table = c.to("cpu")
+    x, at = torch.zeros(1, 128), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(KernelError, match="GPU"):
+        packed_kv_write(x, x, pages, at, at, table)
+    with pytest.raises(KernelError, match="GPU"):
+        evict_tokens(pages.pools(), c.sums, at, table, 4)

@@ -1,0 +1,65 @@
+// Rows of keys and values held in 4 bits, as every kernel over such pages reads and writes them.
+//
+// A row of `dim` values (one token, one KV head) is dim codes c of 4 bits and one 16-bit word: value = (c - zero) * step.  With
+// lo = min(x, 0), hi = max(x, 0): step is the smallest number of four significant bits (at least 2^-126) with 15 step >= hi - lo,
+// zero = -rint(lo / step), c = rint(x / step) + zero within 0 .. 15.  |c - zero| has at most four significant bits, the step
+// four: every value is a bfloat16 number, so that what is computed from codes (products of small whole numbers, the step applied
+// once per row) and what is computed from unpacked bfloat16 rows agree without a second rounding.  A step rounded up to four bits
+// is 4 % too wide on average, 12.5 % at worst.  The word holds the step's bfloat16 bits, whose lowest four are zero, and
+// there the zero.  A row with a NaN, an infinity or a magnitude above 2^120 reads back as NaN throughout.
+//
+// Eight codes are a 32-bit word, element i in bits 4i .. 4i + 3; rows start on 4-byte boundaries (dim a multiple of 8).
+#pragma once
+
+#include "common.cuh"
+
+namespace {
+
+constexpr float kPackedLargest = 1.329227995784916e36f;       // 2^120
+constexpr float kPackedLeast = 1.1754943508222875e-38f;       // 2^-126
+
+struct PackedPages {
+  uint32_t* k;                 // [pages, g, page_size, dim / 8]
+  uint32_t* v;
+  uint32_t* words;             // [pages, g, page_size]: the key's word low, the value's high
+  int num_pages, page_size, g, dim;
+};
+
+__device__ __forceinline__ float step_of(uint32_t word16) { return __uint_as_float((word16 & 0xFFF0u) << 16); }
+__device__ __forceinline__ float zero_of(uint32_t word16) { return (float)(word16 & 15u); }
+
+// The page and row of cached token `at` of a request; page -1 where the table has none.
+__device__ __forceinline__ int page_of(const PackedPages& c, const int32_t* table_row, int table_width, int at, int& row) {
+  const int index = at / c.page_size;
+  row = at - index * c.page_size;
+  const int page = index < table_width ? table_row[index] : -1;
+  return page >= 0 && page < c.num_pages ? page : -1;
+}
+__device__ __forceinline__ size_t row_index(const PackedPages& c, int page, int kvh, int row) {
+  return ((size_t)page * c.g + kvh) * c.page_size + row;
+}
+
+// The step of a row with the given extremes (lo <= 0 <= hi, finite, at most 2^120 in magnitude).  Bits are rounded up to four
+// significant ones; hi - lo and its fifteenth part were rounded before, which can only lose what stands above a number of four
+// bits by less than a rounding: the exact difference (rounded + lost) is compared with 15 step, which is exact.
+__device__ __forceinline__ float step_for(float lo, float hi) {
+  const float range = hi - lo;
+  const float lost = (hi - (range + lo)) + (-lo - (range - (range + lo)));     // range + lost = hi - lo without rounding
+  const uint32_t up = 0x000FFFFFu;
+  float step = __uint_as_float((__float_as_uint(__fdiv_rn(range, 15.f)) + up) & ~up);
+  const float most = 15.f * step;
+  if (range > most || (range == most && lost > 0.f)) step = __uint_as_float(__float_as_uint(step) + up + 1u);
+  return fmaxf(step, kPackedLeast);
+}
+
+// rint(x / step): the quotient's own rounding may land on a tie that the exact one misses by less; what is left over after the
+// rounded multiple is exact and says so.
+__device__ __forceinline__ float multiple_of(float x, float step) {
+  float n = rintf(__fdiv_rn(x, step));
+  const float left = fmaf(-n, step, x), half = 0.5f * step;
+  if (left > half) n += 1.f;
+  if (left < -half) n -= 1.f;
+  return n;
+}
+
+}  // namespace

@@ -32,3 +32,22 @@ def test_tensors_on_the_cpu_are_refused():
         packed_kv_write(x, x, pages, at, at, table)
     with pytest.raises(KernelError, match="GPU"):
         evict_tokens(pages.pools(), c.sums, at, table, 4)
+
+
+def test_argument_types_are_those_of_the_library():
+    """The types that the wrappers set are those of the C entries' parameters, in order."""
+    import glob
+    import os
+    import re
+
+    from yalis_b200.ops import packed
+    root = os.path.dirname(os.path.dirname(packed.__file__))
+    entries = {}
+    for path in glob.glob(os.path.join(root, "csrc", "*.cu")):
+        for name, parameters in re.findall(r"YALIS_API [\w ]+?(\w+)\(([^)]*)\)", open(path).read()):
+            kinds = ["p" if "*" in x or "cudaStream_t" in x else {"int": "i", "long": "l", "float": "f"}[x.split()[0]] for x in parameters.split(",") if x.strip()]
+            entries[name] = "".join(kinds)
+    used = re.findall(r'_entry\("(\w+)", ((?:"[plif]*"(?: \+ )?)+)', open(packed.__file__).read())
+    assert len(used) >= 6
+    for name, signature in used:
+        assert "".join(re.findall(r'"([plif]*)"', signature)) == entries[name], name

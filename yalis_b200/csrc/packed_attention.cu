@@ -156,23 +156,47 @@ __global__ void __launch_bounds__(kThreads) packed_weight_sums_general_kernel(co
 
 }  // namespace
 
+namespace {
+
+bool params_of(AttentionParams& p, const void* q, long long q_stride, void* k_codes, void* v_codes, void* words, int num_pages, int page_size,
+               int g, int dim, const int32_t* positions, const int32_t* q_start, const int32_t* block_table, int table_width, int n_requests,
+               int nh, float scale, int window) {
+  if (dim < 8 || dim > 256 || dim % 8 || page_size < 1 || g < 1 || nh % g || nh > 65535 || n_requests > 65535) return false;
+  p = {};
+  p.q = q; p.q_stride = q_stride;
+  p.positions = positions; p.q_start = q_start; p.block_table = block_table; p.table_width = table_width;
+  p.n_requests = n_requests; p.nh = nh; p.per = nh / g; p.window = window; p.scale = scale;
+  p.pages = {static_cast<uint32_t*>(k_codes), static_cast<uint32_t*>(v_codes), static_cast<uint32_t*>(words), num_pages, page_size, g, dim};
+  return true;
+}
+
+}  // namespace
+
 YALIS_API int yalis_packed_attention_general(const void* q, long long q_stride, int dtype, void* out, long long out_stride, void* k_codes,
                                              void* v_codes, void* words, int num_pages, int page_size, int g, int dim,
                                              const int32_t* positions, const int32_t* q_start, const int32_t* block_table, int table_width,
-                                             int n_requests, int n_tokens, int max_kv_len, int nh, float scale, int window, float* lse,
-                                             float* sums, int32_t* error, cudaStream_t stream) {
-  if (dim < 8 || dim > 256 || dim % 8 || page_size < 1 || g < 1 || nh % g || nh > 65535 || n_requests > 65535) return YALIS_ERR_SHAPE;
+                                             int n_requests, int n_tokens, int nh, float scale, int window, float* lse, int32_t* error,
+                                             cudaStream_t stream) {
+  AttentionParams p;
+  if (!params_of(p, q, q_stride, k_codes, v_codes, words, num_pages, page_size, g, dim, positions, q_start, block_table, table_width, n_requests,
+                 nh, scale, window))
+    return YALIS_ERR_SHAPE;
   if (n_tokens <= 0 || n_requests <= 0) return YALIS_OK;
-  AttentionParams p = {};
-  p.q = q; p.q_stride = q_stride; p.out = out; p.out_stride = out_stride;
-  p.positions = positions; p.q_start = q_start; p.block_table = block_table; p.table_width = table_width;
-  p.n_requests = n_requests; p.n_tokens = n_tokens; p.nh = nh; p.per = nh / g; p.window = window; p.scale = scale;
-  p.lse = lse; p.sums = sums; p.error = error;
-  p.pages = {static_cast<uint32_t*>(k_codes), static_cast<uint32_t*>(v_codes), static_cast<uint32_t*>(words), num_pages, page_size, g, dim};
-  YALIS_DISPATCH_DTYPE(dtype, T, {
-    int rc = yalis_launch(packed_attention_general_kernel<T>, dim3(n_tokens, nh), dim3(kThreads), 0, stream, p);
-    if (rc == YALIS_OK && sums)
-      rc = yalis_launch(packed_weight_sums_general_kernel<T>, dim3((max_kv_len + kThreads - 1) / kThreads, g, n_requests), dim3(kThreads), 0, stream, p);
-    return rc;
-  });
+  p.out = out; p.out_stride = out_stride; p.n_tokens = n_tokens; p.lse = lse; p.error = error;
+  YALIS_DISPATCH_DTYPE(dtype, T, return yalis_launch(packed_attention_general_kernel<T>, dim3(n_tokens, nh), dim3(kThreads), 0, stream, p));
+}
+
+// Adds to `sums` the weights that the step's rows give the cached tokens; `lse` [N, nh] from the attention of the same step.
+YALIS_API int yalis_packed_weight_sums_general(const void* q, long long q_stride, int dtype, void* k_codes, void* v_codes, void* words,
+                                               int num_pages, int page_size, int g, int dim, const int32_t* positions, const int32_t* q_start,
+                                               const int32_t* block_table, int table_width, int n_requests, int max_kv_len, int nh, float scale,
+                                               int window, float* lse, float* sums, cudaStream_t stream) {
+  AttentionParams p;
+  if (!params_of(p, q, q_stride, k_codes, v_codes, words, num_pages, page_size, g, dim, positions, q_start, block_table, table_width, n_requests,
+                 nh, scale, window) || g > 65535)
+    return YALIS_ERR_SHAPE;
+  if (n_requests <= 0 || max_kv_len <= 0) return YALIS_OK;
+  p.lse = lse; p.sums = sums;
+  YALIS_DISPATCH_DTYPE(dtype, T, return yalis_launch(packed_weight_sums_general_kernel<T>, dim3((max_kv_len + kThreads - 1) / kThreads, g, n_requests),
+                                                     dim3(kThreads), 0, stream, p));
 }

@@ -1,0 +1,681 @@
+// Attention over pages held in 4 bits (packed.cuh) on the tensor cores, for single tokens and short portions in bfloat16 and for
+// every step in float32 (head sizes 64 and 128).  What is computed is what packed_attention.cu says.
+//
+// A pair is a KV head of a request with up to 8 NT of its query rows (row = token * heads per KV head + head), which are the columns
+// here: both products are taken transposed, so that the codes are the operand of 16 rows and a lane turns the codes it has loaded
+// into bfloat16 pairs in registers, with nothing in between:
+//
+//   S^T [keys, columns] = C_K [16 keys x 16 elements] q^T       O^T [elements, columns] += C_V^T [16 elements x 16 keys] W^T
+//
+// The order of a product's inner index is free as long as both operands agree, so a lane takes neighbouring codes: with a word of
+// eight codes, (w >> s) & 0x00780078 | 0x41804180 is the pair 16 + c_i, 16 + c_(i + 4) in bfloat16, from which 16 + zero is taken
+// away (exact).  Elements of a V row pair up by key instead: the 16-bit halves of two keys' words are put side by side first.  The
+// scores' accumulators, times step, are the softmax's scores; the weights times the values' steps are rounded to bfloat16
+// (float32: in three parts) and turned from accumulator layout to operand layout by movmatrix.
+//
+// A warp takes 32 keys at a time (a chunk) through a ring of its own in shared memory, filled by 16-byte asynchronous copies, and
+// keeps a softmax and an output of its own; the four warps of a block come together at the end of a pair.  Chunks are
+// dealt to a fixed grid by the step's lengths (choose_deal), so that a recorded launch serves other lengths too; a pair cut between
+// blocks is added up, in the blocks' order, by whichever of them comes last (a counter per pair, left at zero).  Nothing waits for
+// another block.
+#include "packed.cuh"
+
+namespace {
+
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kChunk = 32;     // keys of a chunk
+constexpr int kStages = 2;
+constexpr float kLazy = 8.f;   // how far (log2) scores may rise above the maximum in use before the output is rescaled
+
+struct MmaParams {
+  const void* q;               // [N, q_stride]
+  long long q_stride;
+  void* out;                   // [N, out_stride]
+  long long out_stride;
+  const int32_t* positions;    // [N]
+  const int32_t* q_start;      // [R + 1]
+  const int32_t* block_table;  // [R, table_width]
+  int table_width, n_requests, nh, per, window, page_shift;
+  int q_vector;                // 1: rows of q start on 16-byte boundaries
+  int only_single;             // 1: requests that bring more than one token are left to another kernel
+  float scale_log2;
+  float* lse;                  // [N, nh] or null
+  float* part;                 // [blocks, 2, MT * 32 * 4 + 16 NT * 2]
+  int32_t* tickets;            // one per pair, zero before and after
+  int32_t* error;
+  PackedPages pages;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t pair_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t minus(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// 16 + codes i and i + 4 of the eight in w as bfloat16.
+template <int I>
+__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
+  const uint32_t at = I == 0 ? w << 3 : w >> (I == 0 ? 0 : 4 * I - 3);
+  return (at & 0x00780078u) | 0x41804180u;
+}
+// Parts of a float32 pair in bfloat16: PARTS 1 rounds it; 3 hold every bit.
+template <int PARTS>
+__device__ __forceinline__ void parts_of(float x, float y, uint32_t (&out)[PARTS]) {
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    out[i] = pair_bf16(x, y);
+    if (i + 1 < PARTS) {
+      x -= __uint_as_float(out[i] << 16);
+      y -= __uint_as_float(out[i] & 0xFFFF0000u);
+    }
+  }
+}
+
+// Which key of 16 stands in row i of a product's tile: rows 2t hold keys t, rows 2t + 1 keys 4 + (t ^ X), so that the lanes of a
+// quarter (K) or half (V) of a warp read different banks.
+template <int DIM>
+__device__ __forceinline__ int key_of_row(int i) {
+  constexpr int X = DIM == 128 ? 1 : 2;
+  return (i & 8) + ((i & 1) ? 4 + (((i & 7) >> 1) ^ X) : (i & 7) >> 1);
+}
+// Byte of a chunk's row r (DIM / 2 bytes) in shared memory, in pieces of 16; rows of 64 bytes swap their halves every other pair.
+template <int DIM>
+__device__ __forceinline__ int piece_at(int r, int piece) {
+  return r * (DIM / 2) + ((DIM == 128 ? piece ^ (r & 2) : piece) << 4);
+}
+
+template <int DIM>
+struct Stage {
+  unsigned char k[kChunk * DIM / 2];
+  unsigned char v[kChunk * DIM / 2];
+  uint32_t words[kChunk];
+};
+
+// How a step's chunks are dealt out, by what the slowest block then has to do, counted in chunks:
+//   pieces k > 0: every pair to k blocks in equal pieces, one piece a block;
+//   0: all chunks of all pairs, laid end to end, in equal shares; a block's share begins and ends inside pairs that others share.
+// A piece is at least kLeast chunks; to come together with other blocks takes about kJoin chunks' time.
+struct Deal {
+  int pieces, blocks;
+};
+constexpr int kLeast = 2 * kWarps, kJoin = 4;
+
+__device__ __forceinline__ Deal choose_deal(int grid, int pairs, int most, long long total) {
+  const int even_blocks = (int)min((long long)grid, (total + kLeast - 1) / kLeast);
+  if (pairs > grid) return {0, even_blocks};
+  const int k = max(1, min(grid / pairs, (most + kLeast - 1) / kLeast));
+  const long long even = total / even_blocks + 2 * kJoin;
+  if ((most + k - 1) / k + (k > 1 ? kJoin : 0) <= even) return {k, pairs * k};
+  return {0, even_blocks};
+}
+
+template <typename T, int DIM, int NT, int PARTS>
+__global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packed_attention_mma_kernel(const MmaParams p) {
+  constexpr int W = DIM / 32;                  // words of a K row that a lane takes
+  constexpr int U = DIM / 64;                  // words of a V row that a lane takes
+  constexpr int MT = DIM / 16;                 // tiles of 16 elements of the output
+  constexpr int COLS = 8 * NT;
+  constexpr int PIECES = DIM / 32;             // 16-byte pieces of a row
+  constexpr int COPIES = PIECES;               // of K (and as many of V) that a lane asks for per chunk
+  constexpr int PART_FLOATS = NT * MT * 128 + 2 * COLS;
+  extern __shared__ __align__(128) unsigned char smem[];
+  Stage<DIM>* ring = reinterpret_cast<Stage<DIM>*>(smem) + (threadIdx.x >> 5) * kStages;
+  float4* merge_o = reinterpret_cast<float4*>(smem + sizeof(Stage<DIM>) * kStages * kWarps);       // [kWarps][NT * MT][32]
+  float* merge_ml = reinterpret_cast<float*>(merge_o + kWarps * NT * MT * 32);                     // [kWarps][COLS][2]
+  int* s_last = reinterpret_cast<int*>(merge_ml + kWarps * COLS * 2);
+  int* s_deal = s_last + 1;                                                                        // pieces, blocks
+  long long* cum = reinterpret_cast<long long*>(s_last + 4);                                       // [R + 1] chunks before request r
+  int* cum_pairs = reinterpret_cast<int*>(cum + p.n_requests + 1);                                 // [R + 1] pairs before it
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  pdl_wait();
+
+  // ---- the chunks of every request (KV heads, blocks of columns and chunks of 32 keys), their running sum, this block's share ----
+  auto span_of = [&](int r, int& first_key, int& n_rows) {      // chunks of a pair of request r
+    const int t0 = p.q_start[r], n = p.q_start[r + 1] - t0;
+    n_rows = 0;
+    if (n <= 0 || (p.only_single && n > 1)) return 0;
+    n_rows = n * p.per;
+    const int last = p.positions[t0 + n - 1], begin = p.positions[t0];
+    first_key = p.window > 0 ? max(0, begin - p.window + 1) / kChunk * kChunk : 0;
+    return max(1, last < first_key ? 1 : (last - first_key) / kChunk + 1);       // (rows that see nothing are written too)
+  };
+  for (int r = threadIdx.x; r < p.n_requests; r += kThreads) {
+    int first_key, n_rows;
+    const int chunks = span_of(r, first_key, n_rows);
+    cum_pairs[r + 1] = (n_rows + COLS - 1) / COLS * p.pages.g;
+    cum[r + 1] = chunks;
+  }
+  if (threadIdx.x == 0) cum[0] = cum_pairs[0] = 0;
+  __syncthreads();
+  if (warp == 0) {
+    long long carry = 0;
+    int carry_pairs = 0, most = 0;
+    for (int r0 = 0; r0 < p.n_requests; r0 += 32) {
+      const int r = r0 + lane;
+      int pairs = r < p.n_requests ? cum_pairs[r + 1] : 0;
+      long long v = r < p.n_requests ? cum[r + 1] : 0;
+      most = max(most, (int)v);
+      v *= pairs;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, v, o);
+        const int w = __shfl_up_sync(0xffffffffu, pairs, o);
+        if (lane >= o) { v += u; pairs += w; }
+      }
+      if (r < p.n_requests) { cum[r + 1] = carry + v; cum_pairs[r + 1] = carry_pairs + pairs; }
+      carry += __shfl_sync(0xffffffffu, v, 31);
+      carry_pairs += __shfl_sync(0xffffffffu, pairs, 31);
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) {
+      const Deal deal = carry > 0 ? choose_deal(gridDim.x, carry_pairs, most, carry) : Deal{0, 0};
+      s_deal[0] = deal.pieces;
+      s_deal[1] = deal.blocks;
+    }
+  }
+  __syncthreads();
+  const long long total = cum[p.n_requests];
+  const int pieces = s_deal[0], blocks = s_deal[1];
+  if ((int)blockIdx.x >= blocks) { pdl_launch_dependents(); return; }
+  auto last_at_most = [&](auto* sums, auto value) {             // the request whose range of the running sum holds `value`
+    int lo = 0, hi = p.n_requests - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (sums[mid] <= value) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+  };
+  auto share = [&](int b) { return (long long)b * total / blocks; };
+  long long at, end;
+  int req, first_block = 0, n_blocks = 1;                       // the blocks that hold the current pair
+  if (pieces > 0) {
+    const int pair = blockIdx.x / pieces, piece = blockIdx.x - pair * pieces;
+    req = last_at_most(cum_pairs, pair);
+    const int chunks = (int)((cum[req + 1] - cum[req]) / (cum_pairs[req + 1] - cum_pairs[req]));
+    first_block = pair * pieces;
+    n_blocks = min(pieces, chunks);
+    if (piece >= n_blocks) { pdl_launch_dependents(); return; }
+    at = cum[req] + (long long)(pair - cum_pairs[req]) * chunks;
+    end = at + (long long)(piece + 1) * chunks / n_blocks;
+    at += (long long)piece * chunks / n_blocks;
+  } else {
+    at = share(blockIdx.x);
+    end = share(blockIdx.x + 1);
+    req = last_at_most(cum, at);
+  }
+
+  for (bool first_of_block = true; at < end; first_of_block = false) {
+    while (cum[req + 1] <= at) ++req;
+    int first_key, n_rows;
+    const int chunks = span_of(req, first_key, n_rows);
+    const int col_blocks = (n_rows + COLS - 1) / COLS;
+    const long long inside = at - cum[req];
+    const int sub = (int)(inside / chunks), kvh = sub / col_blocks, column0 = (sub - kvh * col_blocks) * COLS;
+    const int lo = (int)(inside - (long long)sub * chunks), hi = (int)min((long long)chunks, lo + (end - at));    // chunks [lo, hi) of the pair
+    const long long first = at - lo;                            // its first chunk among all
+    at += hi - lo;
+    if (pieces == 0) {
+      auto holder = [&](long long chunk) { return (int)(((chunk + 1) * blocks + total - 1) / total) - 1; };
+      first_block = holder(first);
+      n_blocks = holder(first + chunks - 1) - first_block + 1;
+    }
+
+    // ---- columns: queries in registers as the products' right operand, the keys that each sees ----
+    const int tok0 = p.q_start[req];
+    const int32_t* table_row = p.block_table + (size_t)req * p.table_width;
+    uint32_t qf[NT][2 * W][2][PARTS];
+    int see_hi[NT][2], see_lo[NT][2], all_hi = 0x7fffffff, all_lo = 0, any_hi = -1, any_lo = 0x7fffffff;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = column0 + nt * 8 + g;
+      const bool real = row < n_rows;
+      const int token = tok0 + (real ? row / p.per : 0), head = kvh * p.per + (real ? row % p.per : 0);
+      const T* src = static_cast<const T*>(p.q) + (long long)token * p.q_stride + (long long)head * DIM + t * (DIM / 4);
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        float x[8];
+        if (!real) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = 0.f;
+        } else if (p.q_vector) {
+          const float4 a = load4_f32(src + 8 * w), b = load4_f32(src + 8 * w + 4);
+          x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+          x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(src[8 * w + i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) parts_of<PARTS>(x[i], x[i + 4], qf[nt][2 * w + (i >> 1)][i & 1]);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int column = column0 + nt * 8 + 2 * t + e;
+        see_hi[nt][e] = 0x7fffffff;
+        see_lo[nt][e] = 0;
+        if (column < n_rows) {
+          see_hi[nt][e] = p.positions[tok0 + column / p.per];
+          see_lo[nt][e] = p.window > 0 ? max(0, see_hi[nt][e] - p.window + 1) : 0;
+          all_hi = min(all_hi, see_hi[nt][e]);
+          all_lo = max(all_lo, see_lo[nt][e]);
+          any_hi = max(any_hi, see_hi[nt][e]);
+          any_lo = min(any_lo, see_lo[nt][e]);
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      all_hi = min(all_hi, __shfl_xor_sync(0xffffffffu, all_hi, o));
+      all_lo = max(all_lo, __shfl_xor_sync(0xffffffffu, all_lo, o));
+      any_hi = max(any_hi, __shfl_xor_sync(0xffffffffu, any_hi, o));
+      any_lo = min(any_lo, __shfl_xor_sync(0xffffffffu, any_lo, o));
+    }
+
+    float m[NT][2], l[NT][2], acc[NT][MT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
+    }
+
+    // Chunks of this warp that any column sees: one in kWarps.
+    int c = lo + warp, c_end = hi;
+    if (any_hi < 0) c_end = 0;
+    else c_end = min(c_end, any_hi < first_key ? 0 : (any_hi - first_key) / kChunk + 1);
+    if (any_lo > first_key) {
+      const int skip = (any_lo - first_key) / kChunk;
+      while (c < skip) c += kWarps;
+    }
+    auto lookup = [&](int chunk) {               // the pool's row of the lane's key, -1 without a page
+      const int key = first_key + chunk * kChunk + lane;
+      if (key > any_hi) return -2;               // nobody's
+      const int index = p.page_shift >= 0 ? key >> p.page_shift : key / p.pages.page_size;
+      const int page = index < p.table_width ? table_row[index] : -1;
+      if (page < 0 || page >= p.pages.num_pages) {
+        if (key >= any_lo && p.error) atomicOr(p.error, YALIS_FLAG_BAD_PAGE);
+        return -1;
+      }
+      return (page * p.pages.g + kvh) * p.pages.page_size + (key - index * p.pages.page_size);
+    };
+    auto ask = [&](int stage, int row) {         // rows that are not there are left as they are: their word says so
+      Stage<DIM>& st = ring[stage];
+      const uint32_t k_at = smem_u32(st.k), v_at = smem_u32(st.v);
+#pragma unroll
+      for (int i = 0; i < COPIES; ++i) {
+        const int r = i * (32 / PIECES) + lane / PIECES, piece = lane % PIECES;
+        const int from = __shfl_sync(0xffffffffu, row, r);
+        if (from >= 0) {
+          const size_t byte = (size_t)from * (DIM / 2) + piece * 16;
+          copy16(k_at + piece_at<DIM>(r, piece), reinterpret_cast<const unsigned char*>(p.pages.k) + byte);
+          copy16(v_at + piece_at<DIM>(r, piece), reinterpret_cast<const unsigned char*>(p.pages.v) + byte);
+        }
+      }
+      if (row >= 0) copy4(smem_u32(&st.words[lane]), p.pages.words + row);
+      else st.words[lane] = 0u;
+    };
+    int row = c < c_end ? lookup(c) : -2;
+    if (c < c_end) ask(0, row);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    bool missing = __any_sync(0xffffffffu, row < 0);
+    row = c + kWarps < c_end ? lookup(c + kWarps) : -2;
+    for (int stage = 0; c < c_end; c += kWarps, stage ^= 1) {
+      const bool missing_next = __any_sync(0xffffffffu, row < 0);
+      if (c + kWarps < c_end) ask(stage ^ 1, row);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      if (c + 2 * kWarps < c_end) row = lookup(c + 2 * kWarps);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      __syncwarp();
+      const Stage<DIM>& st = ring[stage];
+      const int key0 = first_key + c * kChunk;
+
+      // ---- scores of 32 keys ----
+      float sc[NT][2][4];
+      uint32_t word[2][2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int ra = half * 16 + key_of_row<DIM>(g), rb = ra + 8;
+        word[half][0] = st.words[ra];
+        word[half][1] = st.words[rb];
+        uint32_t wa[W], wb[W];
+        if constexpr (DIM == 128) {
+          *reinterpret_cast<uint4*>(wa) = *reinterpret_cast<const uint4*>(st.k + piece_at<DIM>(ra, t));
+          *reinterpret_cast<uint4*>(wb) = *reinterpret_cast<const uint4*>(st.k + piece_at<DIM>(rb, t));
+        } else {
+          *reinterpret_cast<uint2*>(wa) = *reinterpret_cast<const uint2*>(st.k + ra * (DIM / 2) + t * 8);
+          *reinterpret_cast<uint2*>(wb) = *reinterpret_cast<const uint2*>(st.k + rb * (DIM / 2) + t * 8);
+        }
+        const uint32_t za = ((word[half][0] & 15u) << 3 | 0x4180u) * 0x10001u, zb = ((word[half][1] & 15u) << 3 | 0x4180u) * 0x10001u;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sc[nt][half][0] = sc[nt][half][1] = sc[nt][half][2] = sc[nt][half][3] = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const uint32_t lo[4] = {minus(code_pair<0>(wa[w]), za), minus(code_pair<0>(wb[w]), zb), minus(code_pair<1>(wa[w]), za), minus(code_pair<1>(wb[w]), zb)};
+          const uint32_t hi[4] = {minus(code_pair<2>(wa[w]), za), minus(code_pair<2>(wb[w]), zb), minus(code_pair<3>(wa[w]), za), minus(code_pair<3>(wb[w]), zb)};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = PARTS - 1; i >= 0; --i) {
+              mma_bf16(sc[nt][half], lo, qf[nt][2 * w][0][i], qf[nt][2 * w][1][i]);
+              mma_bf16(sc[nt][half], hi, qf[nt][2 * w + 1][0][i], qf[nt][2 * w + 1][1][i]);
+            }
+          }
+        }
+      }
+      // ---- softmax: scores in powers of two, maxima over the chunk ----
+      const bool masked = missing || key0 + kChunk - 1 > all_hi || key0 < all_lo;
+      float most[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) most[nt][0] = most[nt][1] = -INFINITY;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float step = step_of(word[half][e]) * p.scale_log2;
+          const int key = key0 + half * 16 + key_of_row<DIM>(g) + 8 * e;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              float& v = sc[nt][half][2 * e + x];
+              v *= step;
+              if (masked && !(key <= see_hi[nt][x] && key >= see_lo[nt][x] && word[half][e] != 0u)) v = -INFINITY;
+              most[nt][x] = fmaxf(most[nt][x], v);
+            }
+          }
+        }
+      }
+      bool grow = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) most[nt][x] = fmaxf(most[nt][x], __shfl_xor_sync(0xffffffffu, most[nt][x], o));
+          grow |= most[nt][x] > m[nt][x] + kLazy || (m[nt][x] == -INFINITY && most[nt][x] != -INFINITY);
+        }
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float keep[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float next = fmaxf(m[nt][x], most[nt][x]);
+            keep[x] = next == -INFINITY ? 1.f : exp2_fast(m[nt][x] - next);
+            m[nt][x] = next;
+            l[nt][x] *= keep[x];
+          }
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            acc[nt][i][0] *= keep[0]; acc[nt][i][1] *= keep[1];
+            acc[nt][i][2] *= keep[0]; acc[nt][i][3] *= keep[1];
+          }
+        }
+      }
+      uint32_t wf[NT][2][2][PARTS];              // [half][keys g, g + 8 of the half]: the weights as the second product's operand
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float base0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], base1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float step = step_of(word[half][e] >> 16);
+            const float s0 = sc[nt][half][2 * e], s1 = sc[nt][half][2 * e + 1];
+            const float e0 = PARTS == 1 ? exp2_fast(s0 - base0) : exp2f(s0 - base0), e1 = PARTS == 1 ? exp2_fast(s1 - base1) : exp2f(s1 - base1);
+            l[nt][0] += e0;
+            l[nt][1] += e1;
+            float w0 = e0 * step, w1 = e1 * step;
+            if (masked) {                        // a row that is not seen may hold anything
+              if (s0 == -INFINITY) w0 = 0.f;
+              if (s1 == -INFINITY) w1 = 0.f;
+            }
+            uint32_t part[PARTS];
+            parts_of<PARTS>(w0, w1, part);
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) wf[nt][half][e][i] = transposed(part[i]);
+          }
+        }
+      }
+      // ---- output ----
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t vw[4][U], z[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {            // keys of rows 2t, 2t + 1, 2t + 8, 2t + 9
+          const int r = half * 16 + key_of_row<DIM>(2 * t + (i & 1) + (i & 2) * 4);
+          z[i] = st.words[r];
+          if constexpr (DIM == 128) {
+            const uint2 two = *reinterpret_cast<const uint2*>(st.v + piece_at<DIM>(r, g >> 1) + (g & 1) * 8);
+            vw[i][0] = two.x;
+            vw[i][U - 1] = two.y;
+          } else {
+            vw[i][0] = *reinterpret_cast<const uint32_t*>(st.v + r * (DIM / 2) + g * 4);
+          }
+        }
+        const uint32_t z01 = ((z[0] >> 13) & 0x78u) | ((z[1] << 3) & 0x00780000u) | 0x41804180u;
+        const uint32_t z23 = ((z[2] >> 13) & 0x78u) | ((z[3] << 3) & 0x00780000u) | 0x41804180u;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t a = __byte_perm(vw[0][u], vw[1][u], h ? 0x7632 : 0x5410), b = __byte_perm(vw[2][u], vw[3][u], h ? 0x7632 : 0x5410);
+            const uint32_t f0[4] = {minus(code_pair<0>(a), z01), minus(code_pair<1>(a), z01), minus(code_pair<0>(b), z23), minus(code_pair<1>(b), z23)};
+            const uint32_t f1[4] = {minus(code_pair<2>(a), z01), minus(code_pair<3>(a), z01), minus(code_pair<2>(b), z23), minus(code_pair<3>(b), z23)};
+            const int tile = 4 * u + 2 * h;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              if constexpr (PARTS == 1) {
+                mma_bf16(acc[nt][tile], f0, wf[nt][half][0][0], wf[nt][half][1][0]);
+                mma_bf16(acc[nt][tile + 1], f1, wf[nt][half][0][0], wf[nt][half][1][0]);
+              } else {                           // added to the running output by float32 additions: the tensor cores cut sums off
+                float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = PARTS - 1; i >= 0; --i) {
+                  mma_bf16(d0, f0, wf[nt][half][0][i], wf[nt][half][1][i]);
+                  mma_bf16(d1, f1, wf[nt][half][0][i], wf[nt][half][1][i]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  acc[nt][tile][i] += d0[i];
+                  acc[nt][tile + 1][i] += d1[i];
+                }
+              }
+            }
+          }
+        }
+      }
+      missing = missing_next;
+      __syncwarp();                              // the stage is read: the next round may fill it
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (at >= end) pdl_launch_dependents();      // this block's last tile is there
+
+    // ---- the four warps' results together ----
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], o);
+        if (g == 0) {
+          merge_ml[(warp * COLS + nt * 8 + 2 * t + x) * 2] = m[nt][x];
+          merge_ml[(warp * COLS + nt * 8 + 2 * t + x) * 2 + 1] = l[nt][x];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        merge_o[(warp * NT * MT + nt * MT + i) * 32 + lane] = make_float4(acc[nt][i][0], acc[nt][i][1], acc[nt][i][2], acc[nt][i][3]);
+    }
+    __syncthreads();
+    const bool whole = n_blocks == 1;
+    constexpr int OWN = MT / kWarps;             // tiles of each column block that a warp finishes: its lanes' elements are neighbours
+    float4 sum[NT][OWN];
+    float top[NT][2], norm[NT][2];
+    auto fold = [&](auto&& ml, auto&& o, int n) {             // n results: ml(i, column) -> (max, sum), o(i, tile) -> float4
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          top[nt][x] = -INFINITY;
+          norm[nt][x] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) sum[nt][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < n; ++k)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) top[nt][x] = fmaxf(top[nt][x], ml(k, nt * 8 + 2 * t + x).x);
+        for (int k = 0; k < n; ++k) {
+          float f[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float2 one = ml(k, nt * 8 + 2 * t + x);
+            f[x] = one.x == -INFINITY && one.y == 0.f ? 0.f : exp2f(one.x == -INFINITY ? 0.f : one.x - top[nt][x]);
+            norm[nt][x] += one.y * f[x];
+          }
+#pragma unroll
+          for (int i = 0; i < OWN; ++i) {
+            const float4 v = o(k, nt * MT + warp * OWN + i);
+            if (f[0] != 0.f) { sum[nt][i].x += v.x * f[0]; sum[nt][i].z += v.z * f[0]; }
+            if (f[1] != 0.f) { sum[nt][i].y += v.y * f[1]; sum[nt][i].w += v.w * f[1]; }
+          }
+        }
+      }
+    };
+    fold([&](int k, int column) { return *reinterpret_cast<const float2*>(merge_ml + (k * COLS + column) * 2); },
+         [&](int k, int tile) { return merge_o[(k * NT * MT + tile) * 32 + lane]; }, kWarps);
+    bool finish = whole;
+    if (!whole) {
+      // A block's share begins inside one pair and ends inside another at most: two places of its own.
+      auto place = [&](int b, bool its_first) { return p.part + ((size_t)b * 2 + (its_first ? 0 : 1)) * PART_FLOATS; };
+      float* mine = place(blockIdx.x, first_of_block);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) reinterpret_cast<float4*>(mine)[(nt * MT + warp * OWN + i) * 32 + lane] = sum[nt][i];
+        if (warp == 0 && g == 0)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            *reinterpret_cast<float2*>(mine + NT * MT * 128 + (nt * 8 + 2 * t + x) * 2) = make_float2(top[nt][x], norm[nt][x]);
+      }
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) {                    // (one pair at most goes on from a block to the next: the first block's number is its counter)
+        const bool last = atomicAdd(p.tickets + first_block, 1) == n_blocks - 1;
+        if (last) p.tickets[first_block] = 0;
+        *s_last = last;
+      }
+      __syncthreads();
+      finish = *s_last != 0;
+      if (finish) {
+        __threadfence();
+        const bool begins = pieces > 0 || share(first_block) >= first;      // whether the pair is the first of its first block
+        auto piece = [&](int k) { return place(first_block + k, k > 0 || begins); };
+        fold([&](int k, int column) { return __ldcg(reinterpret_cast<const float2*>(piece(k) + NT * MT * 128 + column * 2)); },
+             [&](int k, int tile) { return __ldcg(reinterpret_cast<const float4*>(piece(k)) + tile * 32 + lane); }, n_blocks);
+      }
+    }
+    if (finish) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int column = column0 + nt * 8 + 2 * t + x;
+          if (column >= n_rows) continue;
+          const int token = tok0 + column / p.per, head = kvh * p.per + column % p.per;
+          const float inv = norm[nt][x] == 0.f ? 0.f : 1.f / norm[nt][x];
+          T* dst = static_cast<T*>(p.out) + (long long)token * p.out_stride + (long long)head * DIM + g * (DIM / 8) + warp * OWN * 2;
+#pragma unroll
+          for (int i = 0; i < OWN; ++i) {
+            const float a = x ? sum[nt][i].y : sum[nt][i].x, b = x ? sum[nt][i].w : sum[nt][i].z;
+            dst[2 * i] = from_f32<T>(a * inv);
+            dst[2 * i + 1] = from_f32<T>(b * inv);
+          }
+          if (p.lse && warp == 0 && g == 0) p.lse[(size_t)token * p.nh + head] = (top[nt][x] + log2f(norm[nt][x])) * 0.693147180559945309f;
+        }
+      }
+    }
+    __syncthreads();                             // the merge's memory is free again
+  }
+}
+
+template <typename T, int DIM, int NT, int PARTS>
+int launch_mma(const MmaParams& p, int grid, cudaStream_t stream) {
+  constexpr int MT = DIM / 16;
+  const size_t smem = sizeof(Stage<DIM>) * kStages * kWarps + (size_t)kWarps * NT * MT * 512 + (size_t)kWarps * 8 * NT * 8 + 16 +
+                      (size_t)(p.n_requests + 1) * 12;
+  auto* kernel = packed_attention_mma_kernel<T, DIM, NT, PARTS>;
+  static int configured[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return YALIS_ERR_LAUNCH;
+  if (smem > 200 * 1024) return YALIS_ERR_SHAPE;
+  if (dev < 0 || dev >= 64 || configured[dev] < (int)smem) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return YALIS_ERR_LAUNCH;
+    if (dev >= 0 && dev < 64) configured[dev] = (int)smem;
+  }
+  return yalis_launch(kernel, dim3(grid), dim3(kThreads), smem, stream, p);
+}
+
+}  // namespace
+
+// Blocks of the launch (the same for every step of these shapes), and the floats of scratch memory that it needs.
+YALIS_API int yalis_packed_attention_mma_blocks(int dtype, int dim, int columns) {
+  return yalis_sm_count() * (dtype == YALIS_BF16 && columns <= 8 ? 4 : 2);
+}
+YALIS_API long long yalis_packed_attention_mma_scratch_floats(int blocks, int dim, int columns) {
+  const int nt = columns <= 8 ? 1 : 2;
+  return (long long)blocks * 2 * (nt * (dim / 16) * 128 + 16 * nt);
+}
+
+// `columns`: 8 or 16, the query rows of a pair (float32: 8).
+YALIS_API int yalis_packed_attention_mma(const void* q, long long q_stride, int dtype, void* out, long long out_stride, void* k_codes,
+                                         void* v_codes, void* words, int num_pages, int page_size, int g, int dim, const int32_t* positions,
+                                         const int32_t* q_start, const int32_t* block_table, int table_width, int n_requests, int nh,
+                                         int columns, int q_vector, int only_single, float scale, int window, float* lse, int blocks,
+                                         float* scratch, int32_t* tickets, int32_t* error, cudaStream_t stream) {
+  if ((dim != 64 && dim != 128) || nh % g || n_requests > 4096 || blocks < 1) return YALIS_ERR_SHAPE;
+  if (n_requests <= 0) return YALIS_OK;
+  MmaParams p = {};
+  p.q = q; p.q_stride = q_stride; p.out = out; p.out_stride = out_stride;
+  p.positions = positions; p.q_start = q_start; p.block_table = block_table; p.table_width = table_width;
+  p.n_requests = n_requests; p.nh = nh; p.per = nh / g; p.window = window; p.q_vector = q_vector; p.only_single = only_single;
+  p.page_shift = -1;
+  if ((page_size & (page_size - 1)) == 0)
+    for (p.page_shift = 0; 1 << p.page_shift < page_size;) ++p.page_shift;
+  p.scale_log2 = scale * 1.4426950408889634f; p.lse = lse; p.part = scratch; p.tickets = tickets; p.error = error;
+  p.pages = {static_cast<uint32_t*>(k_codes), static_cast<uint32_t*>(v_codes), static_cast<uint32_t*>(words), num_pages, page_size, g, dim};
+  if (dtype == YALIS_BF16) {
+    if (columns == 8) return dim == 64 ? launch_mma<__nv_bfloat16, 64, 1, 1>(p, blocks, stream) : launch_mma<__nv_bfloat16, 128, 1, 1>(p, blocks, stream);
+    if (columns == 16) return dim == 64 ? launch_mma<__nv_bfloat16, 64, 2, 1>(p, blocks, stream) : launch_mma<__nv_bfloat16, 128, 2, 1>(p, blocks, stream);
+  }
+  if (dtype == YALIS_F32 && columns == 8)
+    return dim == 64 ? launch_mma<float, 64, 1, 3>(p, blocks, stream) : launch_mma<float, 128, 1, 3>(p, blocks, stream);
+  return YALIS_ERR_DTYPE;
+}

@@ -14,7 +14,21 @@ from typing import Optional, Sequence, Tuple
 
 import torch
 
-from ._lib import KernelError, check, dtype_code, f32, i32, i64, lib, need, need_cuda, ptr, stream
+from ._lib import F32, KernelError, check, dtype_code, lib, need, stream
+
+_TYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
+_entries = {}
+
+
+def _entry(name: str, signature: str, result=ctypes.c_int):
+    """The library's function with its argument types set once: plain numbers are handed over as they are (these calls are made
+    for every layer of a step, and converting thirty arguments one by one takes longer than the smaller kernels run)."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = getattr(lib(), name)
+        fn.argtypes, fn.restype = [_TYPES[c] for c in signature], result
+        _entries[name] = fn
+    return fn
 
 
 @dataclass(frozen=True)
@@ -53,31 +67,78 @@ class PackedPages:
 
 def _need_here(name: str, *tensors: Optional[torch.Tensor]) -> None:
     """Every tensor on the current device, whose stream the kernels are launched on."""
-    need_cuda(name, *tensors)
-    here = torch.cuda.current_device()
-    need(all(t is None or t.device.index == here for t in tensors), name, "every tensor must be on the current device")
+    here = -1
+    for t in tensors:
+        if t is not None:
+            at = t.get_device()
+            if at < 0:
+                raise KernelError(f"{name}: every tensor must be on the GPU (there is no CPU path)")
+            if at != here and (here >= 0 or at != torch.cuda.current_device()):
+                raise KernelError(f"{name}: every tensor must be on the current device")
+            here = at
+
+
+def _address(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _pages_arguments(name: str, pages: PackedPages):
-    k, v, words = pages.pools()
-    need(k.dtype == v.dtype == torch.uint8 and k.dim() == 4 and k.shape == v.shape and k.is_contiguous() and v.is_contiguous(), name,
-         "codes must be contiguous uint8 [pages, kv_heads, page_size, head_dim / 2]")
-    need(words.dtype == torch.int16 and words.shape == k.shape[:3] + (2,) and words.is_contiguous(), name,
-         "words must be contiguous int16 [pages, kv_heads, page_size, 2]")
-    need(pages.head_dim % 8 == 0 and 8 <= pages.head_dim <= 256, name, f"head_dim {pages.head_dim} must be a multiple of 8 up to 256")
-    need(all(t.data_ptr() % 16 == 0 for t in (k, v, words)), name, "pools must start on 16-byte boundaries")
-    return (ptr(k), ptr(v), ptr(words), i32(k.shape[0]), i32(k.shape[2]), i32(k.shape[1]), i32(pages.head_dim))
+    k, v, words = pages.k, pages.v, pages.words
+    shape = k.shape
+    if not (k.dtype is torch.uint8 and v.dtype is torch.uint8 and len(shape) == 4 and v.shape == shape and k.is_contiguous() and v.is_contiguous()):
+        raise KernelError(f"{name}: codes must be contiguous uint8 [pages, kv_heads, page_size, head_dim / 2]")
+    num_pages, g, page_size, half = shape
+    if not (words.dtype is torch.int16 and words.shape == (num_pages, g, page_size, 2) and words.is_contiguous()):
+        raise KernelError(f"{name}: words must be contiguous int16 [pages, kv_heads, page_size, 2]")
+    if half % 4 or not 4 <= half <= 128:
+        raise KernelError(f"{name}: head_dim {2 * half} must be a multiple of 8 up to 256")
+    if num_pages * g * page_size >= 1 << 31:
+        raise KernelError(f"{name}: {num_pages} pages of {g} x {page_size} rows are 2^31 rows or more")
+    at = (k.data_ptr(), v.data_ptr(), words.data_ptr())
+    if (at[0] | at[1] | at[2]) % 16:
+        raise KernelError(f"{name}: pools must start on 16-byte boundaries")
+    return at + (num_pages, page_size, g, 2 * half)
 
 
 def _check_index(name: str, n: int, block_table: torch.Tensor, *per_token: torch.Tensor) -> None:
     for t in per_token:
-        need(t.dtype == torch.int32 and t.shape == (n,) and t.is_contiguous(), name, "positions/req_of_token: int32 [N]")
-    need(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.is_contiguous(), name,
-         "block_table must be contiguous int32 [R, width]")
+        if not (t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous()):
+            raise KernelError(f"{name}: positions/req_of_token: int32 [N]")
+    if not (block_table.dtype is torch.int32 and block_table.dim() == 2 and block_table.is_contiguous()):
+        raise KernelError(f"{name}: block_table must be contiguous int32 [R, width]")
 
 
 def _check_flag(name: str, error_flag: Optional[torch.Tensor]) -> None:
     need(error_flag is None or (error_flag.dtype == torch.int32 and error_flag.numel() >= 1), name, "the error word must be int32")
+
+
+_counters_of_stream = {}
+
+
+def _counters(n: int, device: torch.device) -> torch.Tensor:
+    """Zeroed int32 counters, which every launch leaves at zero: one buffer per stream, whose launches run one after the other; a
+    recording, which may be replayed on any stream, gets its own with every launch."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(n, dtype=torch.int32, device=device)
+    key = (device.index, stream().value)
+    held = _counters_of_stream.get(key)
+    if held is None or held.numel() < n:
+        held = _counters_of_stream[key] = torch.zeros(max(n, 2048), dtype=torch.int32, device=device)
+    return held
+
+
+_mma_launches = {}
+
+
+def _mma_launch(device: torch.device, code: int, dim: int, columns: int) -> Tuple[int, int]:
+    """(blocks, floats of scratch memory) of the tensor-core kernel."""
+    key = (device.index, code, dim, columns)
+    found = _mma_launches.get(key)
+    if found is None:
+        blocks = _entry("yalis_packed_attention_mma_blocks", "iii")(code, dim, columns)
+        floats = _entry("yalis_packed_attention_mma_scratch_floats", "iii", ctypes.c_longlong)(blocks, dim, columns)
+        found = _mma_launches[key] = (blocks, floats)
+    return found
 
 
 def packed_kv_write(k: torch.Tensor, v: torch.Tensor, pages: PackedPages, positions: torch.Tensor, req_of_token: torch.Tensor,
@@ -88,16 +149,19 @@ def packed_kv_write(k: torch.Tensor, v: torch.Tensor, pages: PackedPages, positi
     word's bit.  Rows with a NaN, an infinity or a magnitude above 2^120 read back as NaN throughout."""
     name = "packed_kv_write"
     _need_here(name, k, v, pages.k, pages.v, pages.words, positions, req_of_token, block_table, error_flag)
-    held, n, width = _pages_arguments(name, pages), k.shape[0], pages.num_kv_heads * pages.head_dim
-    need(k.dtype == v.dtype and k.dim() == 2 and k.shape == v.shape == (n, width) and k.stride(1) == v.stride(1) == 1, name,
-         "k and v must be [N, kv_heads * head_dim] of one dtype with unit inner stride")
-    _check_index(name, n, block_table, positions, req_of_token)
+    held, shape = _pages_arguments(name, pages), k.shape
+    if not (k.dtype is v.dtype and len(shape) == 2 and v.shape == shape and shape[1] == held[5] * held[6] and k.stride(1) == v.stride(1) == 1):
+        raise KernelError(f"{name}: k and v must be [N, kv_heads * head_dim] of one dtype with unit inner stride")
+    _check_index(name, shape[0], block_table, positions, req_of_token)
     _check_flag(name, error_flag)
-    code, size = dtype_code(k.dtype), 8 * k.element_size()
-    vector = all(t.data_ptr() % min(size, 16) == 0 and (t.stride(0) * t.element_size()) % min(size, 16) == 0 for t in (k, v))
-    check(lib().yalis_packed_rows(i32(1), ptr(k), ptr(v), i64(k.stride(0)), i64(v.stride(0)), i32(code), *held, ptr(positions),
-                                  ptr(req_of_token), ptr(block_table), i32(block_table.shape[1]), i32(n), i32(int(vector)), ptr(error_flag),
-                                  stream()), name)
+    code, k_at, v_at, k_step, v_step, size = dtype_code(k.dtype), k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), k.element_size()
+    vector = (k_at | v_at | k_step * size | v_step * size) % 16 == 0
+    check(_rows_entry()(1, k_at, v_at, k_step, v_step, code, *held, positions.data_ptr(), req_of_token.data_ptr(), block_table.data_ptr(),
+                        block_table.shape[1], shape[0], vector, _address(error_flag), stream()), name)
+
+
+def _rows_entry():
+    return _entry("yalis_packed_rows", "ippllipppiiiipppiiipp")
 
 
 def packed_kv_read(pages: PackedPages, positions: torch.Tensor, req_of_token: torch.Tensor, block_table: torch.Tensor,
@@ -107,12 +171,13 @@ def packed_kv_read(pages: PackedPages, positions: torch.Tensor, req_of_token: to
     raise the error word's bit) read as zeros."""
     name = "packed_kv_read"
     _need_here(name, pages.k, pages.v, pages.words, positions, req_of_token, block_table, error_flag)
-    held, n, width, code = _pages_arguments(name, pages), positions.shape[0], pages.num_kv_heads * pages.head_dim, dtype_code(dtype)
+    held, n, code = _pages_arguments(name, pages), positions.shape[0], dtype_code(dtype)
     _check_index(name, n, block_table, positions, req_of_token)
     _check_flag(name, error_flag)
-    k, v = (torch.empty((n, width), dtype=dtype, device=positions.device) for _ in range(2))
-    check(lib().yalis_packed_rows(i32(0), ptr(k), ptr(v), i64(width), i64(width), i32(code), *held, ptr(positions), ptr(req_of_token),
-                                  ptr(block_table), i32(block_table.shape[1]), i32(n), i32(1), ptr(error_flag), stream()), name)
+    width = held[5] * held[6]
+    k, v = torch.empty((n, width), dtype=dtype, device=positions.device), torch.empty((n, width), dtype=dtype, device=positions.device)
+    check(_rows_entry()(0, k.data_ptr(), v.data_ptr(), width, width, code, *held, positions.data_ptr(), req_of_token.data_ptr(),
+                        block_table.data_ptr(), block_table.shape[1], n, True, _address(error_flag), stream()), name)
     return k, v
 
 
@@ -133,30 +198,47 @@ def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tenso
     Scores, weights and sums are float32, and with float32 queries so is every product."""
     name = "packed_attention"
     _need_here(name, q, pages.k, pages.v, pages.words, positions, q_start, block_table, weight_sums, out, error_flag)
-    held, n, r, dim, g = _pages_arguments(name, pages), q.shape[0], q_start.numel() - 1, pages.head_dim, pages.num_kv_heads
-    code = dtype_code(q.dtype)
-    need(num_heads >= 1 and num_heads % g == 0, name, "heads must be a multiple of kv_heads")
-    need(q.dim() == 2 and q.stride(1) == 1 and q.shape[1] >= num_heads * dim, name, "q must be [N, >= heads*head_dim] with unit inner stride")
+    held = _pages_arguments(name, pages)
+    page_size, g, dim = held[4:]
+    code, n, r, width = dtype_code(q.dtype), q.shape[0], q_start.shape[0] - 1 if q_start.dim() == 1 else -1, num_heads * dim
+    if num_heads < 1 or num_heads % g:
+        raise KernelError(f"{name}: heads must be a multiple of kv_heads")
+    if q.dim() != 2 or q.stride(1) != 1 or q.shape[1] < width:
+        raise KernelError(f"{name}: q must be [N, >= heads*head_dim] with unit inner stride")
     _check_index(name, n, block_table, positions)
-    need(q_start.dtype == torch.int32 and q_start.dim() == 1 and q_start.is_contiguous() and r >= 0, name, "q_start must be int32 [R+1]")
+    if q_start.dtype is not torch.int32 or r < 0 or not q_start.is_contiguous():
+        raise KernelError(f"{name}: q_start must be int32 [R+1]")
     need(block_table.shape[0] >= r, name, "block_table has fewer rows than requests")
     need(max_q_len >= 0 and (window is None or window > 0), name, "max_q_len and the window must be positive")
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
     need(math.isfinite(scale), name, "the scale must be finite")
-    reach = block_table.shape[1] * pages.page_size
+    reach = block_table.shape[1] * page_size
     max_kv_len = reach if max_kv_len is None else min(int(max_kv_len), reach)
-    need(weight_sums is None or (weight_sums.dtype == torch.float32 and weight_sums.shape == pages.k.shape[:3] and weight_sums.is_contiguous()),
-         name, "weight_sums must be contiguous float32 [pages, kv_heads, page_size]")
+    if weight_sums is not None:
+        need(weight_sums.dtype == torch.float32 and weight_sums.shape == pages.k.shape[:3] and weight_sums.is_contiguous(), name,
+             "weight_sums must be contiguous float32 [pages, kv_heads, page_size]")
     _check_flag(name, error_flag)
     if out is None:
-        out = torch.empty((n, num_heads * dim), dtype=q.dtype, device=q.device)
-    need(out.shape == (n, num_heads * dim) and out.dtype == q.dtype and out.stride(1) == 1, name, "bad out tensor")
+        out = torch.empty((n, width), dtype=q.dtype, device=q.device)
+    need(out.shape == (n, width) and out.dtype is q.dtype and out.stride(1) == 1, name, "bad out tensor")
     lse = torch.empty((n, num_heads), dtype=torch.float32, device=q.device) if weight_sums is not None else None
-    check(lib().yalis_packed_attention_general(
-        ptr(q), i64(q.stride(0)), i32(code), ptr(out), i64(out.stride(0)), *held, ptr(positions), ptr(q_start), ptr(block_table),
-        i32(block_table.shape[1]), i32(r), i32(n), i32(max_kv_len), i32(num_heads), f32(scale), i32(window or 0), ptr(lse), ptr(weight_sums),
-        ptr(error_flag), stream()), name)
+    at, steps, raw = (positions.data_ptr(), q_start.data_ptr(), block_table.data_ptr(), block_table.shape[1], r), (q.stride(0), out.stride(0)), stream()
+    if dim in (64, 128) and r <= 4096:
+        columns = 8 if code == F32 or max_q_len * (num_heads // g) <= 8 else 16
+        blocks, floats = _mma_launch(q.device, code, dim, columns)
+        scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
+        vector = (q.data_ptr() | steps[0] * q.element_size()) % 16 == 0
+        check(_entry("yalis_packed_attention_mma", "plipl" + "pppiiii" + "pppii" + "iiiifipipppp")(
+            q.data_ptr(), steps[0], code, out.data_ptr(), steps[1], *held, *at, num_heads, columns, vector, False, scale, window or 0,
+            _address(lse), blocks, scratch.data_ptr(), _counters(blocks, q.device).data_ptr(), _address(error_flag), raw), name)
+    else:
+        check(_entry("yalis_packed_attention_general", "plipl" + "pppiiii" + "pppii" + "iifippp")(
+            q.data_ptr(), steps[0], code, out.data_ptr(), steps[1], *held, *at, n, num_heads, scale, window or 0, _address(lse),
+            _address(error_flag), raw), name)
+    if weight_sums is not None:
+        check(_entry("yalis_packed_weight_sums_general", "pli" + "pppiiii" + "pppii" + "iifippp")(
+            q.data_ptr(), steps[0], code, *held, *at, max_kv_len, num_heads, scale, window or 0, lse.data_ptr(), weight_sums.data_ptr(), raw), name)
     return out
 
 
@@ -178,21 +260,20 @@ def evict_tokens(pools: Sequence[torch.Tensor], weight_sums: torch.Tensor, lengt
     need(len(pools) <= 4, name, "at most four pools")
     need(weight_sums.dtype == torch.float32 and weight_sums.dim() == 3 and weight_sums.is_contiguous(), name,
          "weight_sums must be contiguous float32 [pages, kv_heads, page_size]")
-    row_bytes = []
-    for p in pools:
-        need(p.dim() >= 3 and p.shape[:3] == weight_sums.shape and p.is_contiguous(), name, "pools must be contiguous [pages, kv_heads, page_size, ...]")
-        row_bytes.append(p[0, 0, 0].numel() * p.element_size() if p.numel() else 0)
-        need(row_bytes[-1] % 2 == 0 and p.data_ptr() % 2 == 0, name, "rows of a pool must be whole pairs of bytes")
-    r = lengths.shape[0]
+    pages, g, page_size = shape = weight_sums.shape
+    addresses, row_bytes = (ctypes.c_void_p * 4)(), (ctypes.c_int * 4)()
+    for i, p in enumerate(pools):
+        need(p.dim() >= 3 and p.shape[:3] == shape and p.is_contiguous(), name, "pools must be contiguous [pages, kv_heads, page_size, ...]")
+        addresses[i], row_bytes[i] = p.data_ptr(), p.numel() // max(1, pages * g * page_size) * p.element_size()
+        need(row_bytes[i] % 2 == 0 and p.data_ptr() % 2 == 0, name, "rows of a pool must be whole pairs of bytes")
     need(lengths.dtype == torch.int32 and lengths.dim() == 1 and lengths.is_contiguous(), name, "lengths must be int32 [R]")
+    r = lengths.shape[0]
     _check_index(name, 0, block_table)
     _check_flag(name, error_flag)
     need(block_table.shape[0] >= r, name, "block_table has fewer rows than requests")
     need(keep >= 1 and 0 <= recent <= keep, name, "keep must be at least 1 and recent between 0 and keep")
-    pages, g, page_size = weight_sums.shape
     kept = torch.empty((r, g, keep), dtype=torch.int32, device=lengths.device)
-    check(lib().yalis_evict_tokens(
-        (ctypes.c_void_p * 4)(*[p.data_ptr() for p in pools]), (ctypes.c_int * 4)(*row_bytes), i32(len(pools)), ptr(weight_sums), ptr(lengths),
-        ptr(block_table), i32(block_table.shape[1]), i32(page_size), i32(pages), i32(g), i32(r), i32(keep), i32(recent), ptr(kept),
-        ptr(error_flag), stream()), name)
+    check(_entry("yalis_evict_tokens", "ppippp" + "iiiiiii" + "ppp")(
+        ctypes.addressof(addresses), ctypes.addressof(row_bytes), len(pools), weight_sums.data_ptr(), lengths.data_ptr(), block_table.data_ptr(),
+        block_table.shape[1], page_size, pages, g, r, keep, recent, kept.data_ptr(), _address(error_flag), stream()), name)
     return kept

@@ -8,8 +8,9 @@
 //   S^T [keys, columns] = C_K [16 keys x 16 elements] q^T       O^T [elements, columns] += C_V^T [16 elements x 16 keys] W^T
 //
 // The order of a product's inner index is free as long as both operands agree, so a lane takes neighbouring codes: with a word of
-// eight codes, (w >> s) & 0x00780078 | 0x41804180 is the pair 16 + c_i, 16 + c_(i + 4) in bfloat16, from which 16 + zero is taken
-// away (exact).  Elements of a V row pair up by key instead: the 16-bit halves of two keys' words are put side by side first.  The
+// eight codes, (w >> s) & 0x00780078 | 0x41804180 is the pair 16 + c_i, 16 + c_(i + 4) in bfloat16.  For values 16 + zero is taken
+// away from the pairs (exact); for keys (16 + zero) sum(q) is taken away from the product, which is two instructions a score in
+// place of 64 a chunk (with float32 queries the pairs lose it too: the difference of two large sums would show).  Elements of a V row pair up by key instead: the 16-bit halves of two keys' words are put side by side first.  The
 // scores' accumulators, times step, are the softmax's scores; the weights times the values' steps are rounded to bfloat16
 // (float32: in three parts) and turned from accumulator layout to operand layout by movmatrix.
 //
@@ -18,6 +19,8 @@
 // dealt to a fixed grid by the step's lengths (choose_deal), so that a recorded launch serves other lengths too; a pair cut between
 // blocks is added up, in the blocks' order, by whichever of them comes last (a counter per pair, left at zero).  Nothing waits for
 // another block.
+#include <type_traits>
+
 #include "packed.cuh"
 
 namespace {
@@ -25,6 +28,7 @@ namespace {
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kChunk = 32;     // keys of a chunk
 constexpr int kStages = 2;
+constexpr float kNone = -1e30f;  // the maximum of no scores
 constexpr float kLazy = 8.f;   // how far (log2) scores may rise above the maximum in use before the output is rescaled
 
 struct MmaParams {
@@ -36,6 +40,7 @@ struct MmaParams {
   const int32_t* q_start;      // [R + 1]
   const int32_t* block_table;  // [R, table_width]
   int table_width, n_requests, nh, per, window, page_shift;
+  int together;                // 2: a chunk never lies in two pages; 1: the rows that one copy instruction of a warp covers do not
   int q_vector;                // 1: rows of q start on 16-byte boundaries
   int only_single;             // 1: requests that bring more than one token are left to another kernel
   float scale_log2;
@@ -77,10 +82,14 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return r;
 }
 // 16 + codes i and i + 4 of the eight in w as bfloat16.
+// One three-input operation: a register has to hold 16, 16 (an instruction takes one constant; with two written out the compiler
+// made two instructions of it, which was a quarter of all that the kernel issued).
 template <int I>
-__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t sixteens) {
   const uint32_t at = I == 0 ? w << 3 : w >> (I == 0 ? 0 : 4 * I - 3);
-  return (at & 0x00780078u) | 0x41804180u;
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x00780078, %2, 0xEA;" : "=r"(r) : "r"(at), "r"(sixteens));       // (at & mask) | sixteens
+  return r;
 }
 // Parts of a float32 pair in bfloat16: PARTS 1 rounds it; 3 hold every bit.
 template <int PARTS>
@@ -115,6 +124,13 @@ struct Stage {
   uint32_t words[kChunk];
 };
 
+// What a key's word says, as the products use it: the key's step times scale, 16 + its zero, the value's step, 16 + its zero.
+// A key that is not there has steps of 0 (a row that is there has at least 2^-126).
+__device__ __forceinline__ float4 terms_of(uint32_t word, float scale_log2) {
+  return make_float4(step_of(word & 0xFFFFu) * scale_log2, __uint_as_float(0x41800000u | (word & 15u) << 19), step_of(word >> 16),
+                     __uint_as_float(0x41800000u | (word >> 16 & 15u) << 19));
+}
+
 // How a step's chunks are dealt out, by what the slowest block then has to do, counted in chunks:
 //   pieces k > 0: every pair to k blocks in equal pieces, one piece a block;
 //   0: all chunks of all pairs, laid end to end, in equal shares; a block's share begins and ends inside pairs that others share.
@@ -142,9 +158,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
   constexpr int PIECES = DIM / 32;             // 16-byte pieces of a row
   constexpr int COPIES = PIECES;               // of K (and as many of V) that a lane asks for per chunk
   constexpr int PART_FLOATS = NT * MT * 128 + 2 * COLS;
+  constexpr bool SIGNED = PARTS > 1;
   extern __shared__ __align__(128) unsigned char smem[];
   Stage<DIM>* ring = reinterpret_cast<Stage<DIM>*>(smem) + (threadIdx.x >> 5) * kStages;
-  float4* merge_o = reinterpret_cast<float4*>(smem + sizeof(Stage<DIM>) * kStages * kWarps);       // [kWarps][NT * MT][32]
+  float4* terms = reinterpret_cast<float4*>(smem + sizeof(Stage<DIM>) * kStages * kWarps) + (threadIdx.x >> 5) * kChunk;
+  float4* merge_o = reinterpret_cast<float4*>(smem + sizeof(Stage<DIM>) * kStages * kWarps + kWarps * kChunk * 16);   // [kWarps][NT * MT][32]
   float* merge_ml = reinterpret_cast<float*>(merge_o + kWarps * NT * MT * 32);                     // [kWarps][COLS][2]
   int* s_last = reinterpret_cast<int*>(merge_ml + kWarps * COLS * 2);
   int* s_deal = s_last + 1;                                                                        // pieces, blocks
@@ -152,6 +170,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
   int* cum_pairs = reinterpret_cast<int*>(cum + p.n_requests + 1);                                 // [R + 1] pairs before it
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint32_t sixteens;
+  asm volatile("mov.b32 %0, 0x41804180;" : "=r"(sixteens));
   pdl_wait();
 
   // ---- the chunks of every request (KV heads, blocks of columns and chunks of 32 keys), their running sum, this block's share ----
@@ -249,6 +269,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
     const int tok0 = p.q_start[req];
     const int32_t* table_row = p.block_table + (size_t)req * p.table_width;
     uint32_t qf[NT][2 * W][2][PARTS];
+    float q_sum[NT][2];                          // sum(q) of the columns 2t, 2t + 1
     int see_hi[NT][2], see_lo[NT][2], all_hi = 0x7fffffff, all_lo = 0, any_hi = -1, any_lo = 0x7fffffff;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -256,6 +277,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       const bool real = row < n_rows;
       const int token = tok0 + (real ? row / p.per : 0), head = kvh * p.per + (real ? row % p.per : 0);
       const T* src = static_cast<const T*>(p.q) + (long long)token * p.q_stride + (long long)head * DIM + t * (DIM / 4);
+      float own = 0.f;
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         float x[8];
@@ -271,8 +293,15 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
           for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(src[8 * w + i]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) parts_of<PARTS>(x[i], x[i + 4], qf[nt][2 * w + (i >> 1)][i & 1]);
+        for (int i = 0; i < 4; ++i) {
+          parts_of<PARTS>(x[i], x[i + 4], qf[nt][2 * w + (i >> 1)][i & 1]);
+          own += x[i] + x[i + 4];
+        }
       }
+      own += __shfl_xor_sync(0xffffffffu, own, 1);
+      own += __shfl_xor_sync(0xffffffffu, own, 2);             // column g, in its four lanes
+#pragma unroll
+      for (int e = 0; e < 2; ++e) q_sum[nt][e] = __shfl_sync(0xffffffffu, own, (2 * t + e) * 4);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int column = column0 + nt * 8 + 2 * t + e;
@@ -299,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
     float m[NT][2], l[NT][2], acc[NT][MT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = -INFINITY;
+      m[nt][0] = m[nt][1] = kNone;
       l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < MT; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
@@ -327,14 +356,39 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
     auto ask = [&](int stage, int row) {         // rows that are not there are left as they are: their word says so
       Stage<DIM>& st = ring[stage];
       const uint32_t k_at = smem_u32(st.k), v_at = smem_u32(st.v);
-#pragma unroll
-      for (int i = 0; i < COPIES; ++i) {
-        const int r = i * (32 / PIECES) + lane / PIECES, piece = lane % PIECES;
-        const int from = __shfl_sync(0xffffffffu, row, r);
+      if (p.together == 2) {                     // (rows behind the last key are copied too, here and below)
+        const int from = __shfl_sync(0xffffffffu, row, 0);
         if (from >= 0) {
-          const size_t byte = (size_t)from * (DIM / 2) + piece * 16;
-          copy16(k_at + piece_at<DIM>(r, piece), reinterpret_cast<const unsigned char*>(p.pages.k) + byte);
-          copy16(v_at + piece_at<DIM>(r, piece), reinterpret_cast<const unsigned char*>(p.pages.v) + byte);
+          const uint32_t own = piece_at<DIM>(lane / PIECES, lane % PIECES);
+          const size_t byte = (size_t)from * (DIM / 2) + lane * 16;
+          const unsigned char *k_from = reinterpret_cast<const unsigned char*>(p.pages.k) + byte, *v_from = reinterpret_cast<const unsigned char*>(p.pages.v) + byte;
+#pragma unroll
+          for (int i = 0; i < COPIES; ++i) {
+            copy16(k_at + own + i * 512, k_from + i * 512);
+            copy16(v_at + own + i * 512, v_from + i * 512);
+          }
+        }
+      } else if (p.together) {                   // a lane's pieces are neighbours of the group's first row
+        const uint32_t own = piece_at<DIM>(lane / PIECES, lane % PIECES);
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i) {
+          const int from = __shfl_sync(0xffffffffu, row, i * (32 / PIECES));
+          if (from >= 0) {
+            const size_t byte = (size_t)from * (DIM / 2) + lane * 16;
+            copy16(k_at + own + i * 512, reinterpret_cast<const unsigned char*>(p.pages.k) + byte);
+            copy16(v_at + own + i * 512, reinterpret_cast<const unsigned char*>(p.pages.v) + byte);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i) {
+          const int r = i * (32 / PIECES) + lane / PIECES, piece = lane % PIECES;
+          const int from = __shfl_sync(0xffffffffu, row, r);
+          if (from >= 0) {
+            const size_t byte = (size_t)from * (DIM / 2) + piece * 16;
+            copy16(k_at + piece_at<DIM>(r, piece), reinterpret_cast<const unsigned char*>(p.pages.k) + byte);
+            copy16(v_at + piece_at<DIM>(r, piece), reinterpret_cast<const unsigned char*>(p.pages.v) + byte);
+          }
         }
       }
       if (row >= 0) copy4(smem_u32(&st.words[lane]), p.pages.words + row);
@@ -354,15 +408,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       __syncwarp();
       const Stage<DIM>& st = ring[stage];
       const int key0 = first_key + c * kChunk;
+      terms[lane] = terms_of(st.words[lane], p.scale_log2);
+      __syncwarp();
 
-      // ---- scores of 32 keys ----
+      // ---- products with 32 keys ----
       float sc[NT][2][4];
-      uint32_t word[2][2];
+      float4 term[2][2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int ra = half * 16 + key_of_row<DIM>(g), rb = ra + 8;
-        word[half][0] = st.words[ra];
-        word[half][1] = st.words[rb];
+        term[half][0] = terms[ra];
+        term[half][1] = terms[rb];
         uint32_t wa[W], wb[W];
         if constexpr (DIM == 128) {
           *reinterpret_cast<uint4*>(wa) = *reinterpret_cast<const uint4*>(st.k + piece_at<DIM>(ra, t));
@@ -371,13 +427,20 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
           *reinterpret_cast<uint2*>(wa) = *reinterpret_cast<const uint2*>(st.k + ra * (DIM / 2) + t * 8);
           *reinterpret_cast<uint2*>(wb) = *reinterpret_cast<const uint2*>(st.k + rb * (DIM / 2) + t * 8);
         }
-        const uint32_t za = ((word[half][0] & 15u) << 3 | 0x4180u) * 0x10001u, zb = ((word[half][1] & 15u) << 3 | 0x4180u) * 0x10001u;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) sc[nt][half][0] = sc[nt][half][1] = sc[nt][half][2] = sc[nt][half][3] = 0.f;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          const uint32_t lo[4] = {minus(code_pair<0>(wa[w]), za), minus(code_pair<0>(wb[w]), zb), minus(code_pair<1>(wa[w]), za), minus(code_pair<1>(wb[w]), zb)};
-          const uint32_t hi[4] = {minus(code_pair<2>(wa[w]), za), minus(code_pair<2>(wb[w]), zb), minus(code_pair<3>(wa[w]), za), minus(code_pair<3>(wb[w]), zb)};
+          uint32_t lo[4] = {code_pair<0>(wa[w], sixteens), code_pair<0>(wb[w], sixteens), code_pair<1>(wa[w], sixteens), code_pair<1>(wb[w], sixteens)};
+          uint32_t hi[4] = {code_pair<2>(wa[w], sixteens), code_pair<2>(wb[w], sixteens), code_pair<3>(wa[w], sixteens), code_pair<3>(wb[w], sixteens)};
+          if constexpr (SIGNED) {
+            const uint32_t za = __byte_perm(__float_as_uint(term[half][0].y), 0, 0x3232), zb = __byte_perm(__float_as_uint(term[half][1].y), 0, 0x3232);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              lo[i] = minus(lo[i], i & 1 ? zb : za);
+              hi[i] = minus(hi[i], i & 1 ? zb : za);
+            }
+          }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -388,90 +451,123 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
           }
         }
       }
-      // ---- softmax: scores in powers of two, maxima over the chunk ----
-      const bool masked = missing || key0 + kChunk - 1 > all_hi || key0 < all_lo;
-      float most[NT][2];
+      // ---- softmax: scores in powers of two, less the maximum in use ----
+      if constexpr (!SIGNED) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) most[nt][0] = most[nt][1] = -INFINITY;
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float step = step_of(word[half][e]) * p.scale_log2;
-          const int key = key0 + half * 16 + key_of_row<DIM>(g) + 8 * e;
+            for (int i = 0; i < 4; ++i) sc[nt][half][i] = fmaf(-term[half][i >> 1].y, q_sum[nt][i & 1], sc[nt][half][i]);
+      }
+      auto weigh = [&](auto mask) {              // sc: products in, weights times the values' steps out
+        constexpr bool MASK = decltype(mask)::value;
+        float most[NT][2];
+        auto scores = [&](float (&to)[NT][2][4]) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) most[nt][0] = most[nt][1] = -INFINITY;
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) to[nt][half][i] = fmaf(term[half][i >> 1].x, sc[nt][half][i], -m[nt][i & 1]);
+          if constexpr (MASK) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int key = key0 + half * 16 + key_of_row<DIM>(g) + 8 * (i >> 1);
+                  if (!(key <= see_hi[nt][i & 1] && key >= see_lo[nt][i & 1] && term[half][i >> 1].x != 0.f)) to[nt][half][i] = -INFINITY;
+                }
+          }
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) most[nt][i & 1] = fmaxf(most[nt][i & 1], to[nt][half][i]);
+        };
+        float ex[NT][2][4];
+        scores(ex);
+        bool grow = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) grow |= fmaxf(most[nt][0], most[nt][1]) > kLazy;
+        if (__any_sync(0xffffffffu, grow)) {       // seldom after the first chunks: the maximum moves, what was summed is rescaled
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
+            float keep[2];
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              float& v = sc[nt][half][2 * e + x];
-              v *= step;
-              if (masked && !(key <= see_hi[nt][x] && key >= see_lo[nt][x] && word[half][e] != 0u)) v = -INFINITY;
-              most[nt][x] = fmaxf(most[nt][x], v);
+              const float old = m[nt][x];
+              // (the first maximum is taken from scores that kNone has swallowed: once more from the products)
+              float top = most[nt][x] == -INFINITY ? -INFINITY : old == kNone ? -INFINITY : most[nt][x] + old;
+              if (old == kNone) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e)
+                    if (ex[nt][half][2 * e + x] != -INFINITY) top = fmaxf(top, term[half][e].x * sc[nt][half][2 * e + x]);
+              }
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+              m[nt][x] = fmaxf(old, top);
+              keep[x] = exp2_fast(old - m[nt][x]);
+              l[nt][x] *= keep[x];
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              acc[nt][i][0] *= keep[0]; acc[nt][i][1] *= keep[1];
+              acc[nt][i][2] *= keep[0]; acc[nt][i][3] *= keep[1];
             }
           }
+          scores(ex);
         }
-      }
-      bool grow = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) most[nt][x] = fmaxf(most[nt][x], __shfl_xor_sync(0xffffffffu, most[nt][x], o));
-          grow |= most[nt][x] > m[nt][x] + kLazy || (m[nt][x] == -INFINITY && most[nt][x] != -INFINITY);
+            for (int i = 0; i < 4; ++i) {
+              const float e = PARTS == 1 ? exp2_fast(ex[nt][half][i]) : exp2f(ex[nt][half][i]);
+              l[nt][i & 1] += e;
+              sc[nt][half][i] = e * term[half][i >> 1].z;
+            }
+        if constexpr (MASK) {                      // a row that is not seen may hold anything
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (ex[nt][half][i] == -INFINITY) sc[nt][half][i] = 0.f;
         }
-      }
-      if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float keep[2];
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const float next = fmaxf(m[nt][x], most[nt][x]);
-            keep[x] = next == -INFINITY ? 1.f : exp2_fast(m[nt][x] - next);
-            m[nt][x] = next;
-            l[nt][x] *= keep[x];
-          }
-#pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            acc[nt][i][0] *= keep[0]; acc[nt][i][1] *= keep[1];
-            acc[nt][i][2] *= keep[0]; acc[nt][i][3] *= keep[1];
-          }
-        }
-      }
+      };
+      if (missing || key0 + kChunk - 1 > all_hi || key0 < all_lo) weigh(std::true_type());
+      else weigh(std::false_type());
       uint32_t wf[NT][2][2][PARTS];              // [half][keys g, g + 8 of the half]: the weights as the second product's operand
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float base0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], base1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float step = step_of(word[half][e] >> 16);
-            const float s0 = sc[nt][half][2 * e], s1 = sc[nt][half][2 * e + 1];
-            const float e0 = PARTS == 1 ? exp2_fast(s0 - base0) : exp2f(s0 - base0), e1 = PARTS == 1 ? exp2_fast(s1 - base1) : exp2f(s1 - base1);
-            l[nt][0] += e0;
-            l[nt][1] += e1;
-            float w0 = e0 * step, w1 = e1 * step;
-            if (masked) {                        // a row that is not seen may hold anything
-              if (s0 == -INFINITY) w0 = 0.f;
-              if (s1 == -INFINITY) w1 = 0.f;
-            }
             uint32_t part[PARTS];
-            parts_of<PARTS>(w0, w1, part);
+            parts_of<PARTS>(sc[nt][half][2 * e], sc[nt][half][2 * e + 1], part);
 #pragma unroll
             for (int i = 0; i < PARTS; ++i) wf[nt][half][e][i] = transposed(part[i]);
           }
-        }
-      }
       // ---- output ----
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        uint32_t vw[4][U], z[4];
+        uint32_t vw[4][U];
+        float z[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {            // keys of rows 2t, 2t + 1, 2t + 8, 2t + 9
           const int r = half * 16 + key_of_row<DIM>(2 * t + (i & 1) + (i & 2) * 4);
-          z[i] = st.words[r];
+          z[i] = terms[r].w;
           if constexpr (DIM == 128) {
             const uint2 two = *reinterpret_cast<const uint2*>(st.v + piece_at<DIM>(r, g >> 1) + (g & 1) * 8);
             vw[i][0] = two.x;
@@ -480,15 +576,15 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
             vw[i][0] = *reinterpret_cast<const uint32_t*>(st.v + r * (DIM / 2) + g * 4);
           }
         }
-        const uint32_t z01 = ((z[0] >> 13) & 0x78u) | ((z[1] << 3) & 0x00780000u) | 0x41804180u;
-        const uint32_t z23 = ((z[2] >> 13) & 0x78u) | ((z[3] << 3) & 0x00780000u) | 0x41804180u;
+        const uint32_t z01 = __byte_perm(__float_as_uint(z[0]), __float_as_uint(z[1]), 0x7632);
+        const uint32_t z23 = __byte_perm(__float_as_uint(z[2]), __float_as_uint(z[3]), 0x7632);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t a = __byte_perm(vw[0][u], vw[1][u], h ? 0x7632 : 0x5410), b = __byte_perm(vw[2][u], vw[3][u], h ? 0x7632 : 0x5410);
-            const uint32_t f0[4] = {minus(code_pair<0>(a), z01), minus(code_pair<1>(a), z01), minus(code_pair<0>(b), z23), minus(code_pair<1>(b), z23)};
-            const uint32_t f1[4] = {minus(code_pair<2>(a), z01), minus(code_pair<3>(a), z01), minus(code_pair<2>(b), z23), minus(code_pair<3>(b), z23)};
+            const uint32_t f0[4] = {minus(code_pair<0>(a, sixteens), z01), minus(code_pair<1>(a, sixteens), z01), minus(code_pair<0>(b, sixteens), z23), minus(code_pair<1>(b, sixteens), z23)};
+            const uint32_t f1[4] = {minus(code_pair<2>(a, sixteens), z01), minus(code_pair<3>(a, sixteens), z01), minus(code_pair<2>(b, sixteens), z23), minus(code_pair<3>(b, sixteens), z23)};
             const int tile = 4 * u + 2 * h;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -544,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          top[nt][x] = -INFINITY;
+          top[nt][x] = kNone;
           norm[nt][x] = 0.f;
         }
 #pragma unroll
@@ -557,14 +653,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const float2 one = ml(k, nt * 8 + 2 * t + x);
-            f[x] = one.x == -INFINITY && one.y == 0.f ? 0.f : exp2f(one.x == -INFINITY ? 0.f : one.x - top[nt][x]);
+            f[x] = exp2f(one.x - top[nt][x]);
             norm[nt][x] += one.y * f[x];
           }
 #pragma unroll
           for (int i = 0; i < OWN; ++i) {
             const float4 v = o(k, nt * MT + warp * OWN + i);
-            if (f[0] != 0.f) { sum[nt][i].x += v.x * f[0]; sum[nt][i].z += v.z * f[0]; }
-            if (f[1] != 0.f) { sum[nt][i].y += v.y * f[1]; sum[nt][i].w += v.w * f[1]; }
+            sum[nt][i].x += v.x * f[0]; sum[nt][i].z += v.z * f[0];
+            sum[nt][i].y += v.y * f[1]; sum[nt][i].w += v.w * f[1];
           }
         }
       }
@@ -629,7 +725,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
 template <typename T, int DIM, int NT, int PARTS>
 int launch_mma(const MmaParams& p, int grid, cudaStream_t stream) {
   constexpr int MT = DIM / 16;
-  const size_t smem = sizeof(Stage<DIM>) * kStages * kWarps + (size_t)kWarps * NT * MT * 512 + (size_t)kWarps * 8 * NT * 8 + 16 +
+  const size_t smem = sizeof(Stage<DIM>) * kStages * kWarps + kWarps * kChunk * 16 + (size_t)kWarps * NT * MT * 512 + (size_t)kWarps * 8 * NT * 8 + 16 +
                       (size_t)(p.n_requests + 1) * 12;
   auto* kernel = packed_attention_mma_kernel<T, DIM, NT, PARTS>;
   static int configured[64] = {0};
@@ -666,7 +762,7 @@ YALIS_API int yalis_packed_attention_mma(const void* q, long long q_stride, int 
   p.q = q; p.q_stride = q_stride; p.out = out; p.out_stride = out_stride;
   p.positions = positions; p.q_start = q_start; p.block_table = block_table; p.table_width = table_width;
   p.n_requests = n_requests; p.nh = nh; p.per = nh / g; p.window = window; p.q_vector = q_vector; p.only_single = only_single;
-  p.page_shift = -1;
+  p.page_shift = -1; p.together = page_size % kChunk == 0 ? 2 : page_size % (1024 / dim) == 0 ? 1 : 0;
   if ((page_size & (page_size - 1)) == 0)
     for (p.page_shift = 0; 1 << p.page_shift < page_size;) ++p.page_shift;
   p.scale_log2 = scale * 1.4426950408889634f; p.lse = lse; p.part = scratch; p.tickets = tickets; p.error = error;

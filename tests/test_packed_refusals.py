@@ -45,7 +45,7 @@ def test_argument_types_are_those_of_the_library():
     entries = {}
     for path in glob.glob(os.path.join(root, "csrc", "*.cu")):
         for name, parameters in re.findall(r"YALIS_API [\w ]+?(\w+)\(([^)]*)\)", open(path).read()):
-            kinds = ["p" if "*" in x or "cudaStream_t" in x else {"int": "i", "long": "l", "float": "f"}[x.split()[0]] for x in parameters.split(",") if x.strip()]
+            kinds = ["p" if "*" in x or "cudaStream_t" in x else {"long": "l", "int64_t": "l", "float": "f"}.get(x.split()[0], "i") for x in parameters.split(",") if x.strip()]
             entries[name] = "".join(kinds)
     used = re.findall(r'_entry\("(\w+)", ((?:"[plif]*"(?: \+ )?)+)', open(packed.__file__).read())
     assert len(used) >= 6

@@ -75,6 +75,7 @@ struct PrefillParams {
   int skip_single;             // 1: requests that bring one token are left to another kernel
   float* part_o;               // [N, nh, n_splits, HS]
   float* part_ml;              // [N, nh, n_splits, 2]
+  float* lse;                  // [N, nh] the logarithm of a row's sum of exponentials, or null
   int32_t* error;
   // the general form (see attention_mma.cu, whose arithmetic of scores, sinks and gates this is)
   int window, chunk;           // 0: none
@@ -643,6 +644,7 @@ prefill_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, cons
           *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(INFINITY, 0.f);
         }
         float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
+        if (p.lse && valid) p.lse[(size_t)(tok_first + t_in) * p.nh + kvh * p.per + head] = (m_run + log2f(l_run)) * 0.693147180559945309f;
         const __nv_bfloat16* gate = nullptr;
         if constexpr (GEN) {
           if (p.sink) {                                         // the sums stand relative to m_run: the sink joins there
@@ -771,11 +773,14 @@ bool make_q_map(CUtensorMap* map, const void* q, long long n_tokens, int q_strid
 }
 
 // Adds the shares of every (token, head) that was divided: one block per token, a thread per four output columns.
+// `q_start` (or null): tokens outside the requests' ranges are left alone.
 __global__ void prefill_merge_splits_kernel(const float* part_o, const float* part_ml,
-                                            __nv_bfloat16* out, int out_stride, int nh, int hs, int n_splits) {
+                                            __nv_bfloat16* out, int out_stride, int nh, int hs, int n_splits, const int32_t* q_start,
+                                            int n_requests, float* lse) {
   pdl_launch_dependents();
   pdl_wait();
   const int tok = blockIdx.x, vec = hs / 4;
+  if (q_start && (tok < q_start[0] || tok >= q_start[n_requests])) return;
   for (int e = threadIdx.x; e < nh * vec; e += blockDim.x) {
     const int head = e / vec, d = (e - head * vec) * 4;
     const size_t slot0 = ((size_t)tok * nh + head) * n_splits;
@@ -793,6 +798,7 @@ __global__ void prefill_merge_splits_kernel(const float* part_o, const float* pa
       acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
     }
     const float inv = ll > 0.f ? 1.0f / ll : 0.f;
+    if (lse && d == 0) lse[(size_t)tok * nh + head] = (mm + log2f(ll)) * 0.693147180559945309f;
     __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
     uint2 w;
     w.x = *reinterpret_cast<unsigned*>(&lo);
@@ -803,7 +809,7 @@ __global__ void prefill_merge_splits_kernel(const float* part_o, const float* pa
 
 template <int HS, bool GEN>
 int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const PrefillParams& p, int n_splits,
-           int n_tokens, cudaStream_t stream) {
+           int n_tokens, bool rows_of_requests, cudaStream_t stream) {
   const size_t smem = 1024 + (size_t)BM * HS * 2 + (size_t)4 * BN * HS * 2 + kBarriers * 8 + 8 + 2 * sizeof(ItemDesc);
   static bool configured = false;
   if (!configured) {
@@ -817,7 +823,8 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, 
   int st = yalis_launch(prefill_attention_tcgen05_kernel<HS, GEN>, grid, dim3(kThreads), smem, stream, mq, mk, mv, p);
   if (st != YALIS_OK || n_splits == 1) return st;
   return yalis_launch(prefill_merge_splits_kernel, dim3(n_tokens), dim3(256), 0, stream, (const float*)p.part_o,
-                      (const float*)p.part_ml, p.out, p.out_stride, p.nh, HS, n_splits);
+                      (const float*)p.part_ml, p.out, p.out_stride, p.nh, HS, n_splits, rows_of_requests ? p.q_start : (const int32_t*)nullptr,
+                      p.n_requests, p.lse);
 }
 
 // Tiles of queries in the step: sum of ceil(q / tokens_per_tile) over the requests, bounded from their number, the step's
@@ -835,14 +842,14 @@ bool count_items(PrefillParams& p, int n_tokens, int max_q_len, int n_splits) {
 
 template <bool GEN>
 int launch_prefill(const PrefillParams& p, const void* q, int q_stride, const void* k_pool, const void* v_pool, int n_tokens,
-                   int hs, int n_splits, cudaStream_t stream) {
+                   int hs, int n_splits, cudaStream_t stream, bool rows_of_requests = false) {
   CUtensorMap mq, mk, mv;
   const long long rows = (long long)p.num_pages * p.g * p.page_size;
   if (!make_q_map(&mq, q, n_tokens, q_stride, p.nh, hs, p.per, p.tokens_per_tile) ||
       !make_pool_map(&mk, k_pool, rows, hs, p.page_size) || !make_pool_map(&mv, v_pool, rows, hs, p.page_size))
     return YALIS_ERR_LAUNCH;
-  return hs == 64 ? launch<64, GEN>(mq, mk, mv, p, n_splits, n_tokens, stream)
-                  : launch<128, GEN>(mq, mk, mv, p, n_splits, n_tokens, stream);
+  return hs == 64 ? launch<64, GEN>(mq, mk, mv, p, n_splits, n_tokens, rows_of_requests, stream)
+                  : launch<128, GEN>(mq, mk, mv, p, n_splits, n_tokens, rows_of_requests, stream);
 }
 
 }  // namespace
@@ -944,4 +951,38 @@ YALIS_API int yalis_prefill_attention_tcgen05_general(
   p.sink = sink; p.sink_logits = sink ? sink_logits : nullptr; p.slopes = slopes;
   p.gate = (const __nv_bfloat16*)gate; p.gate_stride = gate_stride; p.gate_per_head = gate_per_head;
   return launch_prefill<true>(p, q, q_stride, k_pool, v_pool, n_tokens, hs, 1, stream);
+}
+
+// For caches in another format, whose visible rows were unpacked into pools of this call (see packed_attention.cu): a window (0:
+// none, else without shares of the keys), rows of no request left alone, and `lse` [N, nh] or null.  Otherwise as above.
+YALIS_API int yalis_prefill_attention_tcgen05_unpacked(
+    const void* q, long long q_stride, void* out, long long out_stride, const void* k_pool, const void* v_pool, const int32_t* positions,
+    const int32_t* q_start, const int32_t* block_table, int table_width, int page_size, int num_pages, int n_tokens, int n_requests,
+    int max_q_len, int nh, int g, int hs, float scale, int window, int n_splits, int tiles_per_split, int skip_single, float* lse,
+    float* scratch, int32_t* work, int32_t* error, cudaStream_t stream) {
+  if (n_tokens <= 0 || n_requests <= 0) return YALIS_OK;
+  if (g <= 0 || nh % g != 0 || max_q_len < 1 || !(scale > 0.f) || n_splits < 1 || n_splits > 64 || tiles_per_split < 1) return YALIS_ERR_SHAPE;
+  if (q_stride > 0x7fffffff || out_stride > 0x7fffffff || (window > 0 && n_splits > 1)) return YALIS_ERR_SHAPE;
+  if (n_splits > 1 && (scratch == nullptr || ((uintptr_t)scratch & 15))) return YALIS_ERR_ALIGN;
+  if (!yalis_prefill_attention_tcgen05_supports(hs, page_size, nh / g)) return YALIS_ERR_SHAPE;
+  if ((((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out) & 15) || (q_stride % 8) || (out_stride % 8)) return YALIS_ERR_ALIGN;
+  PrefillParams p = {};
+  p.out = (__nv_bfloat16*)out; p.out_stride = (int)out_stride;
+  p.positions = positions; p.q_start = q_start; p.block_table = block_table;
+  p.table_width = table_width; p.page_size = page_size; p.num_pages = num_pages;
+  p.nh = nh; p.g = g; p.per = nh / g;
+  p.n_requests = n_requests;
+  p.tokens_per_tile = BM / p.per;
+  if (!count_items(p, n_tokens, max_q_len, n_splits)) return YALIS_ERR_SHAPE;
+  p.work = work;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.tiles_per_split = tiles_per_split;
+  p.skip_single = skip_single ? 1 : 0;
+  p.part_o = scratch;
+  p.part_ml = scratch ? scratch + (size_t)n_tokens * nh * n_splits * hs : nullptr;
+  p.lse = lse;
+  p.error = error;
+  p.window = window; p.out_scale = 1.f;
+  return window > 0 ? launch_prefill<true>(p, q, (int)q_stride, k_pool, v_pool, n_tokens, hs, 1, stream, true)
+                    : launch_prefill<false>(p, q, (int)q_stride, k_pool, v_pool, n_tokens, hs, n_splits, stream, true);
 }

@@ -153,6 +153,66 @@ int launch_rows(const RowParams<T>& p, cudaStream_t stream) {
 #undef YALIS_ROWS
 }
 
+// The visible rows of requests' caches into bfloat16 pools of one call, for kernels that read such pools: pages of kUnpackPage
+// keys, request after request (page r * width + i holds keys i * kUnpackPage ... of request r), with the block table that says so
+// and the counters of the kernel behind it at zero.  Exact: every value is a bfloat16 number.  A block takes a page of one KV
+// head, a thread eight codes at a time.  Bound by the writes (512 B a token and KV head at 128), most of which the reader finds
+// in the L2.
+constexpr int kUnpackPage = 64;
+
+struct UnpackParams {
+  __nv_bfloat16* k_out;        // [R * width, g, kUnpackPage, dim]
+  __nv_bfloat16* v_out;
+  int32_t* table_out;          // [R, width]
+  int32_t* zeroed;             // two counters
+  const int32_t* positions;
+  const int32_t* q_start;      // [R + 1]
+  const int32_t* block_table;
+  int table_width, width, window, skip_single;
+  int32_t* error;
+  PackedPages pages;
+};
+
+__global__ void __launch_bounds__(256) packed_unpack_kernel(const UnpackParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int index = blockIdx.x, kvh = blockIdx.y, req = blockIdx.z, words = p.pages.dim / 8;
+  if (threadIdx.x == 0) {
+    if (kvh == 0) p.table_out[(size_t)req * p.width + index] = req * p.width + index;
+    if (index == 0 && kvh == 0 && req == 0) p.zeroed[0] = p.zeroed[1] = 0;
+  }
+  const int t0 = p.q_start[req], n = p.q_start[req + 1] - t0;
+  if (n <= 0 || (p.skip_single && n == 1)) return;
+  const int last = p.positions[t0 + n - 1], begin = p.positions[t0], key0 = index * kUnpackPage;
+  const int first = p.window > 0 ? max(0, begin - p.window + 1) : 0;
+  if (key0 > last || key0 + kUnpackPage <= first) return;
+  const size_t to = (((size_t)req * p.width + index) * p.pages.g + kvh) * kUnpackPage;
+  const int rows = min(kUnpackPage, last - key0 + 1);
+  for (int i = threadIdx.x; i < rows * words; i += 256) {
+    const int r = i / words, w = i - r * words, key = key0 + r;
+    int row;
+    const int page = page_of(p.pages, p.block_table + (size_t)req * p.table_width, p.table_width, key, row);
+    uint4 k = make_uint4(0u, 0u, 0u, 0u), v = k;
+    if (page >= 0) {
+      const size_t at = row_index(p.pages, page, kvh, row);
+      const uint32_t word = p.pages.words[at], kc = p.pages.k[at * words + w], vc = p.pages.v[at * words + w];
+      const float ks = step_of(word & 0xFFFFu), kz = zero_of(word), vs = step_of(word >> 16), vz = zero_of(word >> 16);
+      uint32_t* out[2] = {&k.x, &v.x};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(((float)(kc >> (8 * e) & 15u) - kz) * ks, ((float)(kc >> (8 * e + 4) & 15u) - kz) * ks);
+        const __nv_bfloat162 b = __floats2bfloat162_rn(((float)(vc >> (8 * e) & 15u) - vz) * vs, ((float)(vc >> (8 * e + 4) & 15u) - vz) * vs);
+        out[0][e] = *reinterpret_cast<const uint32_t*>(&a);
+        out[1][e] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+    } else if (key >= first && w == 0 && p.error) {
+      atomicOr(p.error, YALIS_FLAG_BAD_PAGE);
+    }
+    reinterpret_cast<uint4*>(p.k_out)[(to + r) * words + w] = k;
+    reinterpret_cast<uint4*>(p.v_out)[(to + r) * words + w] = v;
+  }
+}
+
 }  // namespace
 
 // Writes the rows of n_tokens tokens (write 1), or reads them back into contiguous [N, g * dim] (write 0).
@@ -172,4 +232,18 @@ YALIS_API int yalis_packed_rows(int write, void* k, void* v, long long k_stride,
     p.pages = {static_cast<uint32_t*>(k_codes), static_cast<uint32_t*>(v_codes), static_cast<uint32_t*>(words), num_pages, page_size, g, dim};
     return write ? launch_rows<T, true>(p, stream) : launch_rows<T, false>(p, stream);
   });
+}
+
+YALIS_API int yalis_packed_unpack(void* k_codes, void* v_codes, void* words, int num_pages, int page_size, int g, int dim, const int32_t* positions,
+                                  const int32_t* q_start, const int32_t* block_table, int table_width, int n_requests, int width, int window,
+                                  int skip_single, void* k_out, void* v_out, int32_t* table_out, int32_t* zeroed, int32_t* error,
+                                  cudaStream_t stream) {
+  if (dim < 8 || dim > 256 || dim % 8 || page_size < 1 || g < 1 || g > 65535 || n_requests > 65535 || width < 1) return YALIS_ERR_SHAPE;
+  if (n_requests <= 0) return YALIS_OK;
+  UnpackParams p = {};
+  p.k_out = static_cast<__nv_bfloat16*>(k_out); p.v_out = static_cast<__nv_bfloat16*>(v_out); p.table_out = table_out; p.zeroed = zeroed;
+  p.positions = positions; p.q_start = q_start; p.block_table = block_table; p.table_width = table_width; p.width = width;
+  p.window = window; p.skip_single = skip_single; p.error = error;
+  p.pages = {static_cast<uint32_t*>(k_codes), static_cast<uint32_t*>(v_codes), static_cast<uint32_t*>(words), num_pages, page_size, g, dim};
+  return yalis_launch(packed_unpack_kernel, dim3(width, g, n_requests), dim3(256), 0, stream, p);
 }

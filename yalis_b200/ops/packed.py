@@ -14,7 +14,8 @@ from typing import Optional, Sequence, Tuple
 
 import torch
 
-from ._lib import F32, KernelError, check, dtype_code, lib, need, stream
+from ._lib import BF16, F32, KernelError, check, dtype_code, lib, need, stream
+from .attention import sm_count
 
 _TYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 _entries = {}
@@ -181,6 +182,43 @@ def packed_kv_read(pages: PackedPages, positions: torch.Tensor, req_of_token: to
     return k, v
 
 
+UNPACK_ROWS = 64          # query rows of a pair (tokens * heads of a KV head) beyond which portions are unpacked for the prompt kernel
+UNPACK_PAGE = 64          # keys of a page of the unpacked pools
+UNPACK_BYTES = 2 << 30    # of unpacked keys and values at a time
+
+
+def _attend_unpacked(name, q, out, held, at, steps, n, max_q_len, max_kv_len, num_heads, scale, window, skip_single, lse, error_flag, raw):
+    """Portions of prompts: the rows that they see are unpacked, as many requests at a time as ``UNPACK_BYTES`` hold, into pools of
+    the call for the prompt kernel on the tcgen05 tensor cores (every value is a bfloat16 number, so nothing is rounded)."""
+    g, dim = held[5:]
+    positions, q_start, table, table_width, r = at
+    width = max(1, -(-max_kv_len // UNPACK_PAGE))
+    rows = width * g * UNPACK_PAGE * dim                # of a request, keys or values
+    group = max(1, min(r, UNPACK_BYTES // (4 * rows)))
+    per = num_heads // g
+    tiles = min(r, group) * -(-max_q_len // (128 // per)) * g
+    splits, share = 1, 1
+    if window == 0:                                     # few tiles of queries with many keys: the keys of a tile in shares
+        splits = max(1, min(8, 2 * sm_count(q.device) // tiles, width // 16))
+        share = -(-width // splits)
+    need_floats = n * num_heads * splits * (dim + 2) if splits > 1 else 0
+    pools = torch.empty(2 * group * rows, dtype=torch.bfloat16, device=q.device)
+    work = torch.empty(group * width + 2, dtype=torch.int32, device=q.device)
+    scratch = torch.empty(need_floats, dtype=torch.float32, device=q.device) if need_floats else None
+    k_at, table_at = pools.data_ptr(), work.data_ptr() + 8
+    v_at = k_at + 2 * group * rows
+    for first in range(0, r, group):
+        m = min(group, r - first)
+        starts, row = q_start + 4 * first, table + 4 * first * table_width
+        check(_entry("yalis_packed_unpack", "pppiiii" + "pppii" + "iii" + "pppppp")(
+            *held, positions, starts, row, table_width, m, width, window, skip_single, k_at, v_at, table_at, work.data_ptr(),
+            _address(error_flag), raw), name)
+        check(_entry("yalis_prefill_attention_tcgen05_unpacked", "plplpp" + "pppiii" + "iiiiii" + "fiiiippppp")(
+            q.data_ptr(), steps[0], out.data_ptr(), steps[1], k_at, v_at, positions, starts, table_at, width, UNPACK_PAGE, m * width, n, m,
+            max_q_len, num_heads, g, dim, scale, window, splits, share, skip_single, _address(lse), _address(scratch), work.data_ptr(),
+            _address(error_flag), raw), name)
+
+
 def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tensor, q_start: torch.Tensor, block_table: torch.Tensor,
                      max_q_len: int, num_heads: int, scale: Optional[float] = None, window: Optional[int] = None,
                      max_kv_len: Optional[int] = None, weight_sums: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -224,15 +262,21 @@ def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tenso
     need(out.shape == (n, width) and out.dtype is q.dtype and out.stride(1) == 1, name, "bad out tensor")
     lse = torch.empty((n, num_heads), dtype=torch.float32, device=q.device) if weight_sums is not None else None
     at, steps, raw = (positions.data_ptr(), q_start.data_ptr(), block_table.data_ptr(), block_table.shape[1], r), (q.stride(0), out.stride(0)), stream()
-    if dim in (64, 128) and r <= 4096:
-        columns = 8 if code == F32 or max_q_len * (num_heads // g) <= 8 else 16
+    per, aligned = num_heads // g, (q.data_ptr() | steps[0] * q.element_size()) % 16 == 0
+    unpack = (code == BF16 and dim in (64, 128) and max_q_len * per > UNPACK_ROWS and per <= 128 and scale > 0 and aligned
+              and (out.data_ptr() | steps[1] * 2) % 16 == 0)
+    mma = dim in (64, 128) and r <= 4096
+    single = unpack and mma and n > max_q_len          # single tokens may stand beside the portions: a kernel of their own
+    if unpack:
+        _attend_unpacked(name, q, out, held, at, steps, n, max_q_len, max_kv_len, num_heads, scale, window or 0, single, lse, error_flag, raw)
+    if mma and (single or not unpack):
+        columns = 8 if code == F32 or (1 if single else max_q_len) * per <= 8 else 16
         blocks, floats = _mma_launch(q.device, code, dim, columns)
         scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
-        vector = (q.data_ptr() | steps[0] * q.element_size()) % 16 == 0
         check(_entry("yalis_packed_attention_mma", "plipl" + "pppiiii" + "pppii" + "iiiifipipppp")(
-            q.data_ptr(), steps[0], code, out.data_ptr(), steps[1], *held, *at, num_heads, columns, vector, False, scale, window or 0,
+            q.data_ptr(), steps[0], code, out.data_ptr(), steps[1], *held, *at, num_heads, columns, aligned, single, scale, window or 0,
             _address(lse), blocks, scratch.data_ptr(), _counters(blocks, q.device).data_ptr(), _address(error_flag), raw), name)
-    else:
+    if not mma and not unpack:
         check(_entry("yalis_packed_attention_general", "plipl" + "pppiiii" + "pppii" + "iifippp")(
             q.data_ptr(), steps[0], code, out.data_ptr(), steps[1], *held, *at, n, num_heads, scale, window or 0, _address(lse),
             _address(error_flag), raw), name)

@@ -75,7 +75,7 @@ struct PrefillParams {
   int skip_single;             // 1: requests that bring one token are left to another kernel
   float* part_o;               // [N, nh, n_splits, HS]
   float* part_ml;              // [N, nh, n_splits, 2]
-  float* lse;                  // [N, nh] the logarithm of a row's sum of exponentials, or null
+  float* lse2;                 // [N, nh] the logarithm to base two of a row's sum of exponentials, or null
   int32_t* error;
   // the general form (see attention_mma.cu, whose arithmetic of scores, sinks and gates this is)
   int window, chunk;           // 0: none
@@ -644,7 +644,7 @@ prefill_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, cons
           *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(INFINITY, 0.f);
         }
         float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
-        if (p.lse && valid) p.lse[(size_t)(tok_first + t_in) * p.nh + kvh * p.per + head] = (m_run + log2f(l_run)) * 0.693147180559945309f;
+        if (p.lse2 && valid) p.lse2[(size_t)(tok_first + t_in) * p.nh + kvh * p.per + head] = m_run + log2f(l_run);
         const __nv_bfloat16* gate = nullptr;
         if constexpr (GEN) {
           if (p.sink) {                                         // the sums stand relative to m_run: the sink joins there
@@ -776,7 +776,7 @@ bool make_q_map(CUtensorMap* map, const void* q, long long n_tokens, int q_strid
 // `q_start` (or null): tokens outside the requests' ranges are left alone.
 __global__ void prefill_merge_splits_kernel(const float* part_o, const float* part_ml,
                                             __nv_bfloat16* out, int out_stride, int nh, int hs, int n_splits, const int32_t* q_start,
-                                            int n_requests, float* lse) {
+                                            int n_requests, float* lse2) {
   pdl_launch_dependents();
   pdl_wait();
   const int tok = blockIdx.x, vec = hs / 4;
@@ -798,7 +798,7 @@ __global__ void prefill_merge_splits_kernel(const float* part_o, const float* pa
       acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
     }
     const float inv = ll > 0.f ? 1.0f / ll : 0.f;
-    if (lse && d == 0) lse[(size_t)tok * nh + head] = (mm + log2f(ll)) * 0.693147180559945309f;
+    if (lse2 && d == 0) lse2[(size_t)tok * nh + head] = mm + log2f(ll);
     __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
     uint2 w;
     w.x = *reinterpret_cast<unsigned*>(&lo);
@@ -824,7 +824,7 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, 
   if (st != YALIS_OK || n_splits == 1) return st;
   return yalis_launch(prefill_merge_splits_kernel, dim3(n_tokens), dim3(256), 0, stream, (const float*)p.part_o,
                       (const float*)p.part_ml, p.out, p.out_stride, p.nh, HS, n_splits, rows_of_requests ? p.q_start : (const int32_t*)nullptr,
-                      p.n_requests, p.lse);
+                      p.n_requests, p.lse2);
 }
 
 // Tiles of queries in the step: sum of ceil(q / tokens_per_tile) over the requests, bounded from their number, the step's
@@ -954,11 +954,11 @@ YALIS_API int yalis_prefill_attention_tcgen05_general(
 }
 
 // For caches in another format, whose visible rows were unpacked into pools of this call (see packed_attention.cu): a window (0:
-// none, else without shares of the keys), rows of no request left alone, and `lse` [N, nh] or null.  Otherwise as above.
+// none, else without shares of the keys), rows of no request left alone, and `lse2` [N, nh] or null.  Otherwise as above.
 YALIS_API int yalis_prefill_attention_tcgen05_unpacked(
     const void* q, long long q_stride, void* out, long long out_stride, const void* k_pool, const void* v_pool, const int32_t* positions,
     const int32_t* q_start, const int32_t* block_table, int table_width, int page_size, int num_pages, int n_tokens, int n_requests,
-    int max_q_len, int nh, int g, int hs, float scale, int window, int n_splits, int tiles_per_split, int skip_single, float* lse,
+    int max_q_len, int nh, int g, int hs, float scale, int window, int n_splits, int tiles_per_split, int skip_single, float* lse2,
     float* scratch, int32_t* work, int32_t* error, cudaStream_t stream) {
   if (n_tokens <= 0 || n_requests <= 0) return YALIS_OK;
   if (g <= 0 || nh % g != 0 || max_q_len < 1 || !(scale > 0.f) || n_splits < 1 || n_splits > 64 || tiles_per_split < 1) return YALIS_ERR_SHAPE;
@@ -980,7 +980,7 @@ YALIS_API int yalis_prefill_attention_tcgen05_unpacked(
   p.skip_single = skip_single ? 1 : 0;
   p.part_o = scratch;
   p.part_ml = scratch ? scratch + (size_t)n_tokens * nh * n_splits * hs : nullptr;
-  p.lse = lse;
+  p.lse2 = lse2;
   p.error = error;
   p.window = window; p.out_scale = 1.f;
   return window > 0 ? launch_prefill<true>(p, q, (int)q_stride, k_pool, v_pool, n_tokens, hs, 1, stream, true)

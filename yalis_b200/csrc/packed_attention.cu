@@ -5,7 +5,7 @@
 // and, where sums are kept, A_j += P_j for every query row and head of j's KV head.  A row that sees nothing gives zeros.
 //
 // The general form: a block per (token, head), a thread per key of a tile for the scores and per element for O; scores, weights
-// and sums in float32.  It takes every size; its weights' normaliser, log(sum exp S), goes to memory for the sums, which a second
+// and sums in float32.  It takes every size; its weights' normaliser, log2(sum exp S), goes to memory for the sums, which a second
 // kernel adds key by key in the order of the rows.
 #include "packed.cuh"
 
@@ -23,7 +23,7 @@ struct AttentionParams {
   const int32_t* block_table;  // [R, table_width]
   int table_width, n_requests, n_tokens, nh, per, window;
   float scale;
-  float* lse;                  // [N, nh] or null
+  float* lse2;                 // [N, nh] the logarithm to base two of a row's sum of exponentials, or null
   float* sums;                 // [pages, g, page_size] or null
   int32_t* error;
   PackedPages pages;
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kThreads) packed_attention_general_kernel(cons
     const int d = tid + h * kThreads;
     if (d < dim) dst[d] = from_f32<T>(l == 0.f ? 0.f : acc[h] / l);
   }
-  if (tid == 0 && p.lse) p.lse[(size_t)token * p.nh + head] = m + logf(l);
+  if (tid == 0 && p.lse2) p.lse2[(size_t)token * p.nh + head] = (m + logf(l)) * 1.4426950408889634f;
 }
 
 // A block per (tile of keys, KV head, request), a thread per key: the rows that see the key, in their order.
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kThreads) packed_weight_sums_general_kernel(co
       const float q_sum = block_sum(part, scratch);
       if (sees) {
         const float s = p.scale * step_of(word & 0xFFFFu) * fmaf(-zero_of(word), q_sum, code_product(p.pages.k + at * words, q, words));
-        total += expf(s - p.lse[(size_t)t * p.nh + head]);
+        total += exp2f(s * 1.4426950408889634f - p.lse2[(size_t)t * p.nh + head]);
         seen = true;
       }
     }
@@ -175,28 +175,28 @@ bool params_of(AttentionParams& p, const void* q, long long q_stride, void* k_co
 YALIS_API int yalis_packed_attention_general(const void* q, long long q_stride, int dtype, void* out, long long out_stride, void* k_codes,
                                              void* v_codes, void* words, int num_pages, int page_size, int g, int dim,
                                              const int32_t* positions, const int32_t* q_start, const int32_t* block_table, int table_width,
-                                             int n_requests, int n_tokens, int nh, float scale, int window, float* lse, int32_t* error,
+                                             int n_requests, int n_tokens, int nh, float scale, int window, float* lse2, int32_t* error,
                                              cudaStream_t stream) {
   AttentionParams p;
   if (!params_of(p, q, q_stride, k_codes, v_codes, words, num_pages, page_size, g, dim, positions, q_start, block_table, table_width, n_requests,
                  nh, scale, window))
     return YALIS_ERR_SHAPE;
   if (n_tokens <= 0 || n_requests <= 0) return YALIS_OK;
-  p.out = out; p.out_stride = out_stride; p.n_tokens = n_tokens; p.lse = lse; p.error = error;
+  p.out = out; p.out_stride = out_stride; p.n_tokens = n_tokens; p.lse2 = lse2; p.error = error;
   YALIS_DISPATCH_DTYPE(dtype, T, return yalis_launch(packed_attention_general_kernel<T>, dim3(n_tokens, nh), dim3(kThreads), 0, stream, p));
 }
 
-// Adds to `sums` the weights that the step's rows give the cached tokens; `lse` [N, nh] from the attention of the same step.
+// Adds to `sums` the weights that the step's rows give the cached tokens; `lse2` [N, nh] from the attention of the same step.
 YALIS_API int yalis_packed_weight_sums_general(const void* q, long long q_stride, int dtype, void* k_codes, void* v_codes, void* words,
                                                int num_pages, int page_size, int g, int dim, const int32_t* positions, const int32_t* q_start,
                                                const int32_t* block_table, int table_width, int n_requests, int max_kv_len, int nh, float scale,
-                                               int window, float* lse, float* sums, cudaStream_t stream) {
+                                               int window, float* lse2, float* sums, cudaStream_t stream) {
   AttentionParams p;
   if (!params_of(p, q, q_stride, k_codes, v_codes, words, num_pages, page_size, g, dim, positions, q_start, block_table, table_width, n_requests,
                  nh, scale, window) || g > 65535)
     return YALIS_ERR_SHAPE;
   if (n_requests <= 0 || max_kv_len <= 0) return YALIS_OK;
-  p.lse = lse; p.sums = sums;
+  p.lse2 = lse2; p.sums = sums;
   YALIS_DISPATCH_DTYPE(dtype, T, return yalis_launch(packed_weight_sums_general_kernel<T>, dim3((max_kv_len + kThreads - 1) / kThreads, g, n_requests),
                                                      dim3(kThreads), 0, stream, p));
 }

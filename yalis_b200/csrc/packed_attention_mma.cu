@@ -44,7 +44,7 @@ struct MmaParams {
   int q_vector;                // 1: rows of q start on 16-byte boundaries
   int only_single;             // 1: requests that bring more than one token are left to another kernel
   float scale_log2;
-  float* lse;                  // [N, nh] or null
+  float* lse2;                 // [N, nh] the logarithm to base two of a row's sum of exponentials, or null
   float* part;                 // [blocks, 2, MT * 32 * 4 + 16 NT * 2]
   int32_t* tickets;            // one per pair, zero before and after
   int32_t* error;
@@ -714,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
             dst[2 * i] = from_f32<T>(a * inv);
             dst[2 * i + 1] = from_f32<T>(b * inv);
           }
-          if (p.lse && warp == 0 && g == 0) p.lse[(size_t)token * p.nh + head] = (top[nt][x] + log2f(norm[nt][x])) * 0.693147180559945309f;
+          if (p.lse2 && warp == 0 && g == 0) p.lse2[(size_t)token * p.nh + head] = top[nt][x] + log2f(norm[nt][x]);
         }
       }
     }
@@ -754,7 +754,7 @@ YALIS_API long long yalis_packed_attention_mma_scratch_floats(int blocks, int di
 YALIS_API int yalis_packed_attention_mma(const void* q, long long q_stride, int dtype, void* out, long long out_stride, void* k_codes,
                                          void* v_codes, void* words, int num_pages, int page_size, int g, int dim, const int32_t* positions,
                                          const int32_t* q_start, const int32_t* block_table, int table_width, int n_requests, int nh,
-                                         int columns, int q_vector, int only_single, float scale, int window, float* lse, int blocks,
+                                         int columns, int q_vector, int only_single, float scale, int window, float* lse2, int blocks,
                                          float* scratch, int32_t* tickets, int32_t* error, cudaStream_t stream) {
   if ((dim != 64 && dim != 128) || nh % g || n_requests > 4096 || blocks < 1) return YALIS_ERR_SHAPE;
   if (n_requests <= 0) return YALIS_OK;
@@ -765,7 +765,7 @@ YALIS_API int yalis_packed_attention_mma(const void* q, long long q_stride, int 
   p.page_shift = -1; p.together = page_size % kChunk == 0 ? 2 : page_size % (1024 / dim) == 0 ? 1 : 0;
   if ((page_size & (page_size - 1)) == 0)
     for (p.page_shift = 0; 1 << p.page_shift < page_size;) ++p.page_shift;
-  p.scale_log2 = scale * 1.4426950408889634f; p.lse = lse; p.part = scratch; p.tickets = tickets; p.error = error;
+  p.scale_log2 = scale * 1.4426950408889634f; p.lse2 = lse2; p.part = scratch; p.tickets = tickets; p.error = error;
   p.pages = {static_cast<uint32_t*>(k_codes), static_cast<uint32_t*>(v_codes), static_cast<uint32_t*>(words), num_pages, page_size, g, dim};
   if (dtype == YALIS_BF16) {
     if (columns == 8) return dim == 64 ? launch_mma<__nv_bfloat16, 64, 1, 1>(p, blocks, stream) : launch_mma<__nv_bfloat16, 128, 1, 1>(p, blocks, stream);

@@ -187,7 +187,7 @@ UNPACK_PAGE = 64          # keys of a page of the unpacked pools
 UNPACK_BYTES = 2 << 30    # of unpacked keys and values at a time
 
 
-def _attend_unpacked(name, q, out, held, at, steps, n, max_q_len, max_kv_len, num_heads, scale, window, skip_single, lse, error_flag, raw):
+def _attend_unpacked(name, q, out, held, at, steps, n, max_q_len, max_kv_len, num_heads, scale, window, skip_single, lse2, error_flag, raw):
     """Portions of prompts: the rows that they see are unpacked, as many requests at a time as ``UNPACK_BYTES`` hold, into pools of
     the call for the prompt kernel on the tcgen05 tensor cores (every value is a bfloat16 number, so nothing is rounded)."""
     g, dim = held[5:]
@@ -215,7 +215,7 @@ def _attend_unpacked(name, q, out, held, at, steps, n, max_q_len, max_kv_len, nu
             _address(error_flag), raw), name)
         check(_entry("yalis_prefill_attention_tcgen05_unpacked", "plplpp" + "pppiii" + "iiiiii" + "fiiiippppp")(
             q.data_ptr(), steps[0], out.data_ptr(), steps[1], k_at, v_at, positions, starts, table_at, width, UNPACK_PAGE, m * width, n, m,
-            max_q_len, num_heads, g, dim, scale, window, splits, share, skip_single, _address(lse), _address(scratch), work.data_ptr(),
+            max_q_len, num_heads, g, dim, scale, window, splits, share, skip_single, _address(lse2), _address(scratch), work.data_ptr(),
             _address(error_flag), raw), name)
 
 
@@ -260,7 +260,7 @@ def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tenso
     if out is None:
         out = torch.empty((n, width), dtype=q.dtype, device=q.device)
     need(out.shape == (n, width) and out.dtype is q.dtype and out.stride(1) == 1, name, "bad out tensor")
-    lse = torch.empty((n, num_heads), dtype=torch.float32, device=q.device) if weight_sums is not None else None
+    lse2 = torch.empty((n, num_heads), dtype=torch.float32, device=q.device) if weight_sums is not None else None
     at, steps, raw = (positions.data_ptr(), q_start.data_ptr(), block_table.data_ptr(), block_table.shape[1], r), (q.stride(0), out.stride(0)), stream()
     per, aligned = num_heads // g, (q.data_ptr() | steps[0] * q.element_size()) % 16 == 0
     unpack = (code == BF16 and dim in (64, 128) and max_q_len * per > UNPACK_ROWS and per <= 128 and scale > 0 and aligned
@@ -268,21 +268,25 @@ def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tenso
     mma = dim in (64, 128) and r <= 4096
     single = unpack and mma and n > max_q_len          # single tokens may stand beside the portions: a kernel of their own
     if unpack:
-        _attend_unpacked(name, q, out, held, at, steps, n, max_q_len, max_kv_len, num_heads, scale, window or 0, single, lse, error_flag, raw)
+        _attend_unpacked(name, q, out, held, at, steps, n, max_q_len, max_kv_len, num_heads, scale, window or 0, single, lse2, error_flag, raw)
     if mma and (single or not unpack):
         columns = 8 if code == F32 or (1 if single else max_q_len) * per <= 8 else 16
         blocks, floats = _mma_launch(q.device, code, dim, columns)
         scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
         check(_entry("yalis_packed_attention_mma", "plipl" + "pppiiii" + "pppii" + "iiiifipipppp")(
             q.data_ptr(), steps[0], code, out.data_ptr(), steps[1], *held, *at, num_heads, columns, aligned, single, scale, window or 0,
-            _address(lse), blocks, scratch.data_ptr(), _counters(blocks, q.device).data_ptr(), _address(error_flag), raw), name)
+            _address(lse2), blocks, scratch.data_ptr(), _counters(blocks, q.device).data_ptr(), _address(error_flag), raw), name)
     if not mma and not unpack:
         check(_entry("yalis_packed_attention_general", "plipl" + "pppiiii" + "pppii" + "iifippp")(
-            q.data_ptr(), steps[0], code, out.data_ptr(), steps[1], *held, *at, n, num_heads, scale, window or 0, _address(lse),
+            q.data_ptr(), steps[0], code, out.data_ptr(), steps[1], *held, *at, n, num_heads, scale, window or 0, _address(lse2),
             _address(error_flag), raw), name)
-    if weight_sums is not None:
+    if weight_sums is not None and mma:
+        check(_entry("yalis_packed_weight_sums", "pli" + "pppiiii" + "pppii" + "iifiiippp")(
+            q.data_ptr(), steps[0], code, *held, *at, max_kv_len, num_heads, scale, window or 0, max_q_len * per, aligned, lse2.data_ptr(),
+            weight_sums.data_ptr(), raw), name)
+    elif weight_sums is not None:
         check(_entry("yalis_packed_weight_sums_general", "pli" + "pppiiii" + "pppii" + "iifippp")(
-            q.data_ptr(), steps[0], code, *held, *at, max_kv_len, num_heads, scale, window or 0, lse.data_ptr(), weight_sums.data_ptr(), raw), name)
+            q.data_ptr(), steps[0], code, *held, *at, max_kv_len, num_heads, scale, window or 0, lse2.data_ptr(), weight_sums.data_ptr(), raw), name)
     return out
 
 

@@ -21,6 +21,7 @@ struct SumsParams {
   const int32_t* q_start;      // [R + 1]
   const int32_t* block_table;
   int table_width, nh, per, window, q_vector;
+  int only_single;             // 1: requests that bring more than one token are left to another kernel
   float scale_log2;
   const float* lse2;           // [N, nh] in powers of two
   float* sums;                 // [pages, g, page_size]
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_weight_sums_kernel(const S
   pdl_launch_dependents();
   pdl_wait();
   const int tok0 = p.q_start[req], n = p.q_start[req + 1] - tok0;
-  if (n <= 0) return;
+  if (n <= 0 || (p.only_single && n > 1)) return;
   const int begin = p.positions[tok0], last = p.positions[tok0 + n - 1];
   if (block0 > last || last < 0) return;
   // Rows stand at consecutive places: those that see a key of the block are [t_lo, t_hi).
@@ -252,12 +253,12 @@ int launch_sums(const SumsParams& p, int n_requests, int max_kv_len, int columns
 YALIS_API int yalis_packed_weight_sums(const void* q, long long q_stride, int dtype, void* k_codes, void* v_codes, void* words, int num_pages,
                                        int page_size, int g, int dim, const int32_t* positions, const int32_t* q_start,
                                        const int32_t* block_table, int table_width, int n_requests, int max_kv_len, int nh, float scale,
-                                       int window, int columns, int q_vector, float* lse2, float* sums, cudaStream_t stream) {
+                                       int window, int columns, int q_vector, int only_single, float* lse2, float* sums, cudaStream_t stream) {
   if ((dim != 64 && dim != 128) || nh % g || page_size < 1) return YALIS_ERR_SHAPE;
   if (n_requests <= 0 || max_kv_len <= 0) return YALIS_OK;
   SumsParams p = {};
   p.q = q; p.q_stride = q_stride; p.positions = positions; p.q_start = q_start; p.block_table = block_table; p.table_width = table_width;
-  p.nh = nh; p.per = nh / g; p.window = window; p.q_vector = q_vector; p.scale_log2 = scale * 1.4426950408889634f;
+  p.nh = nh; p.per = nh / g; p.window = window; p.q_vector = q_vector; p.only_single = only_single; p.scale_log2 = scale * 1.4426950408889634f;
   p.lse2 = lse2; p.sums = sums;
   p.pages = {static_cast<uint32_t*>(k_codes), static_cast<uint32_t*>(v_codes), static_cast<uint32_t*>(words), num_pages, page_size, g, dim};
   if (dtype == YALIS_BF16)

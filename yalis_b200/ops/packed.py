@@ -187,7 +187,8 @@ UNPACK_PAGE = 64          # keys of a page of the unpacked pools
 UNPACK_BYTES = 2 << 30    # of unpacked keys and values at a time
 
 
-def _attend_unpacked(name, q, out, held, at, steps, n, max_q_len, max_kv_len, num_heads, scale, window, skip_single, lse2, error_flag, raw):
+def _attend_unpacked(name, q, out, held, at, steps, n, max_q_len, max_kv_len, num_heads, scale, window, skip_single, lse2,
+                     weight_sums, error_flag, raw):
     """Portions of prompts: the rows that they see are unpacked, as many requests at a time as ``UNPACK_BYTES`` hold, into pools of
     the call for the prompt kernel on the tcgen05 tensor cores (every value is a bfloat16 number, so nothing is rounded)."""
     g, dim = held[5:]
@@ -217,6 +218,10 @@ def _attend_unpacked(name, q, out, held, at, steps, n, max_q_len, max_kv_len, nu
             q.data_ptr(), steps[0], out.data_ptr(), steps[1], k_at, v_at, positions, starts, table_at, width, UNPACK_PAGE, m * width, n, m,
             max_q_len, num_heads, g, dim, scale, window, splits, share, skip_single, _address(lse2), _address(scratch), work.data_ptr(),
             _address(error_flag), raw), name)
+        if weight_sums is not None:
+            check(_entry("yalis_packed_sums_tcgen05", "plpiiiii" + "pppiiiiifii" + "pppp")(
+                q.data_ptr(), steps[0], k_at, width, held[3], held[4], g, dim, positions, starts, row, table_width, m, n, max_kv_len, num_heads, scale,
+                window, skip_single, lse2.data_ptr(), weight_sums.data_ptr(), _address(error_flag), raw), name)
 
 
 def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tensor, q_start: torch.Tensor, block_table: torch.Tensor,
@@ -268,7 +273,8 @@ def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tenso
     mma = dim in (64, 128) and r <= 4096
     single = unpack and mma and n > max_q_len          # single tokens may stand beside the portions: a kernel of their own
     if unpack:
-        _attend_unpacked(name, q, out, held, at, steps, n, max_q_len, max_kv_len, num_heads, scale, window or 0, single, lse2, error_flag, raw)
+        _attend_unpacked(name, q, out, held, at, steps, n, max_q_len, max_kv_len, num_heads, scale, window or 0, single, lse2, weight_sums,
+                         error_flag, raw)
     if mma and (single or not unpack):
         columns = 8 if code == F32 or (1 if single else max_q_len) * per <= 8 else 16
         blocks, floats = _mma_launch(q.device, code, dim, columns)
@@ -280,11 +286,13 @@ def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tenso
         check(_entry("yalis_packed_attention_general", "plipl" + "pppiiii" + "pppii" + "iifippp")(
             q.data_ptr(), steps[0], code, out.data_ptr(), steps[1], *held, *at, n, num_heads, scale, window or 0, _address(lse2),
             _address(error_flag), raw), name)
-    if weight_sums is not None and mma:
-        check(_entry("yalis_packed_weight_sums", "pli" + "pppiiii" + "pppii" + "iifiiippp")(
-            q.data_ptr(), steps[0], code, *held, *at, max_kv_len, num_heads, scale, window or 0, max_q_len * per, aligned, lse2.data_ptr(),
-            weight_sums.data_ptr(), raw), name)
-    elif weight_sums is not None:
+    if weight_sums is None or (unpack and not single):
+        return out
+    if mma:
+        check(_entry("yalis_packed_weight_sums", "pli" + "pppiiii" + "pppii" + "iifiiiippp")(
+            q.data_ptr(), steps[0], code, *held, *at, max_kv_len, num_heads, scale, window or 0, (1 if single else max_q_len) * per, aligned, single,
+            lse2.data_ptr(), weight_sums.data_ptr(), raw), name)
+    else:
         check(_entry("yalis_packed_weight_sums_general", "pli" + "pppiiii" + "pppii" + "iifippp")(
             q.data_ptr(), steps[0], code, *held, *at, max_kv_len, num_heads, scale, window or 0, lse2.data_ptr(), weight_sums.data_ptr(), raw), name)
     return out

@@ -155,7 +155,7 @@ int launch_rows(const RowParams<T>& p, cudaStream_t stream) {
 
 // The visible rows of requests' caches into bfloat16 pools of one call, for kernels that read such pools: pages of kUnpackPage
 // keys, request after request (page r * width + i holds keys i * kUnpackPage ... of request r), with the block table that says so
-// and the counters of the kernel behind it at zero.  Exact: every value is a bfloat16 number.  A block takes a page of one KV
+// and the counters of the kernels behind it at zero.  Exact: every value is a bfloat16 number.  A block takes a page of one KV
 // head, a thread eight codes at a time.  Bound by the writes (512 B a token and KV head at 128), most of which the reader finds
 // in the L2.
 constexpr int kUnpackPage = 64;
@@ -164,7 +164,8 @@ struct UnpackParams {
   __nv_bfloat16* k_out;        // [R * width, g, kUnpackPage, dim]
   __nv_bfloat16* v_out;
   int32_t* table_out;          // [R, width]
-  int32_t* zeroed;             // two counters
+  int32_t* zeroed;             // [n_zeroed] counters (no more than the launch has threads)
+  long long n_zeroed;
   const int32_t* positions;
   const int32_t* q_start;      // [R + 1]
   const int32_t* block_table;
@@ -179,8 +180,9 @@ __global__ void __launch_bounds__(256) packed_unpack_kernel(const UnpackParams p
   const int index = blockIdx.x, kvh = blockIdx.y, req = blockIdx.z, words = p.pages.dim / 8;
   if (threadIdx.x == 0) {
     if (kvh == 0) p.table_out[(size_t)req * p.width + index] = req * p.width + index;
-    if (index == 0 && kvh == 0 && req == 0) p.zeroed[0] = p.zeroed[1] = 0;
   }
+  const long long thread = (((long long)req * p.pages.g + kvh) * p.width + index) * 256 + threadIdx.x;
+  if (thread < p.n_zeroed) p.zeroed[thread] = 0;
   const int t0 = p.q_start[req], n = p.q_start[req + 1] - t0;
   if (n <= 0 || (p.skip_single && n == 1)) return;
   const int last = p.positions[t0 + n - 1], begin = p.positions[t0], key0 = index * kUnpackPage;
@@ -236,11 +238,13 @@ YALIS_API int yalis_packed_rows(int write, void* k, void* v, long long k_stride,
 
 YALIS_API int yalis_packed_unpack(void* k_codes, void* v_codes, void* words, int num_pages, int page_size, int g, int dim, const int32_t* positions,
                                   const int32_t* q_start, const int32_t* block_table, int table_width, int n_requests, int width, int window,
-                                  int skip_single, void* k_out, void* v_out, int32_t* table_out, int32_t* zeroed, int32_t* error,
+                                  int skip_single, void* k_out, void* v_out, int32_t* table_out, int32_t* zeroed, int n_zeroed, int32_t* error,
                                   cudaStream_t stream) {
   if (dim < 8 || dim > 256 || dim % 8 || page_size < 1 || g < 1 || g > 65535 || n_requests > 65535 || width < 1) return YALIS_ERR_SHAPE;
   if (n_requests <= 0) return YALIS_OK;
+  if (n_zeroed > (long long)width * g * n_requests * 256) return YALIS_ERR_SHAPE;
   UnpackParams p = {};
+  p.n_zeroed = n_zeroed;
   p.k_out = static_cast<__nv_bfloat16*>(k_out); p.v_out = static_cast<__nv_bfloat16*>(v_out); p.table_out = table_out; p.zeroed = zeroed;
   p.positions = positions; p.q_start = q_start; p.block_table = block_table; p.table_width = table_width; p.width = width;
   p.window = window; p.skip_single = skip_single; p.error = error;

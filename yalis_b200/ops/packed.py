@@ -204,24 +204,29 @@ def _attend_unpacked(name, q, out, held, at, steps, n, max_q_len, max_kv_len, nu
         share = -(-width // splits)
     need_floats = n * num_heads * splits * (dim + 2) if splits > 1 else 0
     pools = torch.empty(2 * group * rows, dtype=torch.bfloat16, device=q.device)
-    work = torch.empty(group * width + 2, dtype=torch.int32, device=q.device)
+    items = -(-max_kv_len // 128) * group * g if weight_sums is not None else 0         # 128 keys of a KV head each
+    tiles_seen = -(-max_q_len // (128 // per))          # tiles of rows that see an item, at most; about half of them on average
+    each = max(16, items * tiles_seen // (8 * sm_count(q.device)))
+    parts = -(-tiles_seen // each)
+    work = torch.empty(group * width + 3 + 4 * items, dtype=torch.int32, device=q.device)   # counters (two of the prompt kernel's), block table
+    partial = torch.empty(items * parts * 3 * 128, dtype=torch.float32, device=q.device) if items else None
     scratch = torch.empty(need_floats, dtype=torch.float32, device=q.device) if need_floats else None
-    k_at, table_at = pools.data_ptr(), work.data_ptr() + 8
+    k_at, table_at = pools.data_ptr(), work.data_ptr() + 4 * (3 + 4 * items)
     v_at = k_at + 2 * group * rows
     for first in range(0, r, group):
         m = min(group, r - first)
         starts, row = q_start + 4 * first, table + 4 * first * table_width
-        check(_entry("yalis_packed_unpack", "pppiiii" + "pppii" + "iii" + "pppppp")(
+        check(_entry("yalis_packed_unpack", "pppiiii" + "pppii" + "iii" + "ppppipp")(
             *held, positions, starts, row, table_width, m, width, window, skip_single, k_at, v_at, table_at, work.data_ptr(),
-            _address(error_flag), raw), name)
+            3 + 4 * items, _address(error_flag), raw), name)
         check(_entry("yalis_prefill_attention_tcgen05_unpacked", "plplpp" + "pppiii" + "iiiiii" + "fiiiippppp")(
             q.data_ptr(), steps[0], out.data_ptr(), steps[1], k_at, v_at, positions, starts, table_at, width, UNPACK_PAGE, m * width, n, m,
             max_q_len, num_heads, g, dim, scale, window, splits, share, skip_single, _address(lse2), _address(scratch), work.data_ptr(),
             _address(error_flag), raw), name)
         if weight_sums is not None:
-            check(_entry("yalis_packed_sums_tcgen05", "plpiiiii" + "pppiiiiifii" + "pppp")(
+            check(_entry("yalis_packed_sums_tcgen05", "plpiiiii" + "pppiiiiifii" + "ppiipppp")(
                 q.data_ptr(), steps[0], k_at, width, held[3], held[4], g, dim, positions, starts, row, table_width, m, n, max_kv_len, num_heads, scale,
-                window, skip_single, lse2.data_ptr(), weight_sums.data_ptr(), _address(error_flag), raw), name)
+                window, skip_single, lse2.data_ptr(), weight_sums.data_ptr(), each, parts, _address(partial), work.data_ptr() + 8, _address(error_flag), raw), name)
 
 
 def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tensor, q_start: torch.Tensor, block_table: torch.Tensor,

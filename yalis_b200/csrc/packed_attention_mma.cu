@@ -45,6 +45,8 @@ struct MmaParams {
   int only_single;             // 1: requests that bring more than one token are left to another kernel
   float scale_log2;
   float* lse2;                 // [N, nh] the logarithm to base two of a row's sum of exponentials, or null
+  float* scores;               // [N, nh, score_stride] every score in powers of two, by place (those that some row of the pair sees), or null
+  long long score_stride;
   float* part;                 // [blocks, 2, MT * 32 * 4 + 16 NT * 2]
   int32_t* tickets;            // one per pair, zero before and after
   int32_t* error;
@@ -149,7 +151,8 @@ __device__ __forceinline__ Deal choose_deal(int grid, int pairs, int most, long 
   return {0, even_blocks};
 }
 
-template <typename T, int DIM, int NT, int PARTS>
+// SCORES: every score is left in memory as well (a branch on the pointer in the one kernel cost 3 % of the steps that want none).
+template <typename T, int DIM, int NT, int PARTS, bool SCORES>
 __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packed_attention_mma_kernel(const MmaParams p) {
   constexpr int W = DIM / 32;                  // words of a K row that a lane takes
   constexpr int U = DIM / 64;                  // words of a V row that a lane takes
@@ -462,6 +465,24 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       }
       auto weigh = [&](auto mask) {              // sc: products in, weights times the values' steps out
         constexpr bool MASK = decltype(mask)::value;
+        if constexpr (SCORES) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int column = column0 + nt * 8 + 2 * t + x;
+              if (column >= n_rows) continue;
+              float* to = p.scores + ((size_t)(tok0 + column / p.per) * p.nh + kvh * p.per + column % p.per) * p.score_stride + key0;
+#pragma unroll
+              for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int j = half * 16 + key_of_row<DIM>(g) + 8 * e;
+                  if (!MASK || key0 + j <= see_hi[nt][x])
+                    to[j] = MASK && term[half][e].x == 0.f ? -INFINITY : term[half][e].x * sc[nt][half][2 * e + x];
+                }
+            }
+        }
         float most[NT][2];
         auto scores = [&](float (&to)[NT][2][4]) {
 #pragma unroll
@@ -722,12 +743,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
   }
 }
 
-template <typename T, int DIM, int NT, int PARTS>
-int launch_mma(const MmaParams& p, int grid, cudaStream_t stream) {
+template <typename T, int DIM, int NT, int PARTS, bool SCORES>
+int launch_mma_as(const MmaParams& p, int grid, cudaStream_t stream) {
   constexpr int MT = DIM / 16;
   const size_t smem = sizeof(Stage<DIM>) * kStages * kWarps + kWarps * kChunk * 16 + (size_t)kWarps * NT * MT * 512 + (size_t)kWarps * 8 * NT * 8 + 16 +
                       (size_t)(p.n_requests + 1) * 12;
-  auto* kernel = packed_attention_mma_kernel<T, DIM, NT, PARTS>;
+  auto* kernel = packed_attention_mma_kernel<T, DIM, NT, PARTS, SCORES>;
   static int configured[64] = {0};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return YALIS_ERR_LAUNCH;
@@ -737,6 +758,11 @@ int launch_mma(const MmaParams& p, int grid, cudaStream_t stream) {
     if (dev >= 0 && dev < 64) configured[dev] = (int)smem;
   }
   return yalis_launch(kernel, dim3(grid), dim3(kThreads), smem, stream, p);
+}
+
+template <typename T, int DIM, int NT, int PARTS>
+int launch_mma(const MmaParams& p, int grid, cudaStream_t stream) {
+  return p.scores ? launch_mma_as<T, DIM, NT, PARTS, true>(p, grid, stream) : launch_mma_as<T, DIM, NT, PARTS, false>(p, grid, stream);
 }
 
 }  // namespace
@@ -754,8 +780,8 @@ YALIS_API long long yalis_packed_attention_mma_scratch_floats(int blocks, int di
 YALIS_API int yalis_packed_attention_mma(const void* q, long long q_stride, int dtype, void* out, long long out_stride, void* k_codes,
                                          void* v_codes, void* words, int num_pages, int page_size, int g, int dim, const int32_t* positions,
                                          const int32_t* q_start, const int32_t* block_table, int table_width, int n_requests, int nh,
-                                         int columns, int q_vector, int only_single, float scale, int window, float* lse2, int blocks,
-                                         float* scratch, int32_t* tickets, int32_t* error, cudaStream_t stream) {
+                                         int columns, int q_vector, int only_single, float scale, int window, float* lse2, float* scores,
+                                         long long score_stride, int blocks, float* scratch, int32_t* tickets, int32_t* error, cudaStream_t stream) {
   if ((dim != 64 && dim != 128) || nh % g || n_requests > 4096 || blocks < 1) return YALIS_ERR_SHAPE;
   if (n_requests <= 0) return YALIS_OK;
   MmaParams p = {};
@@ -765,7 +791,7 @@ YALIS_API int yalis_packed_attention_mma(const void* q, long long q_stride, int 
   p.page_shift = -1; p.together = page_size % kChunk == 0 ? 2 : page_size % (1024 / dim) == 0 ? 1 : 0;
   if ((page_size & (page_size - 1)) == 0)
     for (p.page_shift = 0; 1 << p.page_shift < page_size;) ++p.page_shift;
-  p.scale_log2 = scale * 1.4426950408889634f; p.lse2 = lse2; p.part = scratch; p.tickets = tickets; p.error = error;
+  p.scale_log2 = scale * 1.4426950408889634f; p.lse2 = lse2; p.scores = scores; p.score_stride = score_stride; p.part = scratch; p.tickets = tickets; p.error = error;
   p.pages = {static_cast<uint32_t*>(k_codes), static_cast<uint32_t*>(v_codes), static_cast<uint32_t*>(words), num_pages, page_size, g, dim};
   if (dtype == YALIS_BF16) {
     if (columns == 8) return dim == 64 ? launch_mma<__nv_bfloat16, 64, 1, 1>(p, blocks, stream) : launch_mma<__nv_bfloat16, 128, 1, 1>(p, blocks, stream);

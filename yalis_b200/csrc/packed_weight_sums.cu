@@ -5,8 +5,12 @@
 // every token's sum is one addition to memory, whatever the number of rows, and its order fixed: a warp keeps 32 keys' codes less
 // their zeros as bfloat16 operands in registers and walks the rows (columns of the product, see packed_attention_mma.cu) that see
 // any of the block's keys.  The rows' queries lie in shared memory in the operand's order, COLUMNS at a time, written from registers
-// that were loaded a round before.  With few columns (single tokens) the warps divide keys among them and stream; with many they also
-// divide the columns, and add up at the end.
+// that were loaded a round before.  Two groups of four warps have 32 keys each; the four divide the columns among them and add up at the
+// end.
+//
+// Steps of few rows (single tokens) leave their scores in memory while the attention computes them: a second kernel raises and adds them,
+// a thread per key.  That moves 8 bytes a row and key, where taking the products once more reads the keys' codes again (16 requests of
+// 2,000 to 4,000 tokens, 32 heads of 128 over 8: 58 us by products).
 #include "packed.cuh"
 
 namespace {
@@ -239,33 +243,84 @@ __global__ void __launch_bounds__(kThreads, 1) packed_weight_sums_kernel(const S
 }
 
 template <typename T, int DIM, int PARTS>
-int launch_sums(const SumsParams& p, int n_requests, int max_kv_len, int columns, cudaStream_t stream) {
-  const int keys = columns <= 16 ? 8 * kKeys : 2 * kKeys;
-  const dim3 grid(p.pages.g, n_requests, (max_kv_len + keys - 1) / keys);
+int launch_sums(const SumsParams& p, int n_requests, int max_kv_len, cudaStream_t stream) {
+  const dim3 grid(p.pages.g, n_requests, (max_kv_len + 2 * kKeys - 1) / (2 * kKeys));
   if (grid.y > 65535 || grid.z > 65535) return YALIS_ERR_SHAPE;
-  return columns <= 16 ? yalis_launch(packed_weight_sums_kernel<T, DIM, PARTS, 8, 1, 16>, grid, dim3(kThreads), 0, stream, p)
-                       : yalis_launch(packed_weight_sums_kernel<T, DIM, PARTS, 2, 4, 64 / (PARTS == 1 ? 1 : 2)>, grid, dim3(kThreads), 0, stream, p);
+  return yalis_launch(packed_weight_sums_kernel<T, DIM, PARTS, 2, 4, 64 / (PARTS == 1 ? 1 : 2)>, grid, dim3(kThreads), 0, stream, p);
+}
+
+// From scores: a thread per key of a KV head, over the rows that see it in their order.
+__global__ void __launch_bounds__(256) packed_sums_of_scores_kernel(const SumsParams p, const float* scores, long long stride) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int key = blockIdx.x * 256 + threadIdx.x, kvh = blockIdx.y, req = blockIdx.z;
+  const int tok0 = p.q_start[req], n = p.q_start[req + 1] - tok0;
+  if (n <= 0 || (p.only_single && n > 1)) return;
+  const int last = p.positions[tok0 + n - 1], begin = p.positions[tok0];
+  if (key > last || (p.window > 0 && key <= begin - p.window)) return;
+  int row;
+  const int page = page_of(p.pages, p.block_table + (size_t)req * p.table_width, p.table_width, key, row);
+  if (page < 0) return;
+  float total = 0.f;
+  for (int t = 0; t < n; ++t) {
+    const int place = p.positions[tok0 + t];
+    if (key > place || (p.window > 0 && key <= place - p.window)) continue;
+    const size_t first = (size_t)(tok0 + t) * p.nh + kvh * p.per;
+    for (int h = 0; h < p.per; h += 4) {
+      float x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = h + i < p.per ? scores[(first + h + i) * stride + key] - p.lse2[first + h + i] : -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) total += exp2f(x[i]);
+    }
+  }
+  atomicAdd(p.sums + row_index(p.pages, page, kvh, row), total);
 }
 
 }  // namespace
 
-// `columns`: the most query rows of a pair (tokens of a request times heads of a KV head).
+namespace {
+
+SumsParams params_of(const void* q, long long q_stride, int num_pages, int page_size, int g, int dim, const int32_t* positions,
+                     const int32_t* q_start, const int32_t* block_table, int table_width, int nh, float scale, int window, int only_single,
+                     float* lse2, float* sums) {
+  SumsParams p = {};
+  p.q = q; p.q_stride = q_stride; p.positions = positions; p.q_start = q_start; p.block_table = block_table; p.table_width = table_width;
+  p.nh = nh; p.per = nh / g; p.window = window; p.only_single = only_single; p.scale_log2 = scale * 1.4426950408889634f;
+  p.lse2 = lse2; p.sums = sums;
+  p.pages = {nullptr, nullptr, nullptr, num_pages, page_size, g, dim};
+  return p;
+}
+
+}  // namespace
+
 YALIS_API int yalis_packed_weight_sums(const void* q, long long q_stride, int dtype, void* k_codes, void* v_codes, void* words, int num_pages,
                                        int page_size, int g, int dim, const int32_t* positions, const int32_t* q_start,
                                        const int32_t* block_table, int table_width, int n_requests, int max_kv_len, int nh, float scale,
-                                       int window, int columns, int q_vector, int only_single, float* lse2, float* sums, cudaStream_t stream) {
-  if ((dim != 64 && dim != 128) || nh % g || page_size < 1) return YALIS_ERR_SHAPE;
+                                       int window, int q_vector, int only_single, float* lse2, float* sums, cudaStream_t stream) {
+  if ((dim != 64 && dim != 128) || g < 1 || nh % g || page_size < 1) return YALIS_ERR_SHAPE;
   if (n_requests <= 0 || max_kv_len <= 0) return YALIS_OK;
-  SumsParams p = {};
-  p.q = q; p.q_stride = q_stride; p.positions = positions; p.q_start = q_start; p.block_table = block_table; p.table_width = table_width;
-  p.nh = nh; p.per = nh / g; p.window = window; p.q_vector = q_vector; p.only_single = only_single; p.scale_log2 = scale * 1.4426950408889634f;
-  p.lse2 = lse2; p.sums = sums;
-  p.pages = {static_cast<uint32_t*>(k_codes), static_cast<uint32_t*>(v_codes), static_cast<uint32_t*>(words), num_pages, page_size, g, dim};
+  SumsParams p = params_of(q, q_stride, num_pages, page_size, g, dim, positions, q_start, block_table, table_width, nh, scale, window, only_single,
+                           lse2, sums);
+  p.q_vector = q_vector;
+  p.pages.k = static_cast<uint32_t*>(k_codes); p.pages.v = static_cast<uint32_t*>(v_codes); p.pages.words = static_cast<uint32_t*>(words);
   if (dtype == YALIS_BF16)
-    return dim == 64 ? launch_sums<__nv_bfloat16, 64, 1>(p, n_requests, max_kv_len, columns, stream)
-                     : launch_sums<__nv_bfloat16, 128, 1>(p, n_requests, max_kv_len, columns, stream);
+    return dim == 64 ? launch_sums<__nv_bfloat16, 64, 1>(p, n_requests, max_kv_len, stream)
+                     : launch_sums<__nv_bfloat16, 128, 1>(p, n_requests, max_kv_len, stream);
   if (dtype == YALIS_F32)
-    return dim == 64 ? launch_sums<float, 64, 3>(p, n_requests, max_kv_len, columns, stream)
-                     : launch_sums<float, 128, 3>(p, n_requests, max_kv_len, columns, stream);
+    return dim == 64 ? launch_sums<float, 64, 3>(p, n_requests, max_kv_len, stream) : launch_sums<float, 128, 3>(p, n_requests, max_kv_len, stream);
   return YALIS_ERR_DTYPE;
+}
+
+// The same from scores [N, nh, score_stride] that the attention of the step left (yalis_packed_attention_mma).
+YALIS_API int yalis_packed_sums_of_scores(float* scores, long long score_stride, int num_pages, int page_size, int g, int dim,
+                                          const int32_t* positions, const int32_t* q_start, const int32_t* block_table, int table_width,
+                                          int n_requests, int max_kv_len, int nh, int window, int only_single, float* lse2, float* sums,
+                                          cudaStream_t stream) {
+  if (g < 1 || g > 65535 || nh % g || page_size < 1 || n_requests > 65535) return YALIS_ERR_SHAPE;
+  if (n_requests <= 0 || max_kv_len <= 0) return YALIS_OK;
+  const SumsParams p = params_of(nullptr, 0, num_pages, page_size, g, dim, positions, q_start, block_table, table_width, nh, 1.f, window, only_single,
+                                 lse2, sums);
+  return yalis_launch(packed_sums_of_scores_kernel, dim3((max_kv_len + 255) / 256, g, n_requests), dim3(256), 0, stream, p, (const float*)scores,
+                      score_stride);
 }

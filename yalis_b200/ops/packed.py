@@ -8,14 +8,17 @@ key and as many for its value, per KV head.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 from typing import Optional, Sequence, Tuple
 
+import numpy as np
 import torch
 
 from ._lib import BF16, F32, KernelError, check, dtype_code, lib, need, stream
-from .attention import sm_count
+from .attention import (PREFILL_SPLIT_GAIN, PREFILL_SPLIT_MIN_TILES, PREFILL_SPLIT_START_UP, PREFILL_SPLIT_UNSHARED, _policy_lib,
+                        sm_count)
 
 _TYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 _entries = {}
@@ -185,6 +188,18 @@ def packed_kv_read(pages: PackedPages, positions: torch.Tensor, req_of_token: to
 UNPACK_ROWS = 64          # query rows of a pair (tokens * heads of a KV head) beyond which portions are unpacked for the prompt kernel
 UNPACK_PAGE = 64          # keys of a page of the unpacked pools
 UNPACK_BYTES = 2 << 30    # of unpacked keys and values at a time
+SCORE_BYTES = 1 << 30     # of scores that a step of few rows may leave for its sums; beyond, the products are taken once more
+
+
+@functools.lru_cache(maxsize=4096)
+def _portion_splits(portions: int, q_len: int, kv_len: int, per: int, g: int, sms: int) -> Tuple[int, int]:
+    """(shares of a tile's keys, tiles of keys of a share) for the prompt kernel, as the plain cache's steps choose them
+    (``prefill_kv_splits``), for ``portions`` portions of ``q_len`` tokens that end at place ``kv_len``."""
+    q_lens, before = (np.full(portions, v, dtype=np.int32) for v in (q_len, max(0, kv_len - q_len)))
+    out = np.ones(2, dtype=np.int32)
+    _policy_lib().ypol_kv_splits(q_lens.ctypes.data, before.ctypes.data, portions, 128 // per, max(1, 2 * sms // g), 0, PREFILL_SPLIT_MIN_TILES,
+                                 PREFILL_SPLIT_START_UP, PREFILL_SPLIT_UNSHARED, PREFILL_SPLIT_GAIN, out.ctypes.data)
+    return int(out[0]), int(out[1])
 
 
 def _attend_unpacked(name, q, out, held, at, steps, n, max_q_len, max_kv_len, num_heads, scale, window, skip_single, lse2,
@@ -197,11 +212,7 @@ def _attend_unpacked(name, q, out, held, at, steps, n, max_q_len, max_kv_len, nu
     rows = width * g * UNPACK_PAGE * dim                # of a request, keys or values
     group = max(1, min(r, UNPACK_BYTES // (4 * rows)))
     per = num_heads // g
-    tiles = min(r, group) * -(-max_q_len // (128 // per)) * g
-    splits, share = 1, 1
-    if window == 0:                                     # few tiles of queries with many keys: the keys of a tile in shares
-        splits = max(1, min(8, 2 * sm_count(q.device) // tiles, width // 16))
-        share = -(-width // splits)
+    splits, share = (1, 1) if window else _portion_splits(max(1, min(r, n // max(1, max_q_len))), max_q_len, max_kv_len, per, g, sm_count(q.device))
     need_floats = n * num_heads * splits * (dim + 2) if splits > 1 else 0
     pools = torch.empty(2 * group * rows, dtype=torch.bfloat16, device=q.device)
     items = -(-max_kv_len // 128) * group * g if weight_sums is not None else 0         # 128 keys of a KV head each
@@ -275,28 +286,34 @@ def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tenso
     per, aligned = num_heads // g, (q.data_ptr() | steps[0] * q.element_size()) % 16 == 0
     unpack = (code == BF16 and dim in (64, 128) and max_q_len * per > UNPACK_ROWS and per <= 128 and scale > 0 and aligned
               and (out.data_ptr() | steps[1] * 2) % 16 == 0)
-    mma = dim in (64, 128) and r <= 4096
+    mma, scores = dim in (64, 128) and r <= 4096, None
     single = unpack and mma and n > max_q_len          # single tokens may stand beside the portions: a kernel of their own
     if unpack:
         _attend_unpacked(name, q, out, held, at, steps, n, max_q_len, max_kv_len, num_heads, scale, window or 0, single, lse2, weight_sums,
                          error_flag, raw)
     if mma and (single or not unpack):
-        columns = 8 if code == F32 or (1 if single else max_q_len) * per <= 8 else 16
+        rows = (1 if single else max_q_len) * per
+        columns = 8 if code == F32 or rows <= 8 else 16
+        if weight_sums is not None and rows <= 16 and 4 * n * num_heads * max_kv_len <= SCORE_BYTES:
+            scores = torch.empty(n * num_heads * max_kv_len, dtype=torch.float32, device=q.device)
         blocks, floats = _mma_launch(q.device, code, dim, columns)
         scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
-        check(_entry("yalis_packed_attention_mma", "plipl" + "pppiiii" + "pppii" + "iiiifipipppp")(
+        check(_entry("yalis_packed_attention_mma", "plipl" + "pppiiii" + "pppii" + "iiiifipplipppp")(
             q.data_ptr(), steps[0], code, out.data_ptr(), steps[1], *held, *at, num_heads, columns, aligned, single, scale, window or 0,
-            _address(lse2), blocks, scratch.data_ptr(), _counters(blocks, q.device).data_ptr(), _address(error_flag), raw), name)
+            _address(lse2), _address(scores), max_kv_len, blocks, scratch.data_ptr(), _counters(blocks, q.device).data_ptr(), _address(error_flag), raw), name)
     if not mma and not unpack:
         check(_entry("yalis_packed_attention_general", "plipl" + "pppiiii" + "pppii" + "iifippp")(
             q.data_ptr(), steps[0], code, out.data_ptr(), steps[1], *held, *at, n, num_heads, scale, window or 0, _address(lse2),
             _address(error_flag), raw), name)
     if weight_sums is None or (unpack and not single):
         return out
-    if mma:
-        check(_entry("yalis_packed_weight_sums", "pli" + "pppiiii" + "pppii" + "iifiiiippp")(
-            q.data_ptr(), steps[0], code, *held, *at, max_kv_len, num_heads, scale, window or 0, (1 if single else max_q_len) * per, aligned, single,
-            lse2.data_ptr(), weight_sums.data_ptr(), raw), name)
+    if scores is not None:
+        check(_entry("yalis_packed_sums_of_scores", "pliiii" + "pppii" + "iiiippp")(
+            scores.data_ptr(), max_kv_len, *held[3:], *at, max_kv_len, num_heads, window or 0, single, lse2.data_ptr(), weight_sums.data_ptr(), raw), name)
+    elif mma:
+        check(_entry("yalis_packed_weight_sums", "pli" + "pppiiii" + "pppii" + "iifiiippp")(
+            q.data_ptr(), steps[0], code, *held, *at, max_kv_len, num_heads, scale, window or 0, aligned, single, lse2.data_ptr(),
+            weight_sums.data_ptr(), raw), name)
     else:
         check(_entry("yalis_packed_weight_sums_general", "pli" + "pppiiii" + "pppii" + "iifippp")(
             q.data_ptr(), steps[0], code, *held, *at, max_kv_len, num_heads, scale, window or 0, lse2.data_ptr(), weight_sums.data_ptr(), raw), name)

@@ -12,7 +12,7 @@ def test_refused_before_anything_is_launched(monkeypatch):
     def launched():
         raise AssertionError("an argument that should have been refused reached the library")
 
-    monkeypatch.setattr(packed, "_need_here", lambda *a: None)
+    monkeypatch.setattr(packed, "_need_here", lambda *a: "cpu")
     monkeypatch.setattr(packed, "lib", launched)
     for what, call in refusals("cpu"):
         with pytest.raises(KernelError):

@@ -52,13 +52,20 @@ __device__ __forceinline__ float step_for(float lo, float hi) {
   return fmaxf(step, kPackedLeast);
 }
 
-// rint(x / step): the quotient's own rounding may land on a tie that the exact one misses by less; what is left over after the
-// rounded multiple is exact and says so.
-__device__ __forceinline__ float multiple_of(float x, float step) {
-  float n = rintf(__fdiv_rn(x, step));
-  const float left = fmaf(-n, step, x), half = 0.5f * step;
-  if (left > half) n += 1.f;
-  if (left < -half) n -= 1.f;
+// 2^22 + n + 2^23 for n = rint(x / step), the whole number in its lowest bits; `inverse` is 1 / step, rounded.  One step of
+// refinement makes the product the rounded quotient (what it leaves is exact), so that ties are ties.  For bfloat16 values that is
+// all: their quotients by four bits are ties or stand well apart from them.  A float32 quotient may round to a tie that the exact one
+// misses by less; what is left over after the multiple is exact and says so.
+template <bool EXACT>
+__device__ __forceinline__ float multiple_of(float x, float step, float inverse) {
+  constexpr float kWhole = 12582912.f;                        // 1.5 * 2^23: sums with it are whole numbers, ties to even
+  const float near = x * inverse;
+  float n = fmaf(fmaf(-near, step, x), inverse, near) + kWhole;
+  if constexpr (EXACT) {
+    const float left = fmaf(-(n - kWhole), step, x), half = 0.5f * step;
+    if (left > half) n += 1.f;
+    if (left < -half) n -= 1.f;
+  }
   return n;
 }
 

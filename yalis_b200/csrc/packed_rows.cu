@@ -1,13 +1,13 @@
 // Rows of keys and values into pages held in 4 bits, and back.
 //
 // A row of one token and KV head is taken by dim / 8 neighbouring lanes (a group of 4, 8, 16 or 32), eight values a lane: the
-// row's extremes by shuffles, then every lane its word of eight codes.  Keys and values are rows of one grid.
+// row's extremes by shuffles, then every lane its word of eight codes.  A block takes rows of one token (keys and values are rows
+// of one list), so that the token's place is looked up without a division a thread; of many tokens it takes TOKENS side by side, whose
+// look-ups (token, page, row: three trips to memory one after the other) overlap.
 // Bound by memory: 2 dim values read and dim + 4 bytes written a token and KV head (bfloat16: 512 -> 132 B at 128).
 #include "packed.cuh"
 
 namespace {
-
-constexpr int kThreads = 128;
 
 template <typename T>
 struct RowParams {
@@ -20,7 +20,7 @@ struct RowParams {
   const int32_t* req_of_token; // [N] row of the block table, -1: not a token
   const int32_t* block_table;
   int table_width, n_tokens;
-  int vector;                  // 1: rows start on boundaries of eight values
+  int vector;                  // 1: rows start on boundaries of 16 bytes
   int32_t* error;
   PackedPages pages;
 };
@@ -28,122 +28,148 @@ struct RowParams {
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, bool vector, float (&x)[8]) {
   if (vector) {
-    const float4 a = load4_f32(p), b = load4_f32(p + 4);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    if constexpr (sizeof(T) == 2) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      }
+    } else {
+      const float4 a = load4_f32(p), b = load4_f32(p + 4);
+      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+      x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(p[i]);
   }
 }
 
-// What a group of lanes works on: row `index` of the grid is token index / (2 g), KV head and key or value from the rest.
-struct Place {
-  int token, kvh, is_v;
-  bool real;                   // a token with a page
-  size_t row;
-};
-
+// The pool's row of a KV head of a token, -1 where the token is none or has no page.
 template <typename T>
-__device__ __forceinline__ Place place_of(const RowParams<T>& p, long long index, int lane_in_row) {
-  Place o;
-  const int per_token = 2 * p.pages.g;
-  o.token = (int)(index / per_token);
-  const int rest = (int)(index - (long long)o.token * per_token);
-  o.is_v = rest & 1;
-  o.kvh = rest >> 1;
-  o.real = o.token < p.n_tokens;
-  o.row = 0;
-  if (o.real) {
-    const int req = p.req_of_token[o.token], at = p.positions[o.token];
-    o.real = req >= 0 && at >= 0;
-    if (o.real) {
-      int row;
-      const int page = page_of(p.pages, p.block_table + (size_t)req * p.table_width, p.table_width, at, row);
-      if (page < 0) {
-        o.real = false;
-        if (lane_in_row == 0 && p.error) atomicOr(p.error, YALIS_FLAG_BAD_PAGE);
-      } else {
-        o.row = row_index(p.pages, page, o.kvh, row);
+__device__ __forceinline__ long long place_of(const RowParams<T>& p, int token, int kvh, bool tells) {
+  const int req = p.req_of_token[token], at = p.positions[token];
+  if (req < 0 || at < 0) return -1;
+  int row;
+  const int page = page_of(p.pages, p.block_table + (size_t)req * p.table_width, p.table_width, at, row);
+  if (page >= 0) return (long long)row_index(p.pages, page, kvh, row);
+  if (tells && p.error) atomicOr(p.error, YALIS_FLAG_BAD_PAGE);
+  return -1;
+}
+
+template <typename T, int LANES, int TOKENS>
+__global__ void packed_rows_write_kernel(const RowParams<T> p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & (LANES - 1), group = (blockIdx.y * blockDim.x + threadIdx.x) / LANES, is_v = group & 1, kvh = group >> 1;
+  const bool listed = kvh < p.pages.g && lane * 8 < p.pages.dim;
+  float x[TOKENS][8];
+  long long row[TOKENS];
+#pragma unroll
+  for (int i = 0; i < TOKENS; ++i) {
+    const int token = blockIdx.x * TOKENS + i;
+    row[i] = -1;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[i][j] = 0.f;
+    if (listed && token < p.n_tokens) {
+      const T* src = is_v ? p.v + (long long)token * p.v_stride : p.k + (long long)token * p.k_stride;
+      load8<T>(src + (size_t)kvh * p.pages.dim + lane * 8, p.vector, x[i]);
+      row[i] = place_of(p, token, kvh, group == 0 && lane == 0);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TOKENS; ++i) {
+    float lo = 0.f, hi = 0.f, odd = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      lo = fminf(lo, x[i][j]);
+      hi = fmaxf(hi, x[i][j]);
+      odd = fmaf(x[i][j], 0.f, odd);                          // not a number where x is none, or infinite
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      odd += __shfl_xor_sync(0xffffffffu, odd, o);
+    }
+    if (row[i] < 0) continue;
+    uint32_t codes = 0, word = 0x7FC0u;                       // not a number: all codes 0
+    if (odd == 0.f && fmaxf(hi, -lo) <= kPackedLargest) {
+      const float step = step_for(lo, hi), inverse = __frcp_rn(step);
+      const float first = multiple_of<sizeof(T) == 4>(lo, step, inverse);
+#pragma unroll
+      for (int j = 7; j >= 0; --j) {                          // (no value lies below the row's least)
+        const int c = __float_as_int(multiple_of<sizeof(T) == 4>(x[i][j], step, inverse)) - __float_as_int(first);
+        codes = codes << 4 | (uint32_t)min(c, 15);
       }
+      word = (__float_as_uint(step) >> 16) | (uint32_t)(__float_as_int(12582912.f) - __float_as_int(first));
     }
+    (is_v ? p.pages.v : p.pages.k)[row[i] * (p.pages.dim / 8) + lane] = codes;
+    if (lane == 0) reinterpret_cast<uint16_t*>(p.pages.words + row[i])[is_v] = (uint16_t)word;
   }
-  return o;
 }
 
-template <typename T, int LANES>
-__global__ void __launch_bounds__(kThreads) packed_rows_write_kernel(const RowParams<T> p) {
+template <typename T, int LANES, int TOKENS>
+__global__ void packed_rows_read_kernel(const RowParams<T> p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & (LANES - 1);
-  const long long index = ((long long)blockIdx.x * kThreads + threadIdx.x) / LANES;
-  const Place at = place_of(p, index, lane);
-  const bool mine = at.real && lane * 8 < p.pages.dim;
-  float x[8];
-  if (mine) {
-    const T* src = at.is_v ? p.v + (long long)at.token * p.v_stride : p.k + (long long)at.token * p.k_stride;
-    load8<T>(src + (size_t)at.kvh * p.pages.dim + lane * 8, p.vector, x);
-  }
-  float lo = 0.f, hi = 0.f;
-  int odd = 0;
-  if (mine) {
+  const int lane = threadIdx.x & (LANES - 1), group = (blockIdx.y * blockDim.x + threadIdx.x) / LANES, is_v = group & 1, kvh = group >> 1;
+  if (kvh >= p.pages.g || lane * 8 >= p.pages.dim) return;
+  long long row[TOKENS];
+  uint32_t codes[TOKENS], word[TOKENS];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      lo = fminf(lo, x[i]);
-      hi = fmaxf(hi, x[i]);
-      odd |= !(fabsf(x[i]) <= kPackedLargest);
+  for (int i = 0; i < TOKENS; ++i) {
+    const int token = blockIdx.x * TOKENS + i;
+    row[i] = token < p.n_tokens ? place_of(p, token, kvh, group == 0 && lane == 0) : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < TOKENS; ++i) {
+    codes[i] = word[i] = 0u;                                  // a token without a page reads as zeros
+    if (row[i] >= 0) {
+      codes[i] = (is_v ? p.pages.v : p.pages.k)[row[i] * (p.pages.dim / 8) + lane];
+      word[i] = reinterpret_cast<const uint16_t*>(p.pages.words + row[i])[is_v];
     }
   }
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    odd |= __shfl_xor_sync(0xffffffffu, odd, o);
-  }
-  if (!mine) return;
-  uint32_t codes = 0, word = 0x7FC0u;                          // not a number: all codes 0
-  if (!odd) {
-    const float step = step_for(lo, hi), first = multiple_of(lo, step);
+  for (int i = 0; i < TOKENS; ++i) {
+    const int token = blockIdx.x * TOKENS + i;
+    if (token >= p.n_tokens) return;
+    const float step = step_of(word[i]), zero = zero_of(word[i]);
+    float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int c = (int)fminf(multiple_of(x[i], step) - first, 15.f);
-      codes |= (uint32_t)max(c, 0) << (4 * i);
+    for (int j = 0; j < 8; ++j) x[j] = ((float)((codes[i] >> (4 * j)) & 15u) - zero) * step;
+    T* dst = (is_v ? p.v_out : p.k_out) + ((size_t)token * p.pages.g + kvh) * p.pages.dim + lane * 8;
+    if constexpr (sizeof(T) == 2) {
+      uint4 u;
+      uint32_t* w = &u.x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const __nv_bfloat162 two = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+        w[j] = *reinterpret_cast<const uint32_t*>(&two);
+      }
+      *reinterpret_cast<uint4*>(dst) = u;
+    } else {
+      store4(dst, make_float4(x[0], x[1], x[2], x[3]));
+      store4(dst + 4, make_float4(x[4], x[5], x[6], x[7]));
     }
-    word = (__float_as_uint(step) >> 16) | (uint32_t)(int)-first;
   }
-  (at.is_v ? p.pages.v : p.pages.k)[at.row * (p.pages.dim / 8) + lane] = codes;
-  if (lane == 0) reinterpret_cast<uint16_t*>(p.pages.words + at.row)[at.is_v] = (uint16_t)word;
-}
-
-template <typename T, int LANES>
-__global__ void __launch_bounds__(kThreads) packed_rows_read_kernel(const RowParams<T> p) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const int lane = threadIdx.x & (LANES - 1);
-  const long long index = ((long long)blockIdx.x * kThreads + threadIdx.x) / LANES;
-  const Place at = place_of(p, index, lane);
-  if (at.token >= p.n_tokens || lane * 8 >= p.pages.dim) return;
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};       // a token without a page reads as zeros
-  if (at.real) {
-    const uint32_t codes = (at.is_v ? p.pages.v : p.pages.k)[at.row * (p.pages.dim / 8) + lane];
-    const uint32_t word = reinterpret_cast<const uint16_t*>(p.pages.words + at.row)[at.is_v];
-    const float step = step_of(word), zero = zero_of(word);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = ((float)((codes >> (4 * i)) & 15u) - zero) * step;
-  }
-  T* dst = (at.is_v ? p.v_out : p.k_out) + ((size_t)at.token * p.pages.g + at.kvh) * p.pages.dim + lane * 8;
-  store4(dst, make_float4(x[0], x[1], x[2], x[3]));
-  store4(dst + 4, make_float4(x[4], x[5], x[6], x[7]));
 }
 
 template <typename T, bool WRITE>
-int launch_rows(const RowParams<T>& p, cudaStream_t stream) {
+int launch_rows(const RowParams<T>& p, int n_tokens, cudaStream_t stream) {
   const int lanes = p.pages.dim <= 32 ? 4 : p.pages.dim <= 64 ? 8 : p.pages.dim <= 128 ? 16 : 32;
-  const long long rows = (long long)p.n_tokens * p.pages.g * 2, per_block = kThreads / lanes, blocks = (rows + per_block - 1) / per_block;
-  if (blocks > 0x7fffffffll) return YALIS_ERR_SHAPE;
-  const dim3 grid((unsigned)blocks), block(kThreads);
-#define YALIS_ROWS(L) \
-  yalis_launch(WRITE ? packed_rows_write_kernel<T, L> : packed_rows_read_kernel<T, L>, grid, block, 0, stream, p)
+  const long long threads = 2LL * p.pages.g * lanes;          // of a token
+  const int block = (int)(threads >= 256 ? 256 : (threads + 31) / 32 * 32);
+  const long long per_token = (threads + block - 1) / block;
+  if (per_token > 65535) return YALIS_ERR_SHAPE;
+  // One token a block while its blocks fit the GPU at once about twice over, else four.
+  const bool many = (long long)n_tokens * per_token * block > 4096LL * yalis_sm_count();
+  const dim3 grid((unsigned)(many ? (n_tokens + 3) / 4 : n_tokens), (unsigned)per_token);
+#define YALIS_ROWS(L)                                                                                                              \
+  (many ? yalis_launch(WRITE ? packed_rows_write_kernel<T, L, 4> : packed_rows_read_kernel<T, L, 4>, grid, dim3(block), 0, stream, p) \
+        : yalis_launch(WRITE ? packed_rows_write_kernel<T, L, 1> : packed_rows_read_kernel<T, L, 1>, grid, dim3(block), 0, stream, p))
   switch (lanes) {
     case 4: return YALIS_ROWS(4);
     case 8: return YALIS_ROWS(8);
@@ -232,7 +258,7 @@ YALIS_API int yalis_packed_rows(int write, void* k, void* v, long long k_stride,
     p.positions = positions; p.req_of_token = req_of_token; p.block_table = block_table;
     p.table_width = table_width; p.n_tokens = n_tokens; p.vector = vector; p.error = error;
     p.pages = {static_cast<uint32_t*>(k_codes), static_cast<uint32_t*>(v_codes), static_cast<uint32_t*>(words), num_pages, page_size, g, dim};
-    return write ? launch_rows<T, true>(p, stream) : launch_rows<T, false>(p, stream);
+    return write ? launch_rows<T, true>(p, n_tokens, stream) : launch_rows<T, false>(p, n_tokens, stream);
   });
 }
 

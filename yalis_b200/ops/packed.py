@@ -16,7 +16,7 @@ from typing import Optional, Sequence, Tuple
 import numpy as np
 import torch
 
-from ._lib import BF16, F32, KernelError, check, dtype_code, lib, need, stream
+from ._lib import BF16, F32, KernelError, check, dtype_code, lib, need
 from .attention import (PREFILL_SPLIT_GAIN, PREFILL_SPLIT_MIN_TILES, PREFILL_SPLIT_START_UP, PREFILL_SPLIT_UNSHARED, _policy_lib,
                         sm_count)
 
@@ -69,17 +69,22 @@ class PackedPages:
         return self.k, self.v, self.words
 
 
-def _need_here(name: str, *tensors: Optional[torch.Tensor]) -> None:
-    """Every tensor on the current device, whose stream the kernels are launched on."""
-    here = -1
+def _need_here(name: str, *tensors: Optional[torch.Tensor]) -> int:
+    """Every tensor on the current device, whose stream the kernels are launched on; returns its number."""
+    here = -2
     for t in tensors:
         if t is not None:
             at = t.get_device()
-            if at < 0:
-                raise KernelError(f"{name}: every tensor must be on the GPU (there is no CPU path)")
-            if at != here and (here >= 0 or at != torch.cuda.current_device()):
-                raise KernelError(f"{name}: every tensor must be on the current device")
-            here = at
+            if at != here:
+                if at < 0:
+                    raise KernelError(f"{name}: every tensor must be on the GPU (there is no CPU path)")
+                if here >= 0 or at != torch.cuda.current_device():
+                    raise KernelError(f"{name}: every tensor must be on the current device")
+                here = at
+    return here
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _address(t: Optional[torch.Tensor]) -> int:
@@ -92,7 +97,7 @@ def _pages_arguments(name: str, pages: PackedPages):
     if not (k.dtype is torch.uint8 and v.dtype is torch.uint8 and len(shape) == 4 and v.shape == shape and k.is_contiguous() and v.is_contiguous()):
         raise KernelError(f"{name}: codes must be contiguous uint8 [pages, kv_heads, page_size, head_dim / 2]")
     num_pages, g, page_size, half = shape
-    if not (words.dtype is torch.int16 and words.shape == (num_pages, g, page_size, 2) and words.is_contiguous()):
+    if not (words.dtype is torch.int16 and words.shape == shape[:3] + (2,) and words.is_contiguous()):
         raise KernelError(f"{name}: words must be contiguous int16 [pages, kv_heads, page_size, 2]")
     if half % 4 or not 4 <= half <= 128:
         raise KernelError(f"{name}: head_dim {2 * half} must be a multiple of 8 up to 256")
@@ -104,39 +109,45 @@ def _pages_arguments(name: str, pages: PackedPages):
     return at + (num_pages, page_size, g, 2 * half)
 
 
-def _check_index(name: str, n: int, block_table: torch.Tensor, *per_token: torch.Tensor) -> None:
+def _check_index(name: str, n: int, block_table: torch.Tensor, *per_token: torch.Tensor) -> Tuple[int, int]:
+    """Checks the arrays of a step's tokens and the block table, whose (rows, columns) it returns."""
     for t in per_token:
-        if not (t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous()):
+        if not (t.dtype is torch.int32 and t.dim() == 1 and t.shape[0] == n and t.is_contiguous()):
             raise KernelError(f"{name}: positions/req_of_token: int32 [N]")
     if not (block_table.dtype is torch.int32 and block_table.dim() == 2 and block_table.is_contiguous()):
         raise KernelError(f"{name}: block_table must be contiguous int32 [R, width]")
+    return block_table.shape
 
 
-def _check_flag(name: str, error_flag: Optional[torch.Tensor]) -> None:
-    need(error_flag is None or (error_flag.dtype == torch.int32 and error_flag.numel() >= 1), name, "the error word must be int32")
+def _flag_address(name: str, error_flag: Optional[torch.Tensor]) -> int:
+    if error_flag is None:
+        return 0
+    need(error_flag.dtype == torch.int32 and error_flag.numel() >= 1, name, "the error word must be int32")
+    return error_flag.data_ptr()
 
 
-_counters_of_stream = {}
+_workspaces = {}
 
 
-def _counters(n: int, device: torch.device) -> torch.Tensor:
-    """Zeroed int32 counters, which every launch leaves at zero: one buffer per stream, whose launches run one after the other; a
-    recording, which may be replayed on any stream, gets its own with every launch."""
+def _workspace(device: int, raw: int, counters: int, floats: int):
+    """(zeroed int32 counters, which every launch leaves at zero, scratch memory) for a launch on the current stream: kept per
+    stream, whose launches run one after the other; a recording, which may be replayed on any stream, gets its own with every
+    launch."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(n, dtype=torch.int32, device=device)
-    key = (device.index, stream().value)
-    held = _counters_of_stream.get(key)
-    if held is None or held.numel() < n:
-        held = _counters_of_stream[key] = torch.zeros(max(n, 2048), dtype=torch.int32, device=device)
+        return torch.zeros(counters, dtype=torch.int32, device=device), torch.empty(floats, dtype=torch.float32, device=device)
+    held = _workspaces.get((device, raw))
+    if held is None or held[0].shape[0] < counters or held[1].shape[0] < floats:
+        held = _workspaces[device, raw] = (torch.zeros(max(counters, 2048), dtype=torch.int32, device=device),
+                                           torch.empty(floats, dtype=torch.float32, device=device))
     return held
 
 
 _mma_launches = {}
 
 
-def _mma_launch(device: torch.device, code: int, dim: int, columns: int) -> Tuple[int, int]:
+def _mma_launch(device: int, code: int, dim: int, columns: int) -> Tuple[int, int]:
     """(blocks, floats of scratch memory) of the tensor-core kernel."""
-    key = (device.index, code, dim, columns)
+    key = (device, code, dim, columns)
     found = _mma_launches.get(key)
     if found is None:
         blocks = _entry("yalis_packed_attention_mma_blocks", "iii")(code, dim, columns)
@@ -152,16 +163,16 @@ def packed_kv_write(k: torch.Tensor, v: torch.Tensor, pages: PackedPages, positi
     ``req_of_token[n]`` (-1: nowhere).  No two tokens may share a place.  A token without a page is left out and raises the error
     word's bit.  Rows with a NaN, an infinity or a magnitude above 2^120 read back as NaN throughout."""
     name = "packed_kv_write"
-    _need_here(name, k, v, pages.k, pages.v, pages.words, positions, req_of_token, block_table, error_flag)
-    held, shape = _pages_arguments(name, pages), k.shape
-    if not (k.dtype is v.dtype and len(shape) == 2 and v.shape == shape and shape[1] == held[5] * held[6] and k.stride(1) == v.stride(1) == 1):
+    device = _need_here(name, k, v, pages.k, pages.v, pages.words, positions, req_of_token, block_table, error_flag)
+    held, shape, size, code = _pages_arguments(name, pages), k.shape, k.element_size(), dtype_code(k.dtype)
+    (k_step, k_unit), (v_step, v_unit) = (k.stride(), v.stride()) if k.dim() == v.dim() == 2 else ((0, 0), (0, 0))
+    if not (k.dtype is v.dtype and k_unit == v_unit == 1 and v.shape == shape and shape[1] == held[5] * held[6]):
         raise KernelError(f"{name}: k and v must be [N, kv_heads * head_dim] of one dtype with unit inner stride")
-    _check_index(name, shape[0], block_table, positions, req_of_token)
-    _check_flag(name, error_flag)
-    code, k_at, v_at, k_step, v_step, size = dtype_code(k.dtype), k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), k.element_size()
-    vector = (k_at | v_at | k_step * size | v_step * size) % 16 == 0
-    check(_rows_entry()(1, k_at, v_at, k_step, v_step, code, *held, positions.data_ptr(), req_of_token.data_ptr(), block_table.data_ptr(),
-                        block_table.shape[1], shape[0], vector, _address(error_flag), stream()), name)
+    _, columns = _check_index(name, shape[0], block_table, positions, req_of_token)
+    flag, k_at, v_at = _flag_address(name, error_flag), k.data_ptr(), v.data_ptr()
+    check(_rows_entry()(1, k_at, v_at, k_step, v_step, code, *held, positions.data_ptr(), req_of_token.data_ptr(),
+                        block_table.data_ptr(), columns, shape[0], (k_at | v_at | k_step * size | v_step * size) % 16 == 0, flag,
+                        _raw_stream(device)), name)
 
 
 def _rows_entry():
@@ -174,15 +185,15 @@ def packed_kv_read(pages: PackedPages, positions: torch.Tensor, req_of_token: to
     ``req_of_token``: what ``packed_kv_write`` left there, exactly.  Tokens of no request (-1) and tokens without a page (which
     raise the error word's bit) read as zeros."""
     name = "packed_kv_read"
-    _need_here(name, pages.k, pages.v, pages.words, positions, req_of_token, block_table, error_flag)
-    held, n, code = _pages_arguments(name, pages), positions.shape[0], dtype_code(dtype)
-    _check_index(name, n, block_table, positions, req_of_token)
-    _check_flag(name, error_flag)
-    width = held[5] * held[6]
-    k, v = torch.empty((n, width), dtype=dtype, device=positions.device), torch.empty((n, width), dtype=dtype, device=positions.device)
-    check(_rows_entry()(0, k.data_ptr(), v.data_ptr(), width, width, code, *held, positions.data_ptr(), req_of_token.data_ptr(),
-                        block_table.data_ptr(), block_table.shape[1], n, True, _address(error_flag), stream()), name)
-    return k, v
+    device = _need_here(name, pages.k, pages.v, pages.words, positions, req_of_token, block_table, error_flag)
+    held, n, code = _pages_arguments(name, pages), positions.shape[0] if positions.dim() else -1, dtype_code(dtype)
+    _, columns = _check_index(name, n, block_table, positions, req_of_token)
+    flag, width = _flag_address(name, error_flag), held[5] * held[6]
+    both = torch.empty((2, n, width), dtype=dtype, device=device)        # one allocation
+    at = both.data_ptr()
+    check(_rows_entry()(0, at, at + n * width * both.element_size(), width, width, code, *held, positions.data_ptr(), req_of_token.data_ptr(),
+                        block_table.data_ptr(), columns, n, True, flag, _raw_stream(device)), name)
+    return both.unbind(0)
 
 
 UNPACK_ROWS = 64          # query rows of a pair (tokens * heads of a KV head) beyond which portions are unpacked for the prompt kernel
@@ -202,42 +213,40 @@ def _portion_splits(portions: int, q_len: int, kv_len: int, per: int, g: int, sm
     return int(out[0]), int(out[1])
 
 
-def _attend_unpacked(name, q, out, held, at, steps, n, max_q_len, max_kv_len, num_heads, scale, window, skip_single, lse2,
-                     weight_sums, error_flag, raw):
-    """Portions of prompts: the rows that they see are unpacked, as many requests at a time as ``UNPACK_BYTES`` hold, into pools of
-    the call for the prompt kernel on the tcgen05 tensor cores (every value is a bfloat16 number, so nothing is rounded)."""
+def _attend_unpacked(name, device, rows, held, at, n, max_q_len, max_kv_len, num_heads, scale, window, skip_single, lse2, weight_sums, flag, raw):
+    """Portions of prompts: what they see is unpacked, as many requests at a time as ``UNPACK_BYTES`` hold, into pools of the call
+    for the prompt kernel on the tcgen05 tensor cores (every value is a bfloat16 number, so nothing is rounded)."""
     g, dim = held[5:]
     positions, q_start, table, table_width, r = at
-    width = max(1, -(-max_kv_len // UNPACK_PAGE))
-    rows = width * g * UNPACK_PAGE * dim                # of a request, keys or values
-    group = max(1, min(r, UNPACK_BYTES // (4 * rows)))
-    per = num_heads // g
-    splits, share = (1, 1) if window else _portion_splits(max(1, min(r, n // max(1, max_q_len))), max_q_len, max_kv_len, per, g, sm_count(q.device))
-    need_floats = n * num_heads * splits * (dim + 2) if splits > 1 else 0
-    pools = torch.empty(2 * group * rows, dtype=torch.bfloat16, device=q.device)
-    items = -(-max_kv_len // 128) * group * g if weight_sums is not None else 0         # 128 keys of a KV head each
-    tiles_seen = -(-max_q_len // (128 // per))          # tiles of rows that see an item, at most; about half of them on average
-    each = max(16, items * tiles_seen // (8 * sm_count(q.device)))
-    parts = -(-tiles_seen // each)
-    work = torch.empty(group * width + 3 + 4 * items, dtype=torch.int32, device=q.device)   # counters (two of the prompt kernel's), block table
-    partial = torch.empty(items * parts * 3 * 128, dtype=torch.float32, device=q.device) if items else None
-    scratch = torch.empty(need_floats, dtype=torch.float32, device=q.device) if need_floats else None
-    k_at, table_at = pools.data_ptr(), work.data_ptr() + 4 * (3 + 4 * items)
-    v_at = k_at + 2 * group * rows
+    width, per, sms = max(1, -(-max_kv_len // UNPACK_PAGE)), num_heads // g, sm_count(device)
+    size = width * g * UNPACK_PAGE * dim                # of a request's keys, or values
+    group = max(1, min(r, UNPACK_BYTES // (4 * size)))
+    splits, share = (1, 1) if window else _portion_splits(max(1, min(r, n // max_q_len)), max_q_len, max_kv_len, per, g, sms)
+    items = -(-max_kv_len // 128) * group * g if lse2 is not None else 0                # sums: 128 keys of a KV head each
+    tiles = -(-max_q_len // (128 // per))               # tiles of rows that see an item, at most; about half of them on average
+    each = max(16, items * tiles // (8 * sms))
+    parts = -(-tiles // each)
+    # pools, counters (two of the prompt kernel's, one and four an item of the sums'), block table, shares of outputs and of sums
+    floats = n * num_heads * splits * (dim + 2) if splits > 1 else 0
+    pools = torch.empty(2 * group * size, dtype=torch.bfloat16, device=device)
+    n_counters = (3 + 4 * items + 3) // 4 * 4
+    work = torch.empty(floats + items * parts * 384 + n_counters + group * width, dtype=torch.int32, device=device)
+    k_at, scratch = pools.data_ptr(), work.data_ptr()
+    v_at, partial = k_at + 2 * group * size, scratch + 4 * floats
+    counters = partial + 4 * items * parts * 384
+    table_at = counters + 4 * n_counters
     for first in range(0, r, group):
         m = min(group, r - first)
         starts, row = q_start + 4 * first, table + 4 * first * table_width
         check(_entry("yalis_packed_unpack", "pppiiii" + "pppii" + "iii" + "ppppipp")(
-            *held, positions, starts, row, table_width, m, width, window, skip_single, k_at, v_at, table_at, work.data_ptr(),
-            3 + 4 * items, _address(error_flag), raw), name)
+            *held, positions, starts, row, table_width, m, width, window, skip_single, k_at, v_at, table_at, counters, 3 + 4 * items, flag, raw), name)
         check(_entry("yalis_prefill_attention_tcgen05_unpacked", "plplpp" + "pppiii" + "iiiiii" + "fiiiippppp")(
-            q.data_ptr(), steps[0], out.data_ptr(), steps[1], k_at, v_at, positions, starts, table_at, width, UNPACK_PAGE, m * width, n, m,
-            max_q_len, num_heads, g, dim, scale, window, splits, share, skip_single, _address(lse2), _address(scratch), work.data_ptr(),
-            _address(error_flag), raw), name)
-        if weight_sums is not None:
+            *rows, k_at, v_at, positions, starts, table_at, width, UNPACK_PAGE, m * width, n, m, max_q_len, num_heads, g, dim, scale, window, splits,
+            share, skip_single, _address(lse2), scratch, counters, flag, raw), name)
+        if lse2 is not None:
             check(_entry("yalis_packed_sums_tcgen05", "plpiiiii" + "pppiiiiifii" + "ppiipppp")(
-                q.data_ptr(), steps[0], k_at, width, held[3], held[4], g, dim, positions, starts, row, table_width, m, n, max_kv_len, num_heads, scale,
-                window, skip_single, lse2.data_ptr(), weight_sums.data_ptr(), each, parts, _address(partial), work.data_ptr() + 8, _address(error_flag), raw), name)
+                *rows[:2], k_at, width, held[3], held[4], g, dim, positions, starts, row, table_width, m, n, max_kv_len, num_heads, scale, window,
+                skip_single, lse2.data_ptr(), weight_sums.data_ptr(), each, parts, partial, counters + 8, flag, raw), name)
 
 
 def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tensor, q_start: torch.Tensor, block_table: torch.Tensor,
@@ -256,67 +265,73 @@ def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tenso
     (``out`` may be a column block of a wider matrix); rows that see nothing are zeros, rows of no request stay as they are.
     Scores, weights and sums are float32, and with float32 queries so is every product."""
     name = "packed_attention"
-    _need_here(name, q, pages.k, pages.v, pages.words, positions, q_start, block_table, weight_sums, out, error_flag)
+    device = _need_here(name, q, pages.k, pages.v, pages.words, positions, q_start, block_table, weight_sums, out, error_flag)
     held = _pages_arguments(name, pages)
     page_size, g, dim = held[4:]
-    code, n, r, width = dtype_code(q.dtype), q.shape[0], q_start.shape[0] - 1 if q_start.dim() == 1 else -1, num_heads * dim
+    dtype, width = q.dtype, num_heads * dim
+    code = dtype_code(dtype)
     if num_heads < 1 or num_heads % g:
         raise KernelError(f"{name}: heads must be a multiple of kv_heads")
-    if q.dim() != 2 or q.stride(1) != 1 or q.shape[1] < width:
+    if q.dim() != 2 or q.shape[1] < width:
         raise KernelError(f"{name}: q must be [N, >= heads*head_dim] with unit inner stride")
-    _check_index(name, n, block_table, positions)
-    if q_start.dtype is not torch.int32 or r < 0 or not q_start.is_contiguous():
-        raise KernelError(f"{name}: q_start must be int32 [R+1]")
-    need(block_table.shape[0] >= r, name, "block_table has fewer rows than requests")
-    need(max_q_len >= 0 and (window is None or window > 0), name, "max_q_len and the window must be positive")
+    n, (step, unit) = q.shape[0], q.stride()
+    if unit != 1:
+        raise KernelError(f"{name}: q must be [N, >= heads*head_dim] with unit inner stride")
+    rows, columns = _check_index(name, n, block_table, positions)
+    if q_start.dtype is not torch.int32 or q_start.dim() != 1 or not q_start.is_contiguous() or not 1 <= q_start.shape[0] <= rows + 1:
+        raise KernelError(f"{name}: q_start must be int32 [R+1], and block_table have a row for every request")
+    if max_q_len < 0 or (window is not None and window <= 0):
+        raise KernelError(f"{name}: max_q_len and the window must be positive")
     if scale is None:
-        scale = 1.0 / math.sqrt(dim)
-    need(math.isfinite(scale), name, "the scale must be finite")
-    reach = block_table.shape[1] * page_size
-    max_kv_len = reach if max_kv_len is None else min(int(max_kv_len), reach)
+        scale = dim ** -0.5
+    elif not math.isfinite(scale):
+        raise KernelError(f"{name}: the scale must be finite")
+    r, reach, window, flag = q_start.shape[0] - 1, columns * page_size, window or 0, _flag_address(name, error_flag)
+    max_kv_len = reach if max_kv_len is None or max_kv_len > reach else int(max_kv_len)
+    lse2 = scores = None
     if weight_sums is not None:
         need(weight_sums.dtype == torch.float32 and weight_sums.shape == pages.k.shape[:3] and weight_sums.is_contiguous(), name,
              "weight_sums must be contiguous float32 [pages, kv_heads, page_size]")
-    _check_flag(name, error_flag)
+        lse2 = torch.empty((n, num_heads), dtype=torch.float32, device=device)
     if out is None:
-        out = torch.empty((n, width), dtype=q.dtype, device=q.device)
-    need(out.shape == (n, width) and out.dtype is q.dtype and out.stride(1) == 1, name, "bad out tensor")
-    lse2 = torch.empty((n, num_heads), dtype=torch.float32, device=q.device) if weight_sums is not None else None
-    at, steps, raw = (positions.data_ptr(), q_start.data_ptr(), block_table.data_ptr(), block_table.shape[1], r), (q.stride(0), out.stride(0)), stream()
-    per, aligned = num_heads // g, (q.data_ptr() | steps[0] * q.element_size()) % 16 == 0
-    unpack = (code == BF16 and dim in (64, 128) and max_q_len * per > UNPACK_ROWS and per <= 128 and scale > 0 and aligned
-              and (out.data_ptr() | steps[1] * 2) % 16 == 0)
-    mma, scores = dim in (64, 128) and r <= 4096, None
+        out = torch.empty_like(q) if step == width else torch.empty((n, width), dtype=dtype, device=device)
+    elif out.shape != (n, width) or out.dtype is not dtype or out.stride(1) != 1:
+        raise KernelError(f"{name}: bad out tensor")
+    per, q_at, out_at, out_step, raw = num_heads // g, q.data_ptr(), out.data_ptr(), out.stride(0), _raw_stream(device)
+    at = (positions.data_ptr(), q_start.data_ptr(), block_table.data_ptr(), columns, r)
+    aligned = (q_at | step * (4 if code == F32 else 2)) % 16 == 0
+    mma = (dim == 64 or dim == 128) and r <= 4096
+    unpack = (max_q_len * per > UNPACK_ROWS and code == BF16 and (dim == 64 or dim == 128) and per <= 128 and scale > 0 and aligned
+              and (out_at | out_step * 2) % 16 == 0)
     single = unpack and mma and n > max_q_len          # single tokens may stand beside the portions: a kernel of their own
     if unpack:
-        _attend_unpacked(name, q, out, held, at, steps, n, max_q_len, max_kv_len, num_heads, scale, window or 0, single, lse2, weight_sums,
-                         error_flag, raw)
+        _attend_unpacked(name, device, (q_at, step, out_at, out_step), held, at, n, max_q_len, max_kv_len, num_heads, scale, window, single, lse2,
+                         weight_sums, flag, raw)
     if mma and (single or not unpack):
-        rows = (1 if single else max_q_len) * per
-        columns = 8 if code == F32 or rows <= 8 else 16
-        if weight_sums is not None and rows <= 16 and 4 * n * num_heads * max_kv_len <= SCORE_BYTES:
-            scores = torch.empty(n * num_heads * max_kv_len, dtype=torch.float32, device=q.device)
-        blocks, floats = _mma_launch(q.device, code, dim, columns)
-        scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
+        q_rows = per if single else max_q_len * per
+        tile = 8 if code == F32 or q_rows <= 8 else 16
+        if lse2 is not None and q_rows <= 16 and 4 * n * num_heads * max_kv_len <= SCORE_BYTES:
+            scores = torch.empty(n * num_heads * max_kv_len, dtype=torch.float32, device=device)
+        blocks, floats = _mma_launch(device, code, dim, tile)
+        counters, scratch = _workspace(device, raw, blocks, floats)
         check(_entry("yalis_packed_attention_mma", "plipl" + "pppiiii" + "pppii" + "iiiifipplipppp")(
-            q.data_ptr(), steps[0], code, out.data_ptr(), steps[1], *held, *at, num_heads, columns, aligned, single, scale, window or 0,
-            _address(lse2), _address(scores), max_kv_len, blocks, scratch.data_ptr(), _counters(blocks, q.device).data_ptr(), _address(error_flag), raw), name)
-    if not mma and not unpack:
+            q_at, step, code, out_at, out_step, *held, *at, num_heads, tile, aligned, single, scale, window, _address(lse2), _address(scores),
+            max_kv_len, blocks, scratch.data_ptr(), counters.data_ptr(), flag, raw), name)
+    elif not unpack:
         check(_entry("yalis_packed_attention_general", "plipl" + "pppiiii" + "pppii" + "iifippp")(
-            q.data_ptr(), steps[0], code, out.data_ptr(), steps[1], *held, *at, n, num_heads, scale, window or 0, _address(lse2),
-            _address(error_flag), raw), name)
-    if weight_sums is None or (unpack and not single):
+            q_at, step, code, out_at, out_step, *held, *at, n, num_heads, scale, window, _address(lse2), flag, raw), name)
+    if lse2 is None or (unpack and not single):
         return out
+    to = (lse2.data_ptr(), weight_sums.data_ptr(), raw)
     if scores is not None:
         check(_entry("yalis_packed_sums_of_scores", "pliiii" + "pppii" + "iiiippp")(
-            scores.data_ptr(), max_kv_len, *held[3:], *at, max_kv_len, num_heads, window or 0, single, lse2.data_ptr(), weight_sums.data_ptr(), raw), name)
+            scores.data_ptr(), max_kv_len, *held[3:], *at, max_kv_len, num_heads, window, single, *to), name)
     elif mma:
         check(_entry("yalis_packed_weight_sums", "pli" + "pppiiii" + "pppii" + "iifiiippp")(
-            q.data_ptr(), steps[0], code, *held, *at, max_kv_len, num_heads, scale, window or 0, aligned, single, lse2.data_ptr(),
-            weight_sums.data_ptr(), raw), name)
+            q_at, step, code, *held, *at, max_kv_len, num_heads, scale, window, aligned, single, *to), name)
     else:
         check(_entry("yalis_packed_weight_sums_general", "pli" + "pppiiii" + "pppii" + "iifippp")(
-            q.data_ptr(), steps[0], code, *held, *at, max_kv_len, num_heads, scale, window or 0, lse2.data_ptr(), weight_sums.data_ptr(), raw), name)
+            q_at, step, code, *held, *at, max_kv_len, num_heads, scale, window, *to), name)
     return out
 
 
@@ -334,24 +349,33 @@ def evict_tokens(pools: Sequence[torch.Tensor], weight_sums: torch.Tensor, lengt
     token had, ascending, -1 where there is none."""
     name = "evict_tokens"
     pools = tuple(pools)
-    _need_here(name, *pools, weight_sums, lengths, block_table, error_flag)
-    need(len(pools) <= 4, name, "at most four pools")
-    need(weight_sums.dtype == torch.float32 and weight_sums.dim() == 3 and weight_sums.is_contiguous(), name,
-         "weight_sums must be contiguous float32 [pages, kv_heads, page_size]")
-    pages, g, page_size = shape = weight_sums.shape
-    addresses, row_bytes = (ctypes.c_void_p * 4)(), (ctypes.c_int * 4)()
+    device = _need_here(name, *pools, weight_sums, lengths, block_table, error_flag)
+    if len(pools) > 4:
+        raise KernelError(f"{name}: at most four pools")
+    if not (weight_sums.dtype is torch.float32 and weight_sums.dim() == 3 and weight_sums.is_contiguous()):
+        raise KernelError(f"{name}: weight_sums must be contiguous float32 [pages, kv_heads, page_size]")
+    shape, rows = weight_sums.shape, max(1, weight_sums.numel())
+    pages, g, page_size = shape
+    addresses, row_bytes = _Addresses(), _Sizes()
     for i, p in enumerate(pools):
-        need(p.dim() >= 3 and p.shape[:3] == shape and p.is_contiguous(), name, "pools must be contiguous [pages, kv_heads, page_size, ...]")
-        addresses[i], row_bytes[i] = p.data_ptr(), p.numel() // max(1, pages * g * page_size) * p.element_size()
-        need(row_bytes[i] % 2 == 0 and p.data_ptr() % 2 == 0, name, "rows of a pool must be whole pairs of bytes")
-    need(lengths.dtype == torch.int32 and lengths.dim() == 1 and lengths.is_contiguous(), name, "lengths must be int32 [R]")
-    r = lengths.shape[0]
-    _check_index(name, 0, block_table)
-    _check_flag(name, error_flag)
-    need(block_table.shape[0] >= r, name, "block_table has fewer rows than requests")
-    need(keep >= 1 and 0 <= recent <= keep, name, "keep must be at least 1 and recent between 0 and keep")
-    kept = torch.empty((r, g, keep), dtype=torch.int32, device=lengths.device)
+        if p.dim() < 3 or p.shape[:3] != shape or not p.is_contiguous():
+            raise KernelError(f"{name}: pools must be contiguous [pages, kv_heads, page_size, ...]")
+        addresses[i], row_bytes[i] = at, size = p.data_ptr(), p.numel() // rows * p.element_size()
+        if (at | size) % 2:
+            raise KernelError(f"{name}: rows of a pool must be whole pairs of bytes")
+    if not (lengths.dtype is torch.int32 and lengths.dim() == 1 and lengths.is_contiguous()):
+        raise KernelError(f"{name}: lengths must be int32 [R]")
+    r, flag = lengths.shape[0], _flag_address(name, error_flag)
+    table_rows, columns = _check_index(name, 0, block_table)
+    if table_rows < r:
+        raise KernelError(f"{name}: block_table has fewer rows than requests")
+    if keep < 1 or not 0 <= recent <= keep:
+        raise KernelError(f"{name}: keep must be at least 1 and recent between 0 and keep")
+    kept = torch.empty((r, g, keep), dtype=torch.int32, device=device)
     check(_entry("yalis_evict_tokens", "ppippp" + "iiiiiii" + "ppp")(
-        ctypes.addressof(addresses), ctypes.addressof(row_bytes), len(pools), weight_sums.data_ptr(), lengths.data_ptr(), block_table.data_ptr(),
-        block_table.shape[1], page_size, pages, g, r, keep, recent, kept.data_ptr(), _address(error_flag), stream()), name)
+        addresses, row_bytes, len(pools), weight_sums.data_ptr(), lengths.data_ptr(), block_table.data_ptr(), columns, page_size, pages, g, r, keep,
+        recent, kept.data_ptr(), flag, _raw_stream(device)), name)
     return kept
+
+
+_Addresses, _Sizes = ctypes.c_void_p * 4, ctypes.c_int * 4

@@ -23,14 +23,22 @@ struct PackedPages {
   uint32_t* v;
   uint32_t* words;             // [pages, g, page_size]: the key's word low, the value's high
   int num_pages, page_size, g, dim;
+  int shift;                   // page_size is 2^shift, or -1
 };
+
+inline PackedPages packed_pages(void* k, void* v, void* words, int num_pages, int page_size, int g, int dim) {
+  int shift = 0;
+  while (1 << shift < page_size) ++shift;
+  return {static_cast<uint32_t*>(k), static_cast<uint32_t*>(v), static_cast<uint32_t*>(words), num_pages, page_size, g, dim,
+          1 << shift == page_size ? shift : -1};
+}
 
 __device__ __forceinline__ float step_of(uint32_t word16) { return __uint_as_float((word16 & 0xFFF0u) << 16); }
 __device__ __forceinline__ float zero_of(uint32_t word16) { return (float)(word16 & 15u); }
 
 // The page and row of cached token `at` of a request; page -1 where the table has none.
 __device__ __forceinline__ int page_of(const PackedPages& c, const int32_t* table_row, int table_width, int at, int& row) {
-  const int index = at / c.page_size;
+  const int index = c.shift >= 0 ? at >> c.shift : at / c.page_size;
   row = at - index * c.page_size;
   const int page = index < table_width ? table_row[index] : -1;
   return page >= 0 && page < c.num_pages ? page : -1;
@@ -39,20 +47,21 @@ __device__ __forceinline__ size_t row_index(const PackedPages& c, int page, int 
   return ((size_t)page * c.g + kvh) * c.page_size + row;
 }
 
-// The step of a row with the given extremes (lo <= 0 <= hi, finite, at most 2^120 in magnitude).  Bits are rounded up to four
-// significant ones; hi - lo and its fifteenth part were rounded before, which can only lose what stands above a number of four
-// bits by less than a rounding: the exact difference (rounded + lost) is compared with 15 step, which is exact.
-__device__ __forceinline__ float step_for(float lo, float hi) {
-  const float range = hi - lo;
-  const float lost = (hi - (range + lo)) + (-lo - (range - (range + lo)));     // range + lost = hi - lo without rounding
+// The step of a row with the extremes -below <= 0 <= above, finite, at most 2^120.  A product with a little less than 1 / 15 is rounded
+// up to four significant bits, and goes one further where 15 steps are still too few.  above + below was rounded before, which can
+// only lose what stands above a number of four bits by less than a rounding: rounded + lost, the exact sum, is compared with 15 step,
+// which is exact.
+__device__ __forceinline__ float step_for(float below, float above) {
+  const float range = above + below;
+  const float a = range - below, lost = (above - a) + (below - (range - a));
   const uint32_t up = 0x000FFFFFu;
-  float step = __uint_as_float((__float_as_uint(__fdiv_rn(range, 15.f)) + up) & ~up);
+  float step = __uint_as_float((__float_as_uint(range * __uint_as_float(0x3D888888u)) + up) & ~up);
   const float most = 15.f * step;
   if (range > most || (range == most && lost > 0.f)) step = __uint_as_float(__float_as_uint(step) + up + 1u);
   return fmaxf(step, kPackedLeast);
 }
 
-// 2^22 + n + 2^23 for n = rint(x / step), the whole number in its lowest bits; `inverse` is 1 / step, rounded.  One step of
+// 2^22 + n + 2^23 for n = rint(x / step), the whole number in its lowest bits; `inverse` is 1 / step, nearly.  One step of
 // refinement makes the product the rounded quotient (what it leaves is exact), so that ties are ties.  For bfloat16 values that is
 // all: their quotients by four bits are ties or stand well apart from them.  A float32 quotient may round to a tie that the exact one
 // misses by less; what is left over after the multiple is exact and says so.

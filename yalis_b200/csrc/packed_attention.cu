@@ -166,7 +166,7 @@ bool params_of(AttentionParams& p, const void* q, long long q_stride, void* k_co
   p.q = q; p.q_stride = q_stride;
   p.positions = positions; p.q_start = q_start; p.block_table = block_table; p.table_width = table_width;
   p.n_requests = n_requests; p.nh = nh; p.per = nh / g; p.window = window; p.scale = scale;
-  p.pages = {static_cast<uint32_t*>(k_codes), static_cast<uint32_t*>(v_codes), static_cast<uint32_t*>(words), num_pages, page_size, g, dim};
+  p.pages = packed_pages(k_codes, v_codes, words, num_pages, page_size, g, dim);
   return true;
 }
 

@@ -39,7 +39,7 @@ struct MmaParams {
   const int32_t* positions;    // [N]
   const int32_t* q_start;      // [R + 1]
   const int32_t* block_table;  // [R, table_width]
-  int table_width, n_requests, nh, per, window, page_shift;
+  int table_width, n_requests, nh, per, window;
   int together;                // 2: a chunk never lies in two pages; 1: the rows that one copy instruction of a warp covers do not
   int q_vector;                // 1: rows of q start on 16-byte boundaries
   int only_single;             // 1: requests that bring more than one token are left to another kernel
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
     auto lookup = [&](int chunk) {               // the pool's row of the lane's key, -1 without a page
       const int key = first_key + chunk * kChunk + lane;
       if (key > any_hi) return -2;               // nobody's
-      const int index = p.page_shift >= 0 ? key >> p.page_shift : key / p.pages.page_size;
+      const int index = p.pages.shift >= 0 ? key >> p.pages.shift : key / p.pages.page_size;
       const int page = index < p.table_width ? table_row[index] : -1;
       if (page < 0 || page >= p.pages.num_pages) {
         if (key >= any_lo && p.error) atomicOr(p.error, YALIS_FLAG_BAD_PAGE);
@@ -788,11 +788,9 @@ YALIS_API int yalis_packed_attention_mma(const void* q, long long q_stride, int 
   p.q = q; p.q_stride = q_stride; p.out = out; p.out_stride = out_stride;
   p.positions = positions; p.q_start = q_start; p.block_table = block_table; p.table_width = table_width;
   p.n_requests = n_requests; p.nh = nh; p.per = nh / g; p.window = window; p.q_vector = q_vector; p.only_single = only_single;
-  p.page_shift = -1; p.together = page_size % kChunk == 0 ? 2 : page_size % (1024 / dim) == 0 ? 1 : 0;
-  if ((page_size & (page_size - 1)) == 0)
-    for (p.page_shift = 0; 1 << p.page_shift < page_size;) ++p.page_shift;
+  p.together = page_size % kChunk == 0 ? 2 : page_size % (1024 / dim) == 0 ? 1 : 0;
   p.scale_log2 = scale * 1.4426950408889634f; p.lse2 = lse2; p.scores = scores; p.score_stride = score_stride; p.part = scratch; p.tickets = tickets; p.error = error;
-  p.pages = {static_cast<uint32_t*>(k_codes), static_cast<uint32_t*>(v_codes), static_cast<uint32_t*>(words), num_pages, page_size, g, dim};
+  p.pages = packed_pages(k_codes, v_codes, words, num_pages, page_size, g, dim);
   if (dtype == YALIS_BF16) {
     if (columns == 8) return dim == 64 ? launch_mma<__nv_bfloat16, 64, 1, 1>(p, blocks, stream) : launch_mma<__nv_bfloat16, 128, 1, 1>(p, blocks, stream);
     if (columns == 16) return dim == 64 ? launch_mma<__nv_bfloat16, 64, 2, 1>(p, blocks, stream) : launch_mma<__nv_bfloat16, 128, 2, 1>(p, blocks, stream);

@@ -395,7 +395,7 @@ YALIS_API int yalis_packed_sums_tcgen05(const void* q, long long q_stride, const
   if (parts < 1 || each < 1 || items * parts > 0x7fffffffll || rows + (long long)g * 64 > 0x7fffffffll) return YALIS_ERR_SHAPE;
   p.n_items = (int)items; p.parts = parts; p.each = each; p.partial = partial; p.counters = counters;
   p.scale_log2 = scale * 1.4426950408889634f; p.lse2 = lse2; p.sums = sums; p.error = error;
-  p.pages = {nullptr, nullptr, nullptr, num_pages, page_size, g, dim};
+  p.pages = packed_pages(nullptr, nullptr, nullptr, num_pages, page_size, g, dim);
   CUtensorMap mq, mk;
   const cuuint64_t q_sizes[3] = {(cuuint64_t)dim, (cuuint64_t)nh, (cuuint64_t)n_tokens}, q_strides[2] = {(cuuint64_t)dim * 2, (cuuint64_t)q_stride * 2};
   const cuuint32_t q_box[3] = {64u, (cuuint32_t)per, (cuuint32_t)p.tokens_per_tile};

@@ -25,26 +25,82 @@ struct RowParams {
   PackedPages pages;
 };
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vector, float (&x)[8]) {
+// Eight values of a row as they lie in memory: bfloat16 in pairs, or float32.
+struct Pairs { uint32_t w[4]; };
+struct Singles { float v[8]; };
+template <typename T> struct Held;
+template <> struct Held<__nv_bfloat16> { using type = Pairs; };
+template <> struct Held<float> { using type = Singles; };
+
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, bool vector, Pairs& x) {
   if (vector) {
-    if constexpr (sizeof(T) == 2) {
-      const uint4 u = *reinterpret_cast<const uint4*>(p);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    *reinterpret_cast<uint4*>(x.w) = *reinterpret_cast<const uint4*>(p);
+  } else {
+    const uint16_t* at = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-      }
-    } else {
-      const float4 a = load4_f32(p), b = load4_f32(p + 4);
-      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-      x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    }
+    for (int i = 0; i < 4; ++i) x.w[i] = at[2 * i] | (uint32_t)at[2 * i + 1] << 16;
+  }
+}
+__device__ __forceinline__ void load8(const float* p, bool vector, Singles& x) {
+  if (vector) {
+    *reinterpret_cast<float4*>(x.v) = load4_f32(p);
+    *reinterpret_cast<float4*>(x.v + 4) = load4_f32(p + 4);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(p[i]);
+    for (int i = 0; i < 8; ++i) x.v[i] = p[i];
   }
+}
+__device__ __forceinline__ void zero8(Pairs& x) { x.w[0] = x.w[1] = x.w[2] = x.w[3] = 0u; }
+__device__ __forceinline__ void zero8(Singles& x) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x.v[i] = 0.f;
+}
+__device__ __forceinline__ void values8(const Pairs& x, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(x.w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(x.w[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void values8(const Singles& x, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = x.v[i];
+}
+
+// The largest of the row's values and 0, and minus the least of them and 0, over LANES neighbouring lanes.
+__device__ __forceinline__ uint32_t most2(uint32_t a, uint32_t b) {           // of each half; not a number if one is none
+  const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+template <int LANES>
+__device__ __forceinline__ void extremes(const Pairs& x, float& above, float& below) {
+  // both extremes as one pair: the values' largest beside the largest of the values with their signs turned
+  const uint32_t sign = 0x80008000u;
+  const uint32_t up = most2(most2(x.w[0], x.w[1]), most2(x.w[2], x.w[3]));
+  const uint32_t down = most2(most2(x.w[0] ^ sign, x.w[1] ^ sign), most2(x.w[2] ^ sign, x.w[3] ^ sign));
+  uint32_t both = most2(most2(__byte_perm(up, down, 0x5410), __byte_perm(up, down, 0x7632)), 0u);
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) both = most2(both, __shfl_xor_sync(0xffffffffu, both, o));
+  above = __uint_as_float(both << 16);
+  below = __uint_as_float(both & 0xFFFF0000u);
+}
+template <int LANES>
+__device__ __forceinline__ void extremes(const Singles& x, float& above, float& below) {
+  float odd = 0.f;
+  above = below = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    above = fmaxf(above, x.v[i]);
+    below = fmaxf(below, -x.v[i]);
+    odd = fmaf(x.v[i], 0.f, odd);                             // not a number where a value is none, or infinite
+  }
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    above = fmaxf(above, __shfl_xor_sync(0xffffffffu, above, o));
+    below = fmaxf(below, __shfl_xor_sync(0xffffffffu, below, o));
+    odd += __shfl_xor_sync(0xffffffffu, odd, o);
+  }
+  above += odd;
 }
 
 // The pool's row of a KV head of a token, -1 where the token is none or has no page.
@@ -65,43 +121,35 @@ __global__ void packed_rows_write_kernel(const RowParams<T> p) {
   pdl_wait();
   const int lane = threadIdx.x & (LANES - 1), group = (blockIdx.y * blockDim.x + threadIdx.x) / LANES, is_v = group & 1, kvh = group >> 1;
   const bool listed = kvh < p.pages.g && lane * 8 < p.pages.dim;
-  float x[TOKENS][8];
+  typename Held<T>::type x[TOKENS];
   long long row[TOKENS];
 #pragma unroll
   for (int i = 0; i < TOKENS; ++i) {
     const int token = blockIdx.x * TOKENS + i;
     row[i] = -1;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[i][j] = 0.f;
+    zero8(x[i]);
     if (listed && token < p.n_tokens) {
       const T* src = is_v ? p.v + (long long)token * p.v_stride : p.k + (long long)token * p.k_stride;
-      load8<T>(src + (size_t)kvh * p.pages.dim + lane * 8, p.vector, x[i]);
+      load8(src + (size_t)kvh * p.pages.dim + lane * 8, p.vector, x[i]);
       row[i] = place_of(p, token, kvh, group == 0 && lane == 0);
     }
   }
 #pragma unroll
   for (int i = 0; i < TOKENS; ++i) {
-    float lo = 0.f, hi = 0.f, odd = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      lo = fminf(lo, x[i][j]);
-      hi = fmaxf(hi, x[i][j]);
-      odd = fmaf(x[i][j], 0.f, odd);                          // not a number where x is none, or infinite
-    }
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      odd += __shfl_xor_sync(0xffffffffu, odd, o);
-    }
+    float above, below;                                       // the row's extremes, not numbers where it holds one that is none
+    extremes<LANES>(x[i], above, below);
     if (row[i] < 0) continue;
     uint32_t codes = 0, word = 0x7FC0u;                       // not a number: all codes 0
-    if (odd == 0.f && fmaxf(hi, -lo) <= kPackedLargest) {
-      const float step = step_for(lo, hi), inverse = __frcp_rn(step);
-      const float first = multiple_of<sizeof(T) == 4>(lo, step, inverse);
+    if (above <= kPackedLargest && below <= kPackedLargest) {
+      const float step = step_for(below, above);
+      float inverse;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(step));
+      const float first = multiple_of<sizeof(T) == 4>(-below, step, inverse);
+      float v[8];
+      values8(x[i], v);
 #pragma unroll
       for (int j = 7; j >= 0; --j) {                          // (no value lies below the row's least)
-        const int c = __float_as_int(multiple_of<sizeof(T) == 4>(x[i][j], step, inverse)) - __float_as_int(first);
+        const int c = __float_as_int(multiple_of<sizeof(T) == 4>(v[j], step, inverse)) - __float_as_int(first);
         codes = codes << 4 | (uint32_t)min(c, 15);
       }
       word = (__float_as_uint(step) >> 16) | (uint32_t)(__float_as_int(12582912.f) - __float_as_int(first));
@@ -257,7 +305,7 @@ YALIS_API int yalis_packed_rows(int write, void* k, void* v, long long k_stride,
     p.k_stride = k_stride; p.v_stride = v_stride;
     p.positions = positions; p.req_of_token = req_of_token; p.block_table = block_table;
     p.table_width = table_width; p.n_tokens = n_tokens; p.vector = vector; p.error = error;
-    p.pages = {static_cast<uint32_t*>(k_codes), static_cast<uint32_t*>(v_codes), static_cast<uint32_t*>(words), num_pages, page_size, g, dim};
+    p.pages = packed_pages(k_codes, v_codes, words, num_pages, page_size, g, dim);
     return write ? launch_rows<T, true>(p, n_tokens, stream) : launch_rows<T, false>(p, n_tokens, stream);
   });
 }
@@ -274,6 +322,6 @@ YALIS_API int yalis_packed_unpack(void* k_codes, void* v_codes, void* words, int
   p.k_out = static_cast<__nv_bfloat16*>(k_out); p.v_out = static_cast<__nv_bfloat16*>(v_out); p.table_out = table_out; p.zeroed = zeroed;
   p.positions = positions; p.q_start = q_start; p.block_table = block_table; p.table_width = table_width; p.width = width;
   p.window = window; p.skip_single = skip_single; p.error = error;
-  p.pages = {static_cast<uint32_t*>(k_codes), static_cast<uint32_t*>(v_codes), static_cast<uint32_t*>(words), num_pages, page_size, g, dim};
+  p.pages = packed_pages(k_codes, v_codes, words, num_pages, page_size, g, dim);
   return yalis_launch(packed_unpack_kernel, dim3(width, g, n_requests), dim3(256), 0, stream, p);
 }

@@ -288,7 +288,7 @@ SumsParams params_of(const void* q, long long q_stride, int num_pages, int page_
   p.q = q; p.q_stride = q_stride; p.positions = positions; p.q_start = q_start; p.block_table = block_table; p.table_width = table_width;
   p.nh = nh; p.per = nh / g; p.window = window; p.only_single = only_single; p.scale_log2 = scale * 1.4426950408889634f;
   p.lse2 = lse2; p.sums = sums;
-  p.pages = {nullptr, nullptr, nullptr, num_pages, page_size, g, dim};
+  p.pages = packed_pages(nullptr, nullptr, nullptr, num_pages, page_size, g, dim);
   return p;
 }
 

@@ -10,15 +10,19 @@
 // The order of a product's inner index is free as long as both operands agree, so a lane takes neighbouring codes: with a word of
 // eight codes, (w >> s) & 0x00780078 | 0x41804180 is the pair 16 + c_i, 16 + c_(i + 4) in bfloat16.  For values 16 + zero is taken
 // away from the pairs (exact); for keys (16 + zero) sum(q) is taken away from the product, which is two instructions a score in
-// place of 64 a chunk (with float32 queries the pairs lose it too: the difference of two large sums would show).  Elements of a V row pair up by key instead: the 16-bit halves of two keys' words are put side by side first.  The
-// scores' accumulators, times step, are the softmax's scores; the weights times the values' steps are rounded to bfloat16
-// (float32: in three parts) and turned from accumulator layout to operand layout by movmatrix.
+// place of 64 a chunk (with float32 queries the pairs lose it too: the difference of two large sums would show).  With bfloat16 queries
+// values and weights meet in float16: two of a half word's codes then need no shift, and a weight keeps eleven bits; the values' steps
+// go in relative to the largest so far.  Elements of a V row pair up by key instead: the 16-bit halves of two keys' words are put side by side first.  The
+// scores' accumulators, times step, are the softmax's scores; the weights times the values' steps are rounded to float16
+// (float32: to three bfloat16 parts) and turned from accumulator layout to operand layout by movmatrix.
 //
 // A warp takes 32 keys at a time (a chunk) through a ring of its own in shared memory, filled by 16-byte asynchronous copies, and
 // keeps a softmax and an output of its own; the four warps of a block come together at the end of a pair.  Chunks are
 // dealt to a fixed grid by the step's lengths (choose_deal), so that a recorded launch serves other lengths too; a pair cut between
 // blocks is added up, in the blocks' order, by whichever of them comes last (a counter per pair, left at zero).  Nothing waits for
 // another block.
+#include <cuda_fp16.h>
+
 #include <type_traits>
 
 #include "packed.cuh"
@@ -43,6 +47,7 @@ struct MmaParams {
   int together;                // 2: a chunk never lies in two pages; 1: the rows that one copy instruction of a warp covers do not
   int q_vector;                // 1: rows of q start on 16-byte boundaries
   int only_single;             // 1: requests that bring more than one token are left to another kernel
+  int slots;                   // blocks resident at once; the launch has as many, or one for every pair
   float scale_log2;
   float* lse2;                 // [N, nh] the logarithm to base two of a row's sum of exponentials, or null
   float* scores;               // [N, nh, score_stride] every score in powers of two, by place (those that some row of the pair sees), or null
@@ -64,6 +69,27 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pair_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t minus_f16(uint32_t a, uint32_t b) {
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Codes of a pair in float16, where two of a 16-bit half's four need no shift: 16 + c / 64 from the lowest bits, 16 + c / 4 from the next.
+template <int SHIFT>
+__device__ __forceinline__ uint32_t code_pair_f16(uint32_t w, uint32_t sixteens) {
+  uint32_t r;
+  if constexpr (SHIFT == 0) asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(r) : "r"(w), "r"(sixteens));
+  else asm("lop3.b32 %0, %1, 0x00F000F0, %2, 0xEA;" : "=r"(r) : "r"(w), "r"(sixteens));
+  return r;
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
   uint32_t r;
@@ -134,22 +160,26 @@ __device__ __forceinline__ float4 terms_of(uint32_t word, float scale_log2) {
 }
 
 // How a step's chunks are dealt out, by what the slowest block then has to do, counted in chunks:
-//   pieces k > 0: every pair to k blocks in equal pieces, one piece a block;
+//   pieces k > 0: every pair to k blocks in equal pieces, one piece a block (one, where there are more pairs than blocks resident at
+//   once: the rest follow as blocks end);
 //   0: all chunks of all pairs, laid end to end, in equal shares; a block's share begins and ends inside pairs that others share.
-// A piece is at least kLeast chunks; to come together with other blocks takes about kJoin chunks' time.
+// A piece is at least kLeast chunks; to come together with other blocks takes about kJoin chunks' time (64 requests of 520 to 1,040
+// tokens, 8 KV heads of 128: 25 us whole, 36 in equal shares; 8 of 16,000 to 32,000: 66 in nine pieces, 69 in equal shares; 96 of 450
+// to 900, 16 heads over 8: 41 in equal shares).
 struct Deal {
   int pieces, blocks;
 };
-constexpr int kLeast = 2 * kWarps, kJoin = 4;
+constexpr int kLeast = 2 * kWarps, kJoin = 32;
 
-__device__ __forceinline__ Deal choose_deal(int grid, int pairs, int most, long long total) {
-  const int even_blocks = (int)min((long long)grid, (total + kLeast - 1) / kLeast);
-  if (pairs > grid) return {0, even_blocks};
-  const int k = max(1, min(grid / pairs, (most + kLeast - 1) / kLeast));
+__device__ __forceinline__ Deal choose_deal(int slots, int pairs, int most, long long total) {
+  if (pairs > slots) return {1, pairs};
+  const int even_blocks = (int)min((long long)slots, (total + kLeast - 1) / kLeast);
+  const int k = max(1, min(slots / pairs, (most + kLeast - 1) / kLeast));
   const long long even = total / even_blocks + 2 * kJoin;
   if ((most + k - 1) / k + (k > 1 ? kJoin : 0) <= even) return {k, pairs * k};
   return {0, even_blocks};
 }
+
 
 // SCORES: every score is left in memory as well (a branch on the pointer in the one kernel cost 3 % of the steps that want none).
 template <typename T, int DIM, int NT, int PARTS, bool SCORES>
@@ -161,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
   constexpr int PIECES = DIM / 32;             // 16-byte pieces of a row
   constexpr int COPIES = PIECES;               // of K (and as many of V) that a lane asks for per chunk
   constexpr int PART_FLOATS = NT * MT * 128 + 2 * COLS;
-  constexpr bool SIGNED = PARTS > 1;
+  constexpr bool SIGNED = PARTS > 1, HALF = PARTS == 1;        // HALF: values and weights meet in float16
   extern __shared__ __align__(128) unsigned char smem[];
   Stage<DIM>* ring = reinterpret_cast<Stage<DIM>*>(smem) + (threadIdx.x >> 5) * kStages;
   float4* terms = reinterpret_cast<float4*>(smem + sizeof(Stage<DIM>) * kStages * kWarps) + (threadIdx.x >> 5) * kChunk;
@@ -175,6 +205,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint32_t sixteens;
   asm volatile("mov.b32 %0, 0x41804180;" : "=r"(sixteens));
+  uint32_t sixteens_f16;
+  asm volatile("mov.b32 %0, 0x4C004C00;" : "=r"(sixteens_f16));
   pdl_wait();
 
   // ---- the chunks of every request (KV heads, blocks of columns and chunks of 32 keys), their running sum, this block's share ----
@@ -216,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
     }
     most = __reduce_max_sync(0xffffffffu, most);
     if (lane == 0) {
-      const Deal deal = carry > 0 ? choose_deal(gridDim.x, carry_pairs, most, carry) : Deal{0, 0};
+      const Deal deal = carry > 0 ? choose_deal(p.slots, carry_pairs, most, carry) : Deal{0, 0};
       s_deal[0] = deal.pieces;
       s_deal[1] = deal.blocks;
     }
@@ -268,43 +300,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       n_blocks = holder(first + chunks - 1) - first_block + 1;
     }
 
-    // ---- columns: queries in registers as the products' right operand, the keys that each sees ----
+    // ---- columns: the keys that each sees ----
     const int tok0 = p.q_start[req];
     const int32_t* table_row = p.block_table + (size_t)req * p.table_width;
-    uint32_t qf[NT][2 * W][2][PARTS];
-    float q_sum[NT][2];                          // sum(q) of the columns 2t, 2t + 1
     int see_hi[NT][2], see_lo[NT][2], all_hi = 0x7fffffff, all_lo = 0, any_hi = -1, any_lo = 0x7fffffff;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int row = column0 + nt * 8 + g;
-      const bool real = row < n_rows;
-      const int token = tok0 + (real ? row / p.per : 0), head = kvh * p.per + (real ? row % p.per : 0);
-      const T* src = static_cast<const T*>(p.q) + (long long)token * p.q_stride + (long long)head * DIM + t * (DIM / 4);
-      float own = 0.f;
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        float x[8];
-        if (!real) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = 0.f;
-        } else if (p.q_vector) {
-          const float4 a = load4_f32(src + 8 * w), b = load4_f32(src + 8 * w + 4);
-          x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-          x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(src[8 * w + i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          parts_of<PARTS>(x[i], x[i + 4], qf[nt][2 * w + (i >> 1)][i & 1]);
-          own += x[i] + x[i + 4];
-        }
-      }
-      own += __shfl_xor_sync(0xffffffffu, own, 1);
-      own += __shfl_xor_sync(0xffffffffu, own, 2);             // column g, in its four lanes
-#pragma unroll
-      for (int e = 0; e < 2; ++e) q_sum[nt][e] = __shfl_sync(0xffffffffu, own, (2 * t + e) * 4);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int column = column0 + nt * 8 + 2 * t + e;
@@ -329,6 +330,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
     }
 
     float m[NT][2], l[NT][2], acc[NT][MT][4];
+    uint32_t v_top = 0u;                         // HALF: no step up to this needs another scale
+    float v_scale = 1.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m[nt][0] = m[nt][1] = kNone;
@@ -345,16 +348,16 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       const int skip = (any_lo - first_key) / kChunk;
       while (c < skip) c += kWarps;
     }
-    auto lookup = [&](int chunk) {               // the pool's row of the lane's key, -1 without a page
-      const int key = first_key + chunk * kChunk + lane;
-      if (key > any_hi) return -2;               // nobody's
-      const int index = p.pages.shift >= 0 ? key >> p.pages.shift : key / p.pages.page_size;
+    auto lookup = [&](int chunk) {               // the pool's row of the lane's key; -1 without a page, -2 for nobody's key
+      const int key0 = first_key + chunk * kChunk, key = key0 + lane, from = p.together == 2 ? key0 : key;
+      if (p.together != 2 && key > any_hi) return -2;
+      const int index = p.pages.shift >= 0 ? from >> p.pages.shift : from / p.pages.page_size;
       const int page = index < p.table_width ? table_row[index] : -1;
-      if (page < 0 || page >= p.pages.num_pages) {
-        if (key >= any_lo && p.error) atomicOr(p.error, YALIS_FLAG_BAD_PAGE);
+      if ((unsigned)page >= (unsigned)p.pages.num_pages) {
+        if (min(key0 + kChunk - 1, any_hi) >= any_lo && (p.together == 2 || key >= any_lo) && p.error) atomicOr(p.error, YALIS_FLAG_BAD_PAGE);
         return -1;
       }
-      return (page * p.pages.g + kvh) * p.pages.page_size + (key - index * p.pages.page_size);
+      return key > any_hi ? -2 : (page * p.pages.g + kvh) * p.pages.page_size + (key - index * p.pages.page_size);
     };
     auto ask = [&](int stage, int row) {         // rows that are not there are left as they are: their word says so
       Stage<DIM>& st = ring[stage];
@@ -402,6 +405,43 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
     asm volatile("cp.async.commit_group;" ::: "memory");
     bool missing = __any_sync(0xffffffffu, row < 0);
     row = c + kWarps < c_end ? lookup(c + kWarps) : -2;
+
+    // ---- queries in registers as the products' right operand, while the first copies are under way ----
+    uint32_t qf[NT][2 * W][2][PARTS];
+    float q_sum[NT][2];                          // sum(q) of the columns 2t, 2t + 1
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = column0 + nt * 8 + g;
+      const bool real = row < n_rows;
+      const int token = tok0 + (real ? row / p.per : 0), head = kvh * p.per + (real ? row % p.per : 0);
+      const T* src = static_cast<const T*>(p.q) + (long long)token * p.q_stride + (long long)head * DIM + t * (DIM / 4);
+      float own = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        float x[8];
+        if (!real) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = 0.f;
+        } else if (p.q_vector) {
+          const float4 a = load4_f32(src + 8 * w), b = load4_f32(src + 8 * w + 4);
+          x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+          x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(src[8 * w + i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          parts_of<PARTS>(x[i], x[i + 4], qf[nt][2 * w + (i >> 1)][i & 1]);
+          own += x[i] + x[i + 4];
+        }
+      }
+      own += __shfl_xor_sync(0xffffffffu, own, 1);
+      own += __shfl_xor_sync(0xffffffffu, own, 2);             // column g, in its four lanes
+#pragma unroll
+      for (int e = 0; e < 2; ++e) q_sum[nt][e] = __shfl_sync(0xffffffffu, own, (2 * t + e) * 4);
+    }
+
     for (int stage = 0; c < c_end; c += kWarps, stage ^= 1) {
       const bool missing_next = __any_sync(0xffffffffu, row < 0);
       if (c + kWarps < c_end) ask(stage ^ 1, row);
@@ -411,7 +451,28 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       __syncwarp();
       const Stage<DIM>& st = ring[stage];
       const int key0 = first_key + c * kChunk;
-      terms[lane] = terms_of(st.words[lane], p.scale_log2);
+      float4 own = terms_of(st.words[lane], p.scale_log2);
+      // HALF: the values' steps relative to the largest so far, as 64 to 128, so that weights stay below 2^15 (kLazy) and are whole
+      // to eleven bits down to 2^-14.
+      if constexpr (HALF) {
+        const uint32_t largest = __reduce_max_sync(0xffffffffu, own.z == own.z ? __float_as_uint(own.z) : 0u);
+        if (largest > v_top) {
+          const float fewer = v_scale;
+          v_top = largest | 0x007FFFFFu;
+          v_scale = __uint_as_float(0x82000000u - max(largest & 0x7F800000u, 0x04000000u));       // 2^(6 - e) for a step of 2^e and more
+          const float less = v_scale / fewer;    // (powers of two; nothing to rescale the first time)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) acc[nt][i][j] *= less;
+        }
+        own.z *= v_scale;
+        // 16 + zero / 64 and 16 + zero / 4 in float16
+        own.w = __uint_as_float(0x4C004C00u | (st.words[lane] >> 16 & 15u) * 0x00100001u);
+      }
+      terms[lane] = own;
       __syncwarp();
 
       // ---- products with 32 keys ----
@@ -575,10 +636,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            uint32_t part[PARTS];
-            parts_of<PARTS>(sc[nt][half][2 * e], sc[nt][half][2 * e + 1], part);
+            if constexpr (HALF) {
+              wf[nt][half][e][0] = transposed(pair_f16(sc[nt][half][2 * e], sc[nt][half][2 * e + 1]));
+            } else {
+              uint32_t part[PARTS];
+              parts_of<PARTS>(sc[nt][half][2 * e], sc[nt][half][2 * e + 1], part);
 #pragma unroll
-            for (int i = 0; i < PARTS; ++i) wf[nt][half][e][i] = transposed(part[i]);
+              for (int i = 0; i < PARTS; ++i) wf[nt][half][e][i] = transposed(part[i]);
+            }
           }
       // ---- output ----
 #pragma unroll
@@ -597,22 +662,42 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
             vw[i][0] = *reinterpret_cast<const uint32_t*>(st.v + r * (DIM / 2) + g * 4);
           }
         }
-        const uint32_t z01 = __byte_perm(__float_as_uint(z[0]), __float_as_uint(z[1]), 0x7632);
-        const uint32_t z23 = __byte_perm(__float_as_uint(z[2]), __float_as_uint(z[3]), 0x7632);
+        if constexpr (HALF) {
+          const uint32_t lo01 = __byte_perm(__float_as_uint(z[0]), __float_as_uint(z[1]), 0x5410), hi01 = __byte_perm(__float_as_uint(z[0]), __float_as_uint(z[1]), 0x7632);
+          const uint32_t lo23 = __byte_perm(__float_as_uint(z[2]), __float_as_uint(z[3]), 0x5410), hi23 = __byte_perm(__float_as_uint(z[2]), __float_as_uint(z[3]), 0x7632);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+          for (int u = 0; u < U; ++u) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t a = __byte_perm(vw[0][u], vw[1][u], h ? 0x7632 : 0x5410), b = __byte_perm(vw[2][u], vw[3][u], h ? 0x7632 : 0x5410);
-            const uint32_t f0[4] = {minus(code_pair<0>(a, sixteens), z01), minus(code_pair<1>(a, sixteens), z01), minus(code_pair<0>(b, sixteens), z23), minus(code_pair<1>(b, sixteens), z23)};
-            const uint32_t f1[4] = {minus(code_pair<2>(a, sixteens), z01), minus(code_pair<3>(a, sixteens), z01), minus(code_pair<2>(b, sixteens), z23), minus(code_pair<3>(b, sixteens), z23)};
-            const int tile = 4 * u + 2 * h;
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t a = __byte_perm(vw[0][u], vw[1][u], h ? 0x7632 : 0x5410), b = __byte_perm(vw[2][u], vw[3][u], h ? 0x7632 : 0x5410);
+              const uint32_t a8 = a >> 8, b8 = b >> 8;
+              const uint32_t f0[4] = {minus_f16(code_pair_f16<0>(a, sixteens_f16), lo01), minus_f16(code_pair_f16<4>(a, sixteens_f16), hi01),
+                                      minus_f16(code_pair_f16<0>(b, sixteens_f16), lo23), minus_f16(code_pair_f16<4>(b, sixteens_f16), hi23)};
+              const uint32_t f1[4] = {minus_f16(code_pair_f16<0>(a8, sixteens_f16), lo01), minus_f16(code_pair_f16<4>(a8, sixteens_f16), hi01),
+                                      minus_f16(code_pair_f16<0>(b8, sixteens_f16), lo23), minus_f16(code_pair_f16<4>(b8, sixteens_f16), hi23)};
+              const int tile = 4 * u + 2 * h;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              if constexpr (PARTS == 1) {
-                mma_bf16(acc[nt][tile], f0, wf[nt][half][0][0], wf[nt][half][1][0]);
-                mma_bf16(acc[nt][tile + 1], f1, wf[nt][half][0][0], wf[nt][half][1][0]);
-              } else {                           // added to the running output by float32 additions: the tensor cores cut sums off
+              for (int nt = 0; nt < NT; ++nt) {
+                mma_f16(acc[nt][tile], f0, wf[nt][half][0][0], wf[nt][half][1][0]);
+                mma_f16(acc[nt][tile + 1], f1, wf[nt][half][0][0], wf[nt][half][1][0]);
+              }
+            }
+          }
+        } else {
+          const uint32_t z01 = __byte_perm(__float_as_uint(z[0]), __float_as_uint(z[1]), 0x7632);
+          const uint32_t z23 = __byte_perm(__float_as_uint(z[2]), __float_as_uint(z[3]), 0x7632);
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t a = __byte_perm(vw[0][u], vw[1][u], h ? 0x7632 : 0x5410), b = __byte_perm(vw[2][u], vw[3][u], h ? 0x7632 : 0x5410);
+              const uint32_t f0[4] = {minus(code_pair<0>(a, sixteens), z01), minus(code_pair<1>(a, sixteens), z01), minus(code_pair<0>(b, sixteens), z23),
+                                      minus(code_pair<1>(b, sixteens), z23)};
+              const uint32_t f1[4] = {minus(code_pair<2>(a, sixteens), z01), minus(code_pair<3>(a, sixteens), z01), minus(code_pair<2>(b, sixteens), z23),
+                                      minus(code_pair<3>(b, sixteens), z23)};
+              const int tile = 4 * u + 2 * h;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {  // added to the running output by float32 additions: the tensor cores cut sums off
                 float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = PARTS - 1; i >= 0; --i) {
@@ -635,61 +720,69 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (at >= end) pdl_launch_dependents();      // this block's last tile is there
 
+    if constexpr (HALF) {                        // codes were taken by 64 and by 4 too small, weights by the scale
+      const float even = 64.f / v_scale, odd = 4.f / v_scale;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          acc[nt][i][0] *= even; acc[nt][i][1] *= even;
+          acc[nt][i][2] *= odd; acc[nt][i][3] *= odd;
+        }
+    }
     // ---- the four warps' results together ----
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], o);
-        if (g == 0) {
-          merge_ml[(warp * COLS + nt * 8 + 2 * t + x) * 2] = m[nt][x];
-          merge_ml[(warp * COLS + nt * 8 + 2 * t + x) * 2 + 1] = l[nt][x];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-        merge_o[(warp * NT * MT + nt * MT + i) * 32 + lane] = make_float4(acc[nt][i][0], acc[nt][i][1], acc[nt][i][2], acc[nt][i][3]);
-    }
-    __syncthreads();
-    const bool whole = n_blocks == 1;
     constexpr int OWN = MT / kWarps;             // tiles of each column block that a warp finishes: its lanes' elements are neighbours
     float4 sum[NT][OWN];
     float top[NT][2], norm[NT][2];
-    auto fold = [&](auto&& ml, auto&& o, int n) {             // n results: ml(i, column) -> (max, sum), o(i, tile) -> float4
+    auto together = [&]() {                      // m, l, acc of every warp -> top, norm, sum
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (g == 0) *reinterpret_cast<float2*>(merge_ml + (warp * COLS + nt * 8 + 2 * t + x) * 2) = make_float2(m[nt][x], l[nt][x]);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+          merge_o[(warp * NT * MT + nt * MT + i) * 32 + lane] = make_float4(acc[nt][i][0], acc[nt][i][1], acc[nt][i][2], acc[nt][i][3]);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float2 ml[kWarps][2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           top[nt][x] = kNone;
           norm[nt][x] = 0.f;
+#pragma unroll
+          for (int k = 0; k < kWarps; ++k) {
+            ml[k][x] = *reinterpret_cast<const float2*>(merge_ml + (k * COLS + nt * 8 + 2 * t + x) * 2);
+            top[nt][x] = fmaxf(top[nt][x], ml[k][x].x);
+          }
         }
 #pragma unroll
         for (int i = 0; i < OWN; ++i) sum[nt][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = 0; k < n; ++k)
 #pragma unroll
-          for (int x = 0; x < 2; ++x) top[nt][x] = fmaxf(top[nt][x], ml(k, nt * 8 + 2 * t + x).x);
-        for (int k = 0; k < n; ++k) {
-          float f[2];
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const float2 one = ml(k, nt * 8 + 2 * t + x);
-            f[x] = exp2f(one.x - top[nt][x]);
-            norm[nt][x] += one.y * f[x];
-          }
+        for (int k = 0; k < kWarps; ++k) {
+          const float f0 = exp2f(ml[k][0].x - top[nt][0]), f1 = exp2f(ml[k][1].x - top[nt][1]);
+          norm[nt][0] += ml[k][0].y * f0;
+          norm[nt][1] += ml[k][1].y * f1;
 #pragma unroll
           for (int i = 0; i < OWN; ++i) {
-            const float4 v = o(k, nt * MT + warp * OWN + i);
-            sum[nt][i].x += v.x * f[0]; sum[nt][i].z += v.z * f[0];
-            sum[nt][i].y += v.y * f[1]; sum[nt][i].w += v.w * f[1];
+            const float4 v = merge_o[(k * NT * MT + nt * MT + warp * OWN + i) * 32 + lane];
+            sum[nt][i].x += v.x * f0; sum[nt][i].z += v.z * f0;
+            sum[nt][i].y += v.y * f1; sum[nt][i].w += v.w * f1;
           }
         }
       }
     };
-    fold([&](int k, int column) { return *reinterpret_cast<const float2*>(merge_ml + (k * COLS + column) * 2); },
-         [&](int k, int tile) { return merge_o[(k * NT * MT + tile) * 32 + lane]; }, kWarps);
-    bool finish = whole;
-    if (!whole) {
+    together();
+    bool finish = n_blocks == 1;
+    if (!finish) {
       // A block's share begins inside one pair and ends inside another at most: two places of its own.
       auto place = [&](int b, bool its_first) { return p.part + ((size_t)b * 2 + (its_first ? 0 : 1)) * PART_FLOATS; };
       float* mine = place(blockIdx.x, first_of_block);
@@ -711,12 +804,43 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       }
       __syncthreads();
       finish = *s_last != 0;
-      if (finish) {
+      if (finish) {                              // the blocks' results, every fourth a warp's, then the warps' as before
         __threadfence();
         const bool begins = pieces > 0 || share(first_block) >= first;      // whether the pair is the first of its first block
-        auto piece = [&](int k) { return place(first_block + k, k > 0 || begins); };
-        fold([&](int k, int column) { return __ldcg(reinterpret_cast<const float2*>(piece(k) + NT * MT * 128 + column * 2)); },
-             [&](int k, int tile) { return __ldcg(reinterpret_cast<const float4*>(piece(k)) + tile * 32 + lane); }, n_blocks);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          m[nt][0] = m[nt][1] = kNone;
+          l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+          for (int i = 0; i < MT; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
+        }
+        for (int k = warp; k < n_blocks; k += kWarps) {
+          const float* from = place(first_block + k, k > 0 || begins);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float4 v[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) v[i] = __ldcg(reinterpret_cast<const float4*>(from) + (nt * MT + i) * 32 + lane);
+            float was[2], is[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float2 ml = __ldcg(reinterpret_cast<const float2*>(from + NT * MT * 128 + (nt * 8 + 2 * t + x) * 2));
+              const float next = fmaxf(m[nt][x], ml.x);
+              was[x] = exp2f(m[nt][x] - next);
+              is[x] = exp2f(ml.x - next);
+              m[nt][x] = next;
+              l[nt][x] = l[nt][x] * was[x] + ml.y * is[x];
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              acc[nt][i][0] = acc[nt][i][0] * was[0] + v[i].x * is[0];
+              acc[nt][i][1] = acc[nt][i][1] * was[1] + v[i].y * is[1];
+              acc[nt][i][2] = acc[nt][i][2] * was[0] + v[i].z * is[0];
+              acc[nt][i][3] = acc[nt][i][3] * was[1] + v[i].w * is[1];
+            }
+          }
+        }
+        together();
       }
     }
     if (finish) {
@@ -776,12 +900,13 @@ YALIS_API long long yalis_packed_attention_mma_scratch_floats(int blocks, int di
   return (long long)blocks * 2 * (nt * (dim / 16) * 128 + 16 * nt);
 }
 
-// `columns`: 8 or 16, the query rows of a pair (float32: 8).
+// `columns`: 8 or 16, the query rows of a pair (float32: 8); `max_rows`: the most that a request has for a KV head.  `blocks`, scratch
+// memory and as many tickets: see above.
 YALIS_API int yalis_packed_attention_mma(const void* q, long long q_stride, int dtype, void* out, long long out_stride, void* k_codes,
                                          void* v_codes, void* words, int num_pages, int page_size, int g, int dim, const int32_t* positions,
                                          const int32_t* q_start, const int32_t* block_table, int table_width, int n_requests, int nh,
                                          int columns, int q_vector, int only_single, float scale, int window, float* lse2, float* scores,
-                                         long long score_stride, int blocks, float* scratch, int32_t* tickets, int32_t* error, cudaStream_t stream) {
+                                         long long score_stride, int max_rows, int blocks, float* scratch, int32_t* tickets, int32_t* error, cudaStream_t stream) {
   if ((dim != 64 && dim != 128) || nh % g || n_requests > 4096 || blocks < 1) return YALIS_ERR_SHAPE;
   if (n_requests <= 0) return YALIS_OK;
   MmaParams p = {};
@@ -789,13 +914,16 @@ YALIS_API int yalis_packed_attention_mma(const void* q, long long q_stride, int 
   p.positions = positions; p.q_start = q_start; p.block_table = block_table; p.table_width = table_width;
   p.n_requests = n_requests; p.nh = nh; p.per = nh / g; p.window = window; p.q_vector = q_vector; p.only_single = only_single;
   p.together = page_size % kChunk == 0 ? 2 : page_size % (1024 / dim) == 0 ? 1 : 0;
+  p.slots = blocks;
+  const long long pairs = (long long)n_requests * g * ((max_rows + columns - 1) / columns), grid = pairs > blocks ? pairs : blocks;
+  if (grid > 0x7fffffffll) return YALIS_ERR_SHAPE;
   p.scale_log2 = scale * 1.4426950408889634f; p.lse2 = lse2; p.scores = scores; p.score_stride = score_stride; p.part = scratch; p.tickets = tickets; p.error = error;
   p.pages = packed_pages(k_codes, v_codes, words, num_pages, page_size, g, dim);
   if (dtype == YALIS_BF16) {
-    if (columns == 8) return dim == 64 ? launch_mma<__nv_bfloat16, 64, 1, 1>(p, blocks, stream) : launch_mma<__nv_bfloat16, 128, 1, 1>(p, blocks, stream);
-    if (columns == 16) return dim == 64 ? launch_mma<__nv_bfloat16, 64, 2, 1>(p, blocks, stream) : launch_mma<__nv_bfloat16, 128, 2, 1>(p, blocks, stream);
+    if (columns == 8) return dim == 64 ? launch_mma<__nv_bfloat16, 64, 1, 1>(p, (int)grid, stream) : launch_mma<__nv_bfloat16, 128, 1, 1>(p, (int)grid, stream);
+    if (columns == 16) return dim == 64 ? launch_mma<__nv_bfloat16, 64, 2, 1>(p, (int)grid, stream) : launch_mma<__nv_bfloat16, 128, 2, 1>(p, (int)grid, stream);
   }
   if (dtype == YALIS_F32 && columns == 8)
-    return dim == 64 ? launch_mma<float, 64, 1, 3>(p, blocks, stream) : launch_mma<float, 128, 1, 3>(p, blocks, stream);
+    return dim == 64 ? launch_mma<float, 64, 1, 3>(p, (int)grid, stream) : launch_mma<float, 128, 1, 3>(p, (int)grid, stream);
   return YALIS_ERR_DTYPE;
 }

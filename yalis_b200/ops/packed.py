@@ -314,9 +314,9 @@ def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tenso
             scores = torch.empty(n * num_heads * max_kv_len, dtype=torch.float32, device=device)
         blocks, floats = _mma_launch(device, code, dim, tile)
         counters, scratch = _workspace(device, raw, blocks, floats)
-        check(_entry("yalis_packed_attention_mma", "plipl" + "pppiiii" + "pppii" + "iiiifipplipppp")(
+        check(_entry("yalis_packed_attention_mma", "plipl" + "pppiiii" + "pppii" + "iiiifippliipppp")(
             q_at, step, code, out_at, out_step, *held, *at, num_heads, tile, aligned, single, scale, window, _address(lse2), _address(scores),
-            max_kv_len, blocks, scratch.data_ptr(), counters.data_ptr(), flag, raw), name)
+            max_kv_len, q_rows, blocks, scratch.data_ptr(), counters.data_ptr(), flag, raw), name)
     elif not unpack:
         check(_entry("yalis_packed_attention_general", "plipl" + "pppiiii" + "pppii" + "iifippp")(
             q_at, step, code, out_at, out_step, *held, *at, n, num_heads, scale, window, _address(lse2), flag, raw), name)

@@ -33,6 +33,7 @@ constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kChunk = 32;     // keys of a chunk
 constexpr int kStages = 2;
 constexpr float kNone = -1e30f;  // the maximum of no scores
+constexpr float kUnset = -3e38f; // limit of a column that has seen no score yet: any will do
 constexpr float kLazy = 8.f;   // how far (log2) scores may rise above the maximum in use before the output is rescaled
 
 struct MmaParams {
@@ -205,6 +206,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint32_t sixteens;
   asm volatile("mov.b32 %0, 0x41804180;" : "=r"(sixteens));
+  // Where this lane finds its operands in a chunk (rows eight and sixteen further on lie as many rows further).
+  const int own_key = key_of_row<DIM>(g), v_key[2] = {key_of_row<DIM>(2 * t), key_of_row<DIM>(2 * t + 1)};
+  const int k_own = DIM == 128 ? piece_at<DIM>(own_key, t) : own_key * (DIM / 2) + t * 8;
+  const int v_own[2] = {DIM == 128 ? piece_at<DIM>(v_key[0], g >> 1) + (g & 1) * 8 : v_key[0] * (DIM / 2) + g * 4,
+                        DIM == 128 ? piece_at<DIM>(v_key[1], g >> 1) + (g & 1) * 8 : v_key[1] * (DIM / 2) + g * 4};
   uint32_t sixteens_f16;
   asm volatile("mov.b32 %0, 0x4C004C00;" : "=r"(sixteens_f16));
   pdl_wait();
@@ -329,13 +335,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       any_lo = min(any_lo, __shfl_xor_sync(0xffffffffu, any_lo, o));
     }
 
-    float m[NT][2], l[NT][2], acc[NT][MT][4];
+    // Scores are taken relative to base; one above limit moves it.
+    float base[NT][2], limit[NT][2], l[NT][2], acc[NT][MT][4];
     uint32_t v_top = 0u;                         // HALF: no step up to this needs another scale
     float v_scale = 1.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = kNone;
-      l[nt][0] = l[nt][1] = 0.f;
+      base[nt][0] = base[nt][1] = l[nt][0] = l[nt][1] = 0.f;
+      limit[nt][0] = limit[nt][1] = kUnset;
 #pragma unroll
       for (int i = 0; i < MT; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
     }
@@ -348,32 +355,35 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       const int skip = (any_lo - first_key) / kChunk;
       while (c < skip) c += kWarps;
     }
-    auto lookup = [&](int chunk) {               // the pool's row of the lane's key; -1 without a page, -2 for nobody's key
-      const int key0 = first_key + chunk * kChunk, key = key0 + lane, from = p.together == 2 ? key0 : key;
-      if (p.together != 2 && key > any_hi) return -2;
-      const int index = p.pages.shift >= 0 ? from >> p.pages.shift : from / p.pages.page_size;
+    // The pool's row of the chunk's first key (chunks inside pages) or of the lane's key, -1 without a page or for nobody's key.
+    auto lookup = [&](int chunk) {
+      const int key0 = first_key + chunk * kChunk, key = p.together == 2 ? key0 : key0 + lane;
+      if (key > any_hi) return -1;
+      const int index = p.pages.shift >= 0 ? key >> p.pages.shift : key / p.pages.page_size;
       const int page = index < p.table_width ? table_row[index] : -1;
       if ((unsigned)page >= (unsigned)p.pages.num_pages) {
-        if (min(key0 + kChunk - 1, any_hi) >= any_lo && (p.together == 2 || key >= any_lo) && p.error) atomicOr(p.error, YALIS_FLAG_BAD_PAGE);
+        if ((p.together == 2 ? key0 + kChunk - 1 : key) >= any_lo && p.error) atomicOr(p.error, YALIS_FLAG_BAD_PAGE);
         return -1;
       }
-      return key > any_hi ? -2 : (page * p.pages.g + kvh) * p.pages.page_size + (key - index * p.pages.page_size);
+      return (page * p.pages.g + kvh) * p.pages.page_size + (key - index * p.pages.page_size);
     };
-    auto ask = [&](int stage, int row) {         // rows that are not there are left as they are: their word says so
+    // Rows that are not there are left as they are: their word says so.
+    auto ask = [&](int chunk, int stage, int row) {
       Stage<DIM>& st = ring[stage];
       const uint32_t k_at = smem_u32(st.k), v_at = smem_u32(st.v);
       if (p.together == 2) {                     // (rows behind the last key are copied too, here and below)
-        const int from = __shfl_sync(0xffffffffu, row, 0);
-        if (from >= 0) {
+        if (row >= 0) {
           const uint32_t own = piece_at<DIM>(lane / PIECES, lane % PIECES);
-          const size_t byte = (size_t)from * (DIM / 2) + lane * 16;
+          const size_t byte = (size_t)row * (DIM / 2) + lane * 16;
           const unsigned char *k_from = reinterpret_cast<const unsigned char*>(p.pages.k) + byte, *v_from = reinterpret_cast<const unsigned char*>(p.pages.v) + byte;
 #pragma unroll
           for (int i = 0; i < COPIES; ++i) {
             copy16(k_at + own + i * 512, k_from + i * 512);
             copy16(v_at + own + i * 512, v_from + i * 512);
           }
+          row += lane;
         }
+        if (first_key + chunk * kChunk + lane > any_hi) row = -1;
       } else if (p.together) {                   // a lane's pieces are neighbours of the group's first row
         const uint32_t own = piece_at<DIM>(lane / PIECES, lane % PIECES);
 #pragma unroll
@@ -400,11 +410,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       if (row >= 0) copy4(smem_u32(&st.words[lane]), p.pages.words + row);
       else st.words[lane] = 0u;
     };
-    int row = c < c_end ? lookup(c) : -2;
-    if (c < c_end) ask(0, row);
+    int row = -1;
+    if (c < c_end) ask(c, 0, lookup(c));
     asm volatile("cp.async.commit_group;" ::: "memory");
-    bool missing = __any_sync(0xffffffffu, row < 0);
-    row = c + kWarps < c_end ? lookup(c + kWarps) : -2;
+    if (c + kWarps < c_end) row = lookup(c + kWarps);
 
     // ---- queries in registers as the products' right operand, while the first copies are under way ----
     uint32_t qf[NT][2 * W][2][PARTS];
@@ -443,8 +452,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
     }
 
     for (int stage = 0; c < c_end; c += kWarps, stage ^= 1) {
-      const bool missing_next = __any_sync(0xffffffffu, row < 0);
-      if (c + kWarps < c_end) ask(stage ^ 1, row);
+      if (c + kWarps < c_end) ask(c + kWarps, stage ^ 1, row);
       asm volatile("cp.async.commit_group;" ::: "memory");
       if (c + 2 * kWarps < c_end) row = lookup(c + 2 * kWarps);
       asm volatile("cp.async.wait_group 1;" ::: "memory");
@@ -456,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       // to eleven bits down to 2^-14.
       if constexpr (HALF) {
         const uint32_t largest = __reduce_max_sync(0xffffffffu, own.z == own.z ? __float_as_uint(own.z) : 0u);
-        if (largest > v_top) {
+        if (__any_sync(0xffffffffu, largest > v_top)) {      // (the vote says that the whole warp goes one way)
           const float fewer = v_scale;
           v_top = largest | 0x007FFFFFu;
           v_scale = __uint_as_float(0x82000000u - max(largest & 0x7F800000u, 0x04000000u));       // 2^(6 - e) for a step of 2^e and more
@@ -480,16 +488,16 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       float4 term[2][2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int ra = half * 16 + key_of_row<DIM>(g), rb = ra + 8;
-        term[half][0] = terms[ra];
-        term[half][1] = terms[rb];
+        term[half][0] = terms[own_key + half * 16];
+        term[half][1] = terms[own_key + half * 16 + 8];
         uint32_t wa[W], wb[W];
+        const unsigned char* from = st.k + k_own + half * 16 * (DIM / 2);
         if constexpr (DIM == 128) {
-          *reinterpret_cast<uint4*>(wa) = *reinterpret_cast<const uint4*>(st.k + piece_at<DIM>(ra, t));
-          *reinterpret_cast<uint4*>(wb) = *reinterpret_cast<const uint4*>(st.k + piece_at<DIM>(rb, t));
+          *reinterpret_cast<uint4*>(wa) = *reinterpret_cast<const uint4*>(from);
+          *reinterpret_cast<uint4*>(wb) = *reinterpret_cast<const uint4*>(from + 8 * (DIM / 2));
         } else {
-          *reinterpret_cast<uint2*>(wa) = *reinterpret_cast<const uint2*>(st.k + ra * (DIM / 2) + t * 8);
-          *reinterpret_cast<uint2*>(wb) = *reinterpret_cast<const uint2*>(st.k + rb * (DIM / 2) + t * 8);
+          *reinterpret_cast<uint2*>(wa) = *reinterpret_cast<const uint2*>(from);
+          *reinterpret_cast<uint2*>(wb) = *reinterpret_cast<const uint2*>(from + 8 * (DIM / 2));
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) sc[nt][half][0] = sc[nt][half][1] = sc[nt][half][2] = sc[nt][half][3] = 0.f;
@@ -538,66 +546,54 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
               for (int half = 0; half < 2; ++half)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                  const int j = half * 16 + key_of_row<DIM>(g) + 8 * e;
+                  const int j = half * 16 + own_key + 8 * e;
                   if (!MASK || key0 + j <= see_hi[nt][x])
                     to[j] = MASK && term[half][e].x == 0.f ? -INFINITY : term[half][e].x * sc[nt][half][2 * e + x];
                 }
             }
         }
         float most[NT][2];
-        auto scores = [&](float (&to)[NT][2][4]) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) most[nt][0] = most[nt][1] = -INFINITY;
+        for (int nt = 0; nt < NT; ++nt) most[nt][0] = most[nt][1] = -INFINITY;
 #pragma unroll
-          for (int half = 0; half < 2; ++half)
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) to[nt][half][i] = fmaf(term[half][i >> 1].x, sc[nt][half][i], -m[nt][i & 1]);
-          if constexpr (MASK) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const int key = key0 + half * 16 + key_of_row<DIM>(g) + 8 * (i >> 1);
-                  if (!(key <= see_hi[nt][i & 1] && key >= see_lo[nt][i & 1] && term[half][i >> 1].x != 0.f)) to[nt][half][i] = -INFINITY;
-                }
-          }
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) most[nt][i & 1] = fmaxf(most[nt][i & 1], to[nt][half][i]);
-        };
-        float ex[NT][2][4];
-        scores(ex);
+            for (int i = 0; i < 4; ++i) {
+              float& v = sc[nt][half][i];
+              v = fmaf(term[half][i >> 1].x, v, -base[nt][i & 1]);
+              if constexpr (MASK) {
+                const int key = key0 + half * 16 + own_key + 8 * (i >> 1);
+                if (!(key <= see_hi[nt][i & 1] && key >= see_lo[nt][i & 1] && term[half][i >> 1].x != 0.f)) v = -INFINITY;
+              }
+              most[nt][i & 1] = fmaxf(most[nt][i & 1], v);
+            }
         bool grow = false;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) grow |= fmaxf(most[nt][0], most[nt][1]) > kLazy;
-        if (__any_sync(0xffffffffu, grow)) {       // seldom after the first chunks: the maximum moves, what was summed is rescaled
+        for (int nt = 0; nt < NT; ++nt) grow |= most[nt][0] > limit[nt][0] || most[nt][1] > limit[nt][1];
+        if (__any_sync(0xffffffffu, grow)) {       // seldom after the first chunks: the base moves, what was summed is rescaled
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float keep[2];
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const float old = m[nt][x];
-              // (the first maximum is taken from scores that kNone has swallowed: once more from the products)
-              float top = most[nt][x] == -INFINITY ? -INFINITY : old == kNone ? -INFINITY : most[nt][x] + old;
-              if (old == kNone) {
-#pragma unroll
-                for (int half = 0; half < 2; ++half)
-#pragma unroll
-                  for (int e = 0; e < 2; ++e)
-                    if (ex[nt][half][2 * e + x] != -INFINITY) top = fmaxf(top, term[half][e].x * sc[nt][half][2 * e + x]);
-              }
+              float top = most[nt][x];
 #pragma unroll
               for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-              m[nt][x] = fmaxf(old, top);
-              keep[x] = exp2_fast(old - m[nt][x]);
+              float up = fmaxf(top, 0.f);
+              keep[x] = exp2_fast(-up);
+              if (limit[nt][x] == kUnset) {        // nothing summed yet: the first maximum, wherever it lies
+                up = top == -INFINITY ? 0.f : top;
+                limit[nt][x] = top == -INFINITY ? kUnset : kLazy;
+                keep[x] = 1.f;
+              }
+              base[nt][x] += up;
               l[nt][x] *= keep[x];
+#pragma unroll
+              for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) sc[nt][half][2 * e + x] -= up;
             }
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
@@ -605,7 +601,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
               acc[nt][i][2] *= keep[0]; acc[nt][i][3] *= keep[1];
             }
           }
-          scores(ex);
         }
 #pragma unroll
         for (int half = 0; half < 2; ++half)
@@ -613,21 +608,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float e = PARTS == 1 ? exp2_fast(ex[nt][half][i]) : exp2f(ex[nt][half][i]);
+              const float v = sc[nt][half][i], e = PARTS == 1 ? exp2_fast(v) : exp2f(v);
               l[nt][i & 1] += e;
-              sc[nt][half][i] = e * term[half][i >> 1].z;
+              sc[nt][half][i] = MASK && v == -INFINITY ? 0.f : e * term[half][i >> 1].z;         // a row that is not seen may hold anything
             }
-        if constexpr (MASK) {                      // a row that is not seen may hold anything
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (ex[nt][half][i] == -INFINITY) sc[nt][half][i] = 0.f;
-        }
       };
-      if (missing || key0 + kChunk - 1 > all_hi || key0 < all_lo) weigh(std::true_type());
+      if (__any_sync(0xffffffffu, key0 + kChunk - 1 > all_hi || key0 < all_lo)) weigh(std::true_type());
       else weigh(std::false_type());
       uint32_t wf[NT][2][2][PARTS];              // [half][keys g, g + 8 of the half]: the weights as the second product's operand
 #pragma unroll
@@ -652,14 +638,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
         float z[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {            // keys of rows 2t, 2t + 1, 2t + 8, 2t + 9
-          const int r = half * 16 + key_of_row<DIM>(2 * t + (i & 1) + (i & 2) * 4);
-          z[i] = terms[r].w;
+          z[i] = terms[v_key[i & 1] + half * 16 + (i & 2) * 4].w;
+          const unsigned char* from = st.v + v_own[i & 1] + (half * 16 + (i & 2) * 4) * (DIM / 2);
           if constexpr (DIM == 128) {
-            const uint2 two = *reinterpret_cast<const uint2*>(st.v + piece_at<DIM>(r, g >> 1) + (g & 1) * 8);
+            const uint2 two = *reinterpret_cast<const uint2*>(from);
             vw[i][0] = two.x;
             vw[i][U - 1] = two.y;
           } else {
-            vw[i][0] = *reinterpret_cast<const uint32_t*>(st.v + r * (DIM / 2) + g * 4);
+            vw[i][0] = *reinterpret_cast<const uint32_t*>(from);
           }
         }
         if constexpr (HALF) {
@@ -714,7 +700,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
           }
         }
       }
-      missing = missing_next;
       __syncwarp();                              // the stage is read: the next round may fill it
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -740,12 +725,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
     constexpr int OWN = MT / kWarps;             // tiles of each column block that a warp finishes: its lanes' elements are neighbours
     float4 sum[NT][OWN];
     float top[NT][2], norm[NT][2];
-    auto together = [&]() {                      // m, l, acc of every warp -> top, norm, sum
+    auto together = [&]() {                      // base, l, acc of every warp -> top, norm, sum
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int x = 0; x < 2; ++x)
-          if (g == 0) *reinterpret_cast<float2*>(merge_ml + (warp * COLS + nt * 8 + 2 * t + x) * 2) = make_float2(m[nt][x], l[nt][x]);
+          if (g == 0) *reinterpret_cast<float2*>(merge_ml + (warp * COLS + nt * 8 + 2 * t + x) * 2) = make_float2(limit[nt][x] == kUnset ? kNone : base[nt][x], l[nt][x]);
 #pragma unroll
         for (int i = 0; i < MT; ++i)
           merge_o[(warp * NT * MT + nt * MT + i) * 32 + lane] = make_float4(acc[nt][i][0], acc[nt][i][1], acc[nt][i][2], acc[nt][i][3]);
@@ -809,7 +794,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
         const bool begins = pieces > 0 || share(first_block) >= first;      // whether the pair is the first of its first block
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          m[nt][0] = m[nt][1] = kNone;
+          base[nt][0] = base[nt][1] = kNone;
+          limit[nt][0] = limit[nt][1] = kLazy;
           l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
           for (int i = 0; i < MT; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
@@ -825,10 +811,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               const float2 ml = __ldcg(reinterpret_cast<const float2*>(from + NT * MT * 128 + (nt * 8 + 2 * t + x) * 2));
-              const float next = fmaxf(m[nt][x], ml.x);
-              was[x] = exp2f(m[nt][x] - next);
+              const float next = fmaxf(base[nt][x], ml.x);
+              was[x] = exp2f(base[nt][x] - next);
               is[x] = exp2f(ml.x - next);
-              m[nt][x] = next;
+              base[nt][x] = next;
               l[nt][x] = l[nt][x] * was[x] + ml.y * is[x];
             }
 #pragma unroll

@@ -78,4 +78,21 @@ __device__ __forceinline__ float multiple_of(float x, float step, float inverse)
   return n;
 }
 
+// The eight values of a word of codes as bfloat16, in order; exact.  Codes go into the middle bits of bytes 0x80 | c << 3, which under
+// bytes 0x41 are the bfloat16 numbers 16 + c.
+__device__ __forceinline__ uint4 unpack_bf16(uint32_t codes, uint32_t word16) {
+  const uint32_t even = (codes << 3 & 0x78787878u) | 0x80808080u, odd = (codes >> 1 & 0x78787878u) | 0x80808080u;
+  const uint32_t low = __byte_perm(even, odd, 0x5140), high = __byte_perm(even, odd, 0x7362);        // codes 0 .. 3, 4 .. 7
+  const uint32_t zero = ((word16 & 15u) << 3 | 0x4180u) * 0x10001u, step = (word16 & 0xFFF0u) * 0x10001u;
+  uint32_t pair[4] = {__byte_perm(low, 0x41414141u, 0x4140), __byte_perm(low, 0x41414141u, 0x4342), __byte_perm(high, 0x41414141u, 0x4140),
+                      __byte_perm(high, 0x41414141u, 0x4342)};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 v = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&pair[i]), *reinterpret_cast<const __nv_bfloat162*>(&zero)),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&step));
+    pair[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return make_uint4(pair[0], pair[1], pair[2], pair[3]);
+}
+
 }  // namespace

@@ -184,21 +184,14 @@ __global__ void packed_rows_read_kernel(const RowParams<T> p) {
   for (int i = 0; i < TOKENS; ++i) {
     const int token = blockIdx.x * TOKENS + i;
     if (token >= p.n_tokens) return;
-    const float step = step_of(word[i]), zero = zero_of(word[i]);
-    float x[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = ((float)((codes[i] >> (4 * j)) & 15u) - zero) * step;
     T* dst = (is_v ? p.v_out : p.k_out) + ((size_t)token * p.pages.g + kvh) * p.pages.dim + lane * 8;
     if constexpr (sizeof(T) == 2) {
-      uint4 u;
-      uint32_t* w = &u.x;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const __nv_bfloat162 two = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
-        w[j] = *reinterpret_cast<const uint32_t*>(&two);
-      }
-      *reinterpret_cast<uint4*>(dst) = u;
+      *reinterpret_cast<uint4*>(dst) = unpack_bf16(codes[i], word[i]);
     } else {
+      const float step = step_of(word[i]), zero = zero_of(word[i]);
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = ((float)((codes[i] >> (4 * j)) & 15u) - zero) * step;
       store4(dst, make_float4(x[0], x[1], x[2], x[3]));
       store4(dst + 4, make_float4(x[4], x[5], x[6], x[7]));
     }
@@ -263,29 +256,37 @@ __global__ void __launch_bounds__(256) packed_unpack_kernel(const UnpackParams p
   const int first = p.window > 0 ? max(0, begin - p.window + 1) : 0;
   if (key0 > last || key0 + kUnpackPage <= first) return;
   const size_t to = (((size_t)req * p.width + index) * p.pages.g + kvh) * kUnpackPage;
-  const int rows = min(kUnpackPage, last - key0 + 1);
-  for (int i = threadIdx.x; i < rows * words; i += 256) {
-    const int r = i / words, w = i - r * words, key = key0 + r;
-    int row;
-    const int page = page_of(p.pages, p.block_table + (size_t)req * p.table_width, p.table_width, key, row);
-    uint4 k = make_uint4(0u, 0u, 0u, 0u), v = k;
-    if (page >= 0) {
-      const size_t at = row_index(p.pages, page, kvh, row);
-      const uint32_t word = p.pages.words[at], kc = p.pages.k[at * words + w], vc = p.pages.v[at * words + w];
-      const float ks = step_of(word & 0xFFFFu), kz = zero_of(word), vs = step_of(word >> 16), vz = zero_of(word >> 16);
-      uint32_t* out[2] = {&k.x, &v.x};
+  // A thread has the same word of codes of every 256 / words-th row: four rows' look-ups and loads are under way at a time.
+  const int rows = min(kUnpackPage, last - key0 + 1), w = threadIdx.x % words, per_round = 256 / words;
+  if ((int)threadIdx.x >= per_round * words) return;
+  for (int r0 = threadIdx.x / words; r0 < rows; r0 += 4 * per_round) {
+    long long at[4];
+    uint32_t word[4], kc[4], vc[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const __nv_bfloat162 a = __floats2bfloat162_rn(((float)(kc >> (8 * e) & 15u) - kz) * ks, ((float)(kc >> (8 * e + 4) & 15u) - kz) * ks);
-        const __nv_bfloat162 b = __floats2bfloat162_rn(((float)(vc >> (8 * e) & 15u) - vz) * vs, ((float)(vc >> (8 * e + 4) & 15u) - vz) * vs);
-        out[0][e] = *reinterpret_cast<const uint32_t*>(&a);
-        out[1][e] = *reinterpret_cast<const uint32_t*>(&b);
-      }
-    } else if (key >= first && w == 0 && p.error) {
-      atomicOr(p.error, YALIS_FLAG_BAD_PAGE);
+    for (int i = 0; i < 4; ++i) {
+      const int r = r0 + i * per_round, key = key0 + r;
+      at[i] = -1;
+      if (r >= rows) continue;
+      int row;
+      const int page = page_of(p.pages, p.block_table + (size_t)req * p.table_width, p.table_width, key, row);
+      if (page >= 0) at[i] = (long long)row_index(p.pages, page, kvh, row);
+      else if (key >= first && w == 0 && p.error) atomicOr(p.error, YALIS_FLAG_BAD_PAGE);
     }
-    reinterpret_cast<uint4*>(p.k_out)[(to + r) * words + w] = k;
-    reinterpret_cast<uint4*>(p.v_out)[(to + r) * words + w] = v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      word[i] = kc[i] = vc[i] = 0u;                           // (a key without a page: zeros)
+      if (at[i] < 0) continue;
+      word[i] = p.pages.words[at[i]];
+      kc[i] = p.pages.k[at[i] * words + w];
+      vc[i] = p.pages.v[at[i] * words + w];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = r0 + i * per_round;
+      if (r >= rows) break;
+      reinterpret_cast<uint4*>(p.k_out)[(to + r) * words + w] = unpack_bf16(kc[i], word[i] & 0xFFFFu);
+      reinterpret_cast<uint4*>(p.v_out)[(to + r) * words + w] = unpack_bf16(vc[i], word[i] >> 16);
+    }
   }
 }
 

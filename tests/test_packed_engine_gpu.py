@@ -1,0 +1,79 @@
+"""Generation with keys and values held in 4 bits: against the plain implementation whose keys and values are packed the same way."""
+
+import numpy as np
+import pytest
+import torch
+
+import plain_llama as plain
+from packed_plain import pack, quantize, values
+from test_generate_gpu import engine_for, prompts_for
+from tiny import page_size_of, tiny_model_dir
+
+pytestmark = pytest.mark.gpu
+
+
+def packed(x):
+    code, word = quantize(x)
+    return values(pack(code), word).to(x.dtype)
+
+
+@pytest.fixture
+def plain_packed(monkeypatch):
+    """The plain implementation with every key (rotated) and value replaced by what 4 bits hold of it."""
+    whole = plain.causal_attention
+    monkeypatch.setattr(plain, "causal_attention", lambda q, k, v, *a, **o: whole(q, packed(k), packed(v), *a, **o))
+
+
+@pytest.mark.parametrize("which, lengths, new, chunk", [("A", [5, 17, 33], 12, None), ("B", [1, 40, 100], 10, 24), ("C", [5, 70, 33], 12, None), ("D", [9, 40], 8, 16)])
+def test_greedy_generation_equals_plain_float32(plain_packed, which, lengths, new, chunk):
+    d = tiny_model_dir(which, 0.3)
+    cfg, w = plain.read_config(d), plain.read_weights(d)
+    prompts = prompts_for(cfg, lengths)
+    eng = engine_for(d, "fp32", page_size=page_size_of(which), prefill_chunk=chunk, max_tokens_per_step=64, cache_bits=4)
+    tokens, _, logits = eng.generate(prompts, tokens_to_generate=new, get_logits=True)
+    for p, row, lg in zip(prompts, tokens.tolist(), logits):
+        assert row == plain.greedy_generate(p, new, w, cfg)
+        ref = plain.forward_logits(p + row[:-1], w, cfg)[len(p) - 1:]
+        assert np.abs(lg.cpu().numpy() - ref.numpy()).max() <= 1e-4 * float(ref.abs().max())
+    eng.engine.manager.check()
+    assert all(eng.engine.manager.free_pages(g.name) == g.num_pages for g in eng.engine.groups)
+
+
+@pytest.mark.parametrize("which", ["C", "D"])
+def test_bfloat16_recorded_steps_are_the_launched_ones(which):
+    """Decode steps replayed from recordings, prompts long enough for the unpacked form: the same tokens as launch by launch, and
+    a cache of little more than a quarter of the bytes."""
+    d = tiny_model_dir(which, 0.02)
+    cfg = plain.read_config(d)
+    prompts = prompts_for(cfg, [5, 90, 33, 64])
+    got = []
+    for graphs in (True, False):
+        eng = engine_for(d, "bf16", page_size=16, cache_bits=4, use_graphs=graphs)
+        got.append([eng.generate(prompts, tokens_to_generate=20)[0].tolist() for _ in range(2)])
+        eng.engine.check_device_errors()
+        small = eng.engine.storage.bytes
+    assert got[0][0] == got[0][1] == got[1][0] == got[1][1]
+    whole = engine_for(d, "bf16", page_size=16).engine.storage.bytes
+    head = cfg["head_dim"]
+    assert small * 2 * head * 2 == whole * (head + 4)
+
+
+def test_bfloat16_follows_the_oracle(plain_packed):
+    """Every generated token is the oracle's best or within rounding of it."""
+    d = tiny_model_dir("C", 0.02)
+    cfg, w = plain.read_config(d), plain.read_weights(d)
+    prompts = prompts_for(cfg, [5, 100, 33])
+    tokens, _ = engine_for(d, "bf16", page_size=page_size_of("C"), cache_bits=4).generate(prompts, tokens_to_generate=16)
+    for p, row in zip(prompts, tokens.tolist()):
+        seq = list(p)
+        for tok in row:
+            ref = plain.forward_logits(seq, w, cfg)[-1]
+            assert float(ref.max() - ref[tok]) <= 0.05 * float(ref.abs().max())
+            seq.append(tok)
+
+
+def test_caches_that_cannot_be_packed_are_refused():
+    from yalis_b200.config.presets import preset
+    from yalis_b200.engine.engine import Engine
+    with pytest.raises(ValueError, match="4 bits"):
+        Engine(config=preset("vepivik-tiny-A"), cache_bits=4, max_slots=2)

@@ -51,3 +51,17 @@ def test_argument_types_are_those_of_the_library():
     assert len(used) >= 6
     for name, signature in used:
         assert "".join(re.findall(r'"([plif]*)"', signature)) == entries[name], name
+
+
+def test_options_of_a_packed_cache():
+    from yalis_b200 import InferenceConfig
+    from yalis_b200.cache.storage import group_page_bytes
+    from yalis_b200.config.engine_config import EngineConfig
+    from yalis_b200.parts.base import PagedKV
+    for bad in (8, 2, True, "4"):
+        with pytest.raises(ValueError, match="cache_bits"):
+            EngineConfig(cache_bits=bad)
+    assert InferenceConfig(cache_bits=4).engine_config("bf16").cache_bits == 4 and EngineConfig().cache_bits is None
+    request = PagedKV(8, 128, packable=True)
+    assert group_page_bytes([request], [None], 64, 2, 4) == {"kv_all": 8 * 64 * (128 + 4)}
+    assert group_page_bytes([request], [None], 64, 2) == {"kv_all": 8 * 64 * 512}

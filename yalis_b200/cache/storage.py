@@ -24,7 +24,8 @@ import torch
 
 from collections.abc import Mapping
 
-from yalis_b200.parts.base import PagedKV, PagedKVCache, SlotState, SlotStateCache, cache_leaves
+from yalis_b200.ops.packed import PackedPages
+from yalis_b200.parts.base import PackedKVCache, PagedKV, PagedKVCache, SlotState, SlotStateCache, cache_leaves
 from .manager import PageGroup
 
 
@@ -36,15 +37,17 @@ def group_name(request: PagedKV) -> str:
 
 
 def group_page_bytes(requests: List[Optional[object]], cache_of: List[Optional[int]], page_size: int,
-                     element_size: int) -> Dict[str, int]:
+                     element_size: int, cache_bits: Optional[int] = None) -> Dict[str, int]:
     """Bytes that one page id of each group stands for: the K and V pages of every schedule entry of the group
-    that keeps a cache of its own (of a group with a row per P tokens, the P-th part: it has so many fewer pages)."""
+    that keeps a cache of its own (of a group with a row per P tokens, the P-th part: it has so many fewer pages).
+    ``cache_bits`` 4: rows held in 4 bits, with a 16-bit word each."""
     out: Dict[str, int] = {}
     for top, src in zip(requests, cache_of):
         for req in cache_leaves(top):
             if isinstance(req, PagedKV) and src is None:
                 name = group_name(req)
-                out[name] = out.get(name, 0) + -(-req.num_kv_heads * page_size * (req.head_dim + req.value_dim) * element_size // req.pool)
+                row = (req.head_dim + req.value_dim) * element_size if cache_bits is None else (req.head_dim + req.value_dim) // 2 + 4
+                out[name] = out.get(name, 0) + -(-req.num_kv_heads * page_size * row // req.pool)
     return out
 
 
@@ -80,7 +83,8 @@ class CacheStorage:
     """Allocates what every schedule entry asked for and hands out the per-entry views."""
 
     def __init__(self, requests: List[Optional[object]], cache_of: List[Optional[int]], groups: List[PageGroup],
-                 max_slots: int, device, dtype: torch.dtype):
+                 max_slots: int, device, dtype: torch.dtype, cache_bits: Optional[int] = None):
+        self._cache_bits = cache_bits
         self._by_name = {g.name: g for g in groups}
         self._max_slots, self._device, self._dtype = max_slots, device, dtype
         self.entries: List[Optional[object]] = []
@@ -102,6 +106,10 @@ class CacheStorage:
             if not isinstance(req, PagedKV) or (req.num_kv_heads, req.head_dim, req.value_dim) != (own.k.shape[1], own.k.shape[3], own.v.shape[3]):
                 raise ValueError(f"schedule entry {i} cannot read the cache of entry {src}: shapes differ")
             return PagedKVCache(own.k, own.v, own.group, writable=False)
+        if isinstance(own, PackedKVCache):
+            if not isinstance(req, PagedKV) or not req.packable or (req.num_kv_heads, req.head_dim) != (own.pages.num_kv_heads, own.pages.head_dim):
+                raise ValueError(f"schedule entry {i} cannot read the cache of entry {src}, which is held in 4 bits")
+            return PackedKVCache(own.pages, own.group, writable=False)
         if isinstance(own, SlotStateCache):
             return SlotStateCache(own.state, writable=False)
         raise ValueError(f"schedule entry {i} reads the cache of entry {src}, which keeps none")
@@ -114,6 +122,13 @@ class CacheStorage:
         if isinstance(req, PagedKV):
             g = self._by_name[group_name(req)]
             rows = g.page_size // req.pool
+            if self._cache_bits is not None:
+                if not req.packable or req.pool != 1 or req.value_dim != req.head_dim or req.head_dim % 8:
+                    raise ValueError(f"schedule entry {i}: its cache cannot be held in 4 bits (only plain paged attention's, with head sizes "
+                                     "that are multiples of 8)")
+                pages = PackedPages.empty(g.num_pages, req.num_kv_heads, rows, req.head_dim, self._device)
+                self.bytes += sum(t.numel() * t.element_size() for t in pages.pools())
+                return PackedKVCache(pages, g.name)
             k = torch.empty((g.num_pages, req.num_kv_heads, rows, req.head_dim), dtype=self._dtype, device=self._device)
             v = torch.empty((g.num_pages, req.num_kv_heads, rows, req.value_dim), dtype=self._dtype, device=self._device)
             self.bytes += k.numel() * k.element_size() + v.numel() * v.element_size()

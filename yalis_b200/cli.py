@@ -55,6 +55,7 @@ def build_parser() -> argparse.ArgumentParser:
                    help="size of the page pool as a share of the device memory free after loading")
     e.add_argument("--no-graphs", action="store_true", help="launch every step kernel by kernel")
     e.add_argument("--max-tokens-per-step", type=int, default=2048)
+    e.add_argument("--cache-bits", type=int, default=None, choices=(4,), help="hold keys and values in 4 bits (plain paged attention only)")
     e.add_argument("--chunk", "--prefill-chunk", dest="prefill_chunk", type=int, default=None)
     p = ap.add_argument_group("prompts")
     p.add_argument("--prompt-ids", action="append", default=[], metavar="I,J,K", help="one prompt as token ids (repeatable)")
@@ -91,7 +92,8 @@ def main(argv=None) -> int:
         max_batch_size=args.max_batch_size, max_length_of_generated_sequences=args.max_length, top_k=args.top_k,
         top_p=args.top_p, temperature=args.temperature, page_size=args.page_size, cache_tokens=args.cache_tokens,
         num_pages=args.num_pages, memory_fraction=args.memory_fraction, use_graphs=not args.no_graphs,
-        max_tokens_per_step=args.max_tokens_per_step, prefill_chunk=args.prefill_chunk, seed=args.sampling_seed)
+        max_tokens_per_step=args.max_tokens_per_step, prefill_chunk=args.prefill_chunk, seed=args.sampling_seed,
+        cache_bits=args.cache_bits)
     engine = LLMEngine(model_config=model_config, inference_config=inference_config)
 
     prompts = [_ids(p) for p in args.prompt_ids]

@@ -31,6 +31,8 @@ class EngineConfig:
     max_tokens_per_step token budget of one step (decoding requests first, the rest to prompt portions).
     prefill_chunk       largest portion of one prompt in a step (None: the step's budget).
     max_context         most tokens a request may hold (None: the model's limit).
+    cache_bits          4: keys and values are held in 4 bits (models whose caches all belong to plain paged attention, head
+                        sizes that are multiples of 8); None: in ``dtype``.
     use_graphs          replay recorded steps where a step's shape allows it.
     device              the CUDA device.
     """
@@ -44,6 +46,7 @@ class EngineConfig:
     max_tokens_per_step: int = 2048
     prefill_chunk: Optional[int] = None
     max_context: Optional[int] = None
+    cache_bits: Optional[int] = None
     use_graphs: bool = True
     device: str = "cuda:0"
 
@@ -61,6 +64,8 @@ class EngineConfig:
             v = getattr(self, name)
             if v is not None and (isinstance(v, bool) or not isinstance(v, int) or v < 1):
                 raise ValueError(f"{name} = {v!r}: leave it None or give a whole number of at least 1")
+        if self.cache_bits not in (None, 4):
+            raise ValueError(f"cache_bits = {self.cache_bits!r}: leave it None or give 4")
         given = [n for n in ("num_pages", "cache_tokens", "memory_fraction") if getattr(self, n) is not None]
         if len(given) > 1:
             raise ValueError(f"the pool is sized by one of num_pages, cache_tokens, memory_fraction; got {' and '.join(given)}")

@@ -63,7 +63,8 @@ class InferenceConfig:
     ``max_length``), ``top_k``, ``top_p``, ``temperature`` (defaults of requests that bring no sampling
     parameters of their own), ``metrics``.  This engine's own: ``page_size``; the pool as one of ``num_pages``,
     ``cache_tokens`` or ``memory_fraction`` (default: ``max_batch_size * max_length`` tokens);
-    ``max_tokens_per_step``; ``prefill_chunk``; ``seed`` (of the draws); ``use_graphs``.
+    ``max_tokens_per_step``; ``prefill_chunk``; ``seed`` (of the draws); ``use_graphs``; ``cache_bits`` (4: keys and
+    values held in 4 bits).
     """
 
     def __init__(self, max_batch_size: int = 1, max_length_of_generated_sequences: int = 1024,
@@ -71,7 +72,8 @@ class InferenceConfig:
                  metrics: bool = False, attention_backend: Optional[str] = None, use_paged_kv_caching: bool = True,
                  page_size: int = 64, num_pages: Optional[int] = None, cache_tokens: Optional[int] = None,
                  memory_fraction: Optional[float] = None, max_tokens_per_step: int = 2048,
-                 prefill_chunk: Optional[int] = None, seed: int = 1234, use_graphs: bool = True):
+                 prefill_chunk: Optional[int] = None, seed: int = 1234, use_graphs: bool = True,
+                 cache_bits: Optional[int] = None):
         if attention_backend not in (None, "paged"):
             raise ValueError(f"InferenceConfig: attention_backend {attention_backend!r} selects nothing here; the engine "
                              "has one attention path, its own paged kernels (leave the option out or pass 'paged')")
@@ -86,7 +88,7 @@ class InferenceConfig:
         self.metrics = metrics
         self.page_size, self.num_pages, self.cache_tokens, self.memory_fraction = page_size, num_pages, cache_tokens, memory_fraction
         self.max_tokens_per_step, self.prefill_chunk = max_tokens_per_step, prefill_chunk
-        self.seed, self.use_graphs = seed, use_graphs
+        self.seed, self.use_graphs, self.cache_bits = seed, use_graphs, cache_bits
         self.default_sampling()          # validates the three sampling numbers
         self.engine_config("bf16")       # validates the rest
 
@@ -102,9 +104,10 @@ class InferenceConfig:
             pool["cache_tokens"] = self.max_batch_size * self.max_length
         return EngineConfig(dtype=precision, page_size=self.page_size, max_slots=self.max_batch_size,
                             max_tokens_per_step=self.max_tokens_per_step, prefill_chunk=self.prefill_chunk,
-                            max_context=max_context or self.max_length, use_graphs=self.use_graphs, device=device, **pool)
+                            max_context=max_context or self.max_length, use_graphs=self.use_graphs, cache_bits=self.cache_bits,
+                            device=device, **pool)
 
     def __repr__(self) -> str:
         shown = ("max_batch_size", "max_length", "top_k", "top_p", "temperature", "page_size", "num_pages", "cache_tokens",
-                 "memory_fraction", "max_tokens_per_step", "prefill_chunk", "seed", "use_graphs")
+                 "memory_fraction", "max_tokens_per_step", "prefill_chunk", "seed", "use_graphs", "cache_bits")
         return "InferenceConfig(" + ", ".join(f"{k}={getattr(self, k)!r}" for k in shown) + ")"

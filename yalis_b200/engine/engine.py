@@ -47,7 +47,7 @@ from yalis_b200.weights.loader import init_random, load_weights
 
 DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32, "fp32": torch.float32}
 _ENGINE_OPTIONS = ("dtype", "page_size", "num_pages", "cache_tokens", "memory_fraction", "max_slots",
-                   "max_tokens_per_step", "prefill_chunk", "max_context", "use_graphs", "device")
+                   "max_tokens_per_step", "prefill_chunk", "max_context", "cache_bits", "use_graphs", "device")
 
 
 class OutOfPages(RuntimeError):
@@ -162,13 +162,14 @@ class Engine:
         requests = self.model.cache_requests()
         cache_of = self.model.cache_sources()
         element = 2 if self.dtype == torch.bfloat16 else 4
-        page_bytes = sum(group_page_bytes(requests, cache_of, self.page_size, element).values())
+        page_bytes = sum(group_page_bytes(requests, cache_of, self.page_size, element, ec.cache_bits).values())
         free_bytes = torch.cuda.mem_get_info(self.device)[0] if ec.memory_fraction is not None else None
         self.num_pages = ec.pool_pages(self.spec.max_position, free_bytes, page_bytes or None) if page_bytes else 1
         self.groups = plan_groups(requests, self.page_size, self.num_pages, self.max_context, self.max_slots,
                                   ec.max_tokens_per_step)
         self.manager = CacheManager(self.max_slots, self.groups)
-        self.storage = CacheStorage(requests, cache_of, self.groups, self.max_slots, self.device, self.dtype)
+        self.storage = CacheStorage(requests, cache_of, self.groups, self.max_slots, self.device, self.dtype, ec.cache_bits)
+        self.model.set_cache_bits(ec.cache_bits)
         self._slot_of: Dict[Hashable, int] = {}
         self._error_word = _lib.error_word(self.device)
         # per slot the token chosen last; then the slot that is nobody's (padding); then a copy of the error word

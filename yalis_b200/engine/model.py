@@ -107,6 +107,13 @@ class Model:
         """For each item of ``cache_requests``: the index of the item whose cache it reads instead of its own."""
         return [e.cache_of for e in self.spec.schedule] + ([None] if self.entry is not None else [])
 
+    def set_cache_bits(self, bits: Optional[int]) -> None:
+        """Tells the mixers that take packed caches how the engine holds theirs (what a step launches depends on it)."""
+        for block in self.blocks:
+            for part in block.parts.values():
+                if hasattr(part, "cache_bits"):
+                    part.cache_bits = bits
+
     def capture_key(self, host):
         """The keys of all parts that run in a step, or ``NOT_CAPTURABLE`` if one of them cannot be recorded."""
         keys = []

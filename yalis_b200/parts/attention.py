@@ -20,7 +20,8 @@ from yalis_b200.config.spec import PartSpec
 from yalis_b200.ops import attention as attn_ops
 from yalis_b200.ops.linear import linear_partial
 from yalis_b200.ops.elementwise import qkv_prepare
-from .base import NOT_ROTARY, Mixer, NormedSum, PagedKV, PagedKVCache, ParamSpec, PositionEncoding, Projected, register_part
+from yalis_b200.ops.packed import packed_attention
+from .base import NOT_ROTARY, Mixer, NormedSum, PackedKVCache, PagedKV, PagedKVCache, ParamSpec, PositionEncoding, Projected, register_part
 
 
 class PagedAttention(Mixer):
@@ -44,6 +45,7 @@ class PagedAttention(Mixer):
             raise ValueError("paged_attention needs a position part (use kind 'none' for no encoding)")
         self.w_qkv: Optional[torch.Tensor] = None
         self.w_o: Optional[torch.Tensor] = None
+        self.cache_bits: Optional[int] = None          # how the engine holds the cache (it says so)
 
     def param_specs(self) -> Dict[str, ParamSpec]:
         return {
@@ -58,11 +60,13 @@ class PagedAttention(Mixer):
         self.w_o = tensors["o_proj"].contiguous()
 
     def cache_request(self) -> PagedKV:
-        return PagedKV(self.g, self.hs, self.window)
+        return PagedKV(self.g, self.hs, self.window, packable=True)
 
     def capture_key(self, host):
         # everything the choice of kernel and its launch depend on besides the shapes of the step's tensors
         per = self.nh // self.g
+        if self.cache_bits is not None:
+            return ("packed", host.max_q_len, 0 if host.max_q_len == 1 else self._packed_reach(host))
         if host.max_q_len == 1:
             return host.once(("decode_step_kind",), lambda: attn_ops.decode_step_kind([b + 1 for b in host.ctx_before]))
         return host.once(("portion_step_kind", per, self.g, self.hs),
@@ -74,8 +78,20 @@ class PagedAttention(Mixer):
             else q_len * ctx_before + q_len * (q_len + 1) / 2
         return 4.0 * self.nh * self.hs * keys
 
+    @staticmethod
+    def _packed_reach(host) -> int:
+        """How far the step's rows see, rounded up: recorded steps of the same rounded reach launch the same."""
+        return -(-host.max_kv_len // 512) * 512
+
     def forward(self, x: torch.Tensor, ctx, cache: PagedKVCache) -> torch.Tensor:
         qkv = linear_partial(x, self.w_qkv)          # [N, width], or float32 partial sums [S, N, width]
+        if isinstance(cache, PackedKVCache):
+            rows = self.position.encode_and_store(qkv, self.nh, self.g, self.hs, ctx, cache, dtype=x.dtype)
+            single = ctx.host.max_q_len == 1           # (a recorded step's lengths change; its portions' reach is in its key)
+            y = packed_attention(rows, cache.pages, ctx.positions, ctx.q_start, ctx.block_tables[cache.group], ctx.host.max_q_len, self.nh,
+                                 scale=self.scale, window=self.window, max_kv_len=None if single else self._packed_reach(ctx.host),
+                                 error_flag=ctx.error_flag)
+            return linear_partial(y, self.w_o)
         if (attn_ops.USE_FUSED_ROPE and ctx.n_requests * self.g <= 2 * attn_ops.sm_count(x.device)
                 and attn_ops.decode_tma_applicable(x.dtype, ctx, self.hs, cache.k.shape[2], self.nh // self.g, self.window)
                 and not attn_ops.decode_lean_preferred(ctx.n_requests, self.g, self.hs, attn_ops.step_kind(ctx)[0])):

@@ -82,6 +82,7 @@ class PagedKV:
     window: Optional[int] = None
     v_head_dim: Optional[int] = None      # head size of the values when it is not the keys'
     pool: int = 1                         # tokens that one entry stands for
+    packable: bool = False                # the mixer also takes keys and values held in 4 bits (``PackedKVCache``)
 
     @property
     def value_dim(self) -> int:
@@ -121,6 +122,18 @@ class PagedKVCache:
     @property
     def page_size(self) -> int:
         return self.k.shape[2]
+
+
+class PackedKVCache:
+    """What a paged mixer that said ``packable`` gets when the engine holds its cache in 4 bits: ``pages``
+    (``ops.packed.PackedPages``) in place of two pools; otherwise as ``PagedKVCache``."""
+
+    def __init__(self, pages, group: str, writable: bool = True):
+        self.pages, self.group, self.writable = pages, group, writable
+
+    @property
+    def page_size(self) -> int:
+        return self.pages.page_size
 
 
 class SlotStateCache:

@@ -14,8 +14,9 @@ from typing import Optional
 import torch
 
 from yalis_b200.config.spec import PartSpec
-from yalis_b200.ops.elementwise import rope_kv_write
-from .base import PagedKVCache, PositionEncoding, register_part
+from yalis_b200.ops.elementwise import rope_kv_write, rotate_heads
+from yalis_b200.ops.packed import packed_kv_write
+from .base import PackedKVCache, PagedKVCache, PositionEncoding, register_part
 
 
 def inverse_frequencies(head_dim: int, theta: float, scaling: Optional[dict], exact_powers: bool = False) -> torch.Tensor:
@@ -57,6 +58,19 @@ def yarn_frequencies(dims: int, theta: float, factor: float, original: float, fa
         ramp = min(max((i - lo) / max(hi - lo, 0.001), 0.0), 1.0)
         out.append(f / factor * ramp + f * (1.0 - ramp))
     return torch.tensor(out, dtype=torch.float64).float(), 0.1 * math.log(factor) + 1.0
+
+
+def _store_packed(qkv, inv_freq, num_heads, num_kv_heads, head_dim, ctx, cache: PackedKVCache, dtype):
+    """``encode_and_store`` for a cache held in 4 bits: queries and keys are rotated together, keys and values packed from the
+    rows in the model dtype.  The result's first heads * head_dim columns are the queries."""
+    heads = num_heads + num_kv_heads if cache.writable else num_heads
+    rows = rotate_heads(qkv, ctx.positions, ctx.req_of_token, inv_freq, 0, heads, head_dim, out_dtype=dtype)
+    if cache.writable:
+        values = qkv[:, heads * head_dim:] if qkv.dim() == 2 else rotate_heads(qkv, ctx.positions, ctx.req_of_token, None, heads, num_kv_heads,
+                                                                             head_dim, out_dtype=dtype)
+        packed_kv_write(rows[:, num_heads * head_dim:], values, cache.pages, ctx.positions, ctx.req_of_token, ctx.block_tables[cache.group],
+                        error_flag=ctx.error_flag)
+    return rows
 
 
 class RotaryEncoding(PositionEncoding):
@@ -104,6 +118,8 @@ class RotaryEncoding(PositionEncoding):
         if self.inv_freq is None or self.inv_freq.device != qkv.device:
             self.to(qkv.device)
         store = cache.writable
+        if isinstance(cache, PackedKVCache):
+            return _store_packed(qkv, self.inv_freq, num_heads, num_kv_heads, head_dim, ctx, cache, dtype)
         return rope_kv_write(qkv, ctx.positions, ctx.req_of_token, self.inv_freq, cache.k if store else None,
                              cache.v if store else None, ctx.block_tables[cache.group], num_heads, num_kv_heads,
                              head_dim, out_dtype=dtype, bad_flag=ctx.error_flag)
@@ -135,6 +151,8 @@ class NoPositionEncoding(PositionEncoding):
 
     def encode_and_store(self, qkv, num_heads, num_kv_heads, head_dim, ctx, cache: PagedKVCache, dtype=None):
         store = cache.writable
+        if isinstance(cache, PackedKVCache):
+            return _store_packed(qkv, None, num_heads, num_kv_heads, head_dim, ctx, cache, dtype)
         return rope_kv_write(qkv, ctx.positions, ctx.req_of_token, None, cache.k if store else None,
                              cache.v if store else None, ctx.block_tables[cache.group], num_heads, num_kv_heads,
                              head_dim, out_dtype=dtype, bad_flag=ctx.error_flag)

@@ -222,71 +222,106 @@ int launch_rows(const RowParams<T>& p, int n_tokens, cudaStream_t stream) {
 
 // The visible rows of requests' caches into bfloat16 pools of one call, for kernels that read such pools: pages of kUnpackPage
 // keys, request after request (page r * width + i holds keys i * kUnpackPage ... of request r), with the block table that says so
-// and the counters of the kernels behind it at zero.  Exact: every value is a bfloat16 number.  A block takes a page of one KV
-// head, a thread eight codes at a time.  Bound by the writes (512 B a token and KV head at 128), most of which the reader finds
-// in the L2.
-constexpr int kUnpackPage = 64;
+// and the counters of the kernels behind it at zero.  Exact: every value is a bfloat16 number.
+// An item is a page of one KV head; a resident grid walks the items that some request needs, which every block counts for itself
+// from the step's lengths (a block for every page that a request could have took 75 us of 64 requests, one of them a portion of
+// 4,033 tokens behind 3,967 and the others single tokens behind 8,000 that need none; now 12).  A thread takes eight codes of a row at
+// a time.  Bound by the writes (512 B a token and KV head at 128), most of which the reader finds in the L2: 16,384 tokens, 8 KV heads
+// of 128, 85 MB: 19 us; of 64: 15 us; 2,048 tokens of 64: 5.6 us (six or eight blocks an SM in place of four: 3 to 14 % slower).
+constexpr int kUnpackPage = 64, kUnpackThreads = 256;
 
 struct UnpackParams {
   __nv_bfloat16* k_out;        // [R * width, g, kUnpackPage, dim]
   __nv_bfloat16* v_out;
   int32_t* table_out;          // [R, width]
-  int32_t* zeroed;             // [n_zeroed] counters (no more than the launch has threads)
-  long long n_zeroed;
+  int32_t* zeroed;             // [n_zeroed] counters
+  int n_zeroed;
   const int32_t* positions;
   const int32_t* q_start;      // [R + 1]
   const int32_t* block_table;
-  int table_width, width, window, skip_single;
+  int table_width, n_requests, width, window, skip_single;
   int32_t* error;
   PackedPages pages;
 };
 
-__global__ void __launch_bounds__(256) packed_unpack_kernel(const UnpackParams p) {
+__global__ void __launch_bounds__(kUnpackThreads, 4) packed_unpack_kernel(const UnpackParams p) {
+  __shared__ int start[kUnpackThreads + 1], first_key[kUnpackThreads], last_key[kUnpackThreads], warp_sum[kUnpackThreads / 32];
   pdl_launch_dependents();
   pdl_wait();
-  const int index = blockIdx.x, kvh = blockIdx.y, req = blockIdx.z, words = p.pages.dim / 8;
-  if (threadIdx.x == 0) {
-    if (kvh == 0) p.table_out[(size_t)req * p.width + index] = req * p.width + index;
-  }
-  const long long thread = (((long long)req * p.pages.g + kvh) * p.width + index) * 256 + threadIdx.x;
-  if (thread < p.n_zeroed) p.zeroed[thread] = 0;
-  const int t0 = p.q_start[req], n = p.q_start[req + 1] - t0;
-  if (n <= 0 || (p.skip_single && n == 1)) return;
-  const int last = p.positions[t0 + n - 1], begin = p.positions[t0], key0 = index * kUnpackPage;
-  const int first = p.window > 0 ? max(0, begin - p.window + 1) : 0;
-  if (key0 > last || key0 + kUnpackPage <= first) return;
-  const size_t to = (((size_t)req * p.width + index) * p.pages.g + kvh) * kUnpackPage;
-  // A thread has the same word of codes of every 256 / words-th row: four rows' look-ups and loads are under way at a time.
-  const int rows = min(kUnpackPage, last - key0 + 1), w = threadIdx.x % words, per_round = 256 / words;
-  if ((int)threadIdx.x >= per_round * words) return;
-  for (int r0 = threadIdx.x / words; r0 < rows; r0 += 4 * per_round) {
-    long long at[4];
-    uint32_t word[4], kc[4], vc[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = r0 + i * per_round, key = key0 + r;
-      at[i] = -1;
-      if (r >= rows) continue;
-      int row;
-      const int page = page_of(p.pages, p.block_table + (size_t)req * p.table_width, p.table_width, key, row);
-      if (page >= 0) at[i] = (long long)row_index(p.pages, page, kvh, row);
-      else if (key >= first && w == 0 && p.error) atomicOr(p.error, YALIS_FLAG_BAD_PAGE);
+  const int tid = threadIdx.x, lane = tid & 31, words = p.pages.dim / 8;
+  const long long thread = (long long)blockIdx.x * kUnpackThreads + tid, threads = (long long)gridDim.x * kUnpackThreads;
+  for (long long i = thread; i < p.n_zeroed; i += threads) p.zeroed[i] = 0;
+  for (long long i = thread; i < (long long)p.n_requests * p.width; i += threads) p.table_out[i] = (int32_t)i;
+  // A thread has the same word of codes of every per_round-th row: four rows' look-ups and loads are under way at a time.
+  const int w = tid % words, own = tid / words, per_round = kUnpackThreads / words;
+  int item = blockIdx.x;                                      // counted from the first item of these requests
+  for (int r0 = 0; r0 < p.n_requests; r0 += kUnpackThreads) {
+    int pages = 0;
+    if (r0 + tid < p.n_requests) {
+      const int t0 = p.q_start[r0 + tid], n = p.q_start[r0 + tid + 1] - t0;
+      if (n > 1 || (n == 1 && !p.skip_single)) {
+        const int last = min(p.positions[t0 + n - 1], p.width * kUnpackPage - 1);
+        const int first = p.window > 0 ? max(0, p.positions[t0] - p.window + 1) : 0;
+        first_key[tid] = first;
+        last_key[tid] = last;
+        if (last >= first) pages = last / kUnpackPage - first / kUnpackPage + 1;
+      }
     }
+    int sum = pages * p.pages.g;                              // a running sum over the requests
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      word[i] = kc[i] = vc[i] = 0u;                           // (a key without a page: zeros)
-      if (at[i] < 0) continue;
-      word[i] = p.pages.words[at[i]];
-      kc[i] = p.pages.k[at[i] * words + w];
-      vc[i] = p.pages.v[at[i] * words + w];
+    for (int d = 1; d < 32; d <<= 1) {
+      const int before = __shfl_up_sync(0xFFFFFFFFu, sum, d);
+      if (lane >= d) sum += before;
     }
+    if (lane == 31) warp_sum[tid >> 5] = sum;
+    __syncthreads();
+    for (int i = 0; i < tid >> 5; ++i) sum += warp_sum[i];
+    start[tid + 1] = sum;
+    if (tid == 0) start[0] = 0;
+    __syncthreads();
+    const int total = start[kUnpackThreads];
+    for (; item < total; item += gridDim.x) {
+      int i = 0;                                              // the request: the last that starts at or before the item
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = r0 + i * per_round;
-      if (r >= rows) break;
-      reinterpret_cast<uint4*>(p.k_out)[(to + r) * words + w] = unpack_bf16(kc[i], word[i] & 0xFFFFu);
-      reinterpret_cast<uint4*>(p.v_out)[(to + r) * words + w] = unpack_bf16(vc[i], word[i] >> 16);
+      for (int d = kUnpackThreads / 2; d > 0; d >>= 1)
+        if (start[i + d] <= item) i += d;
+      const int req = r0 + i, local = item - start[i], first = first_key[i], last = last_key[i];
+      const int index = first / kUnpackPage + local / p.pages.g, kvh = local % p.pages.g, key0 = index * kUnpackPage;
+      const size_t to = (((size_t)req * p.width + index) * p.pages.g + kvh) * kUnpackPage;
+      const int32_t* table_row = p.block_table + (size_t)req * p.table_width;
+      const int rows = own < per_round ? min(kUnpackPage, last - key0 + 1) : 0;
+      for (int q = own; q < rows; q += 4 * per_round) {
+        long long at[4];
+        uint32_t word[4], kc[4], vc[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = q + j * per_round, key = key0 + r;
+          at[j] = -1;
+          if (r >= rows) continue;
+          int row;
+          const int page = page_of(p.pages, table_row, p.table_width, key, row);
+          if (page >= 0) at[j] = (long long)row_index(p.pages, page, kvh, row);
+          else if (key >= first && w == 0 && p.error) atomicOr(p.error, YALIS_FLAG_BAD_PAGE);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          word[j] = kc[j] = vc[j] = 0u;                       // (a key without a page: zeros)
+          if (at[j] < 0) continue;
+          word[j] = p.pages.words[at[j]];
+          kc[j] = p.pages.k[at[j] * words + w];
+          vc[j] = p.pages.v[at[j] * words + w];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = q + j * per_round;
+          if (r >= rows) break;
+          reinterpret_cast<uint4*>(p.k_out)[(to + r) * words + w] = unpack_bf16(kc[j], word[j] & 0xFFFFu);
+          reinterpret_cast<uint4*>(p.v_out)[(to + r) * words + w] = unpack_bf16(vc[j], word[j] >> 16);
+        }
+      }
     }
+    item -= total;
+    __syncthreads();                                          // (the requests' arrays are written again)
   }
 }
 
@@ -315,14 +350,14 @@ YALIS_API int yalis_packed_unpack(void* k_codes, void* v_codes, void* words, int
                                   const int32_t* q_start, const int32_t* block_table, int table_width, int n_requests, int width, int window,
                                   int skip_single, void* k_out, void* v_out, int32_t* table_out, int32_t* zeroed, int n_zeroed, int32_t* error,
                                   cudaStream_t stream) {
-  if (dim < 8 || dim > 256 || dim % 8 || page_size < 1 || g < 1 || g > 65535 || n_requests > 65535 || width < 1) return YALIS_ERR_SHAPE;
+  if (dim < 8 || dim > 256 || dim % 8 || page_size < 1 || g < 1 || width < 1) return YALIS_ERR_SHAPE;
   if (n_requests <= 0) return YALIS_OK;
-  if (n_zeroed > (long long)width * g * n_requests * 256) return YALIS_ERR_SHAPE;
   UnpackParams p = {};
   p.n_zeroed = n_zeroed;
   p.k_out = static_cast<__nv_bfloat16*>(k_out); p.v_out = static_cast<__nv_bfloat16*>(v_out); p.table_out = table_out; p.zeroed = zeroed;
-  p.positions = positions; p.q_start = q_start; p.block_table = block_table; p.table_width = table_width; p.width = width;
-  p.window = window; p.skip_single = skip_single; p.error = error;
+  p.positions = positions; p.q_start = q_start; p.block_table = block_table; p.table_width = table_width; p.n_requests = n_requests;
+  p.width = width; p.window = window; p.skip_single = skip_single; p.error = error;
   p.pages = packed_pages(k_codes, v_codes, words, num_pages, page_size, g, dim);
-  return yalis_launch(packed_unpack_kernel, dim3(width, g, n_requests), dim3(256), 0, stream, p);
+  const long long most = (long long)width * g * n_requests, resident = 4LL * yalis_sm_count();
+  return yalis_launch(packed_unpack_kernel, dim3((unsigned)(most < resident ? most : resident)), dim3(kUnpackThreads), 0, stream, p);
 }

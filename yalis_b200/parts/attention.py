@@ -66,7 +66,7 @@ class PagedAttention(Mixer):
         # everything the choice of kernel and its launch depend on besides the shapes of the step's tensors
         per = self.nh // self.g
         if self.cache_bits is not None:
-            return ("packed", host.max_q_len, 0 if host.max_q_len == 1 else self._packed_reach(host))
+            return ("packed", 0 if host.max_q_len == 1 else self._packed_reach(host))
         if host.max_q_len == 1:
             return host.once(("decode_step_kind",), lambda: attn_ops.decode_step_kind([b + 1 for b in host.ctx_before]))
         return host.once(("portion_step_kind", per, self.g, self.hs),
@@ -80,8 +80,9 @@ class PagedAttention(Mixer):
 
     @staticmethod
     def _packed_reach(host) -> int:
-        """How far the step's rows see, rounded up: recorded steps of the same rounded reach launch the same."""
-        return -(-host.max_kv_len // 512) * 512
+        """How far the step's rows see, rounded up to a power of two (from 512 on): recorded steps of the same rounded reach launch
+        the same, and there are few of them."""
+        return max(512, 1 << (host.max_kv_len - 1).bit_length())
 
     def forward(self, x: torch.Tensor, ctx, cache: PagedKVCache) -> torch.Tensor:
         qkv = linear_partial(x, self.w_qkv)          # [N, width], or float32 partial sums [S, N, width]

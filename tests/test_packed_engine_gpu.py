@@ -77,3 +77,26 @@ def test_caches_that_cannot_be_packed_are_refused():
     from yalis_b200.engine.engine import Engine
     with pytest.raises(ValueError, match="4 bits"):
         Engine(config=preset("vepivik-tiny-A"), cache_bits=4, max_slots=2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("parts, n, hs", [(1, 5, 64), (3, 5, 20), (1, 200, 64), (2, 200, 18), (2, 130, 128)])
+def test_rotate_heads_gives_the_bits_of_the_cache_write(dtype, parts, n, hs):
+    from yalis_b200.ops.elementwise import rope_kv_write, rotate_heads
+    dev, nh, g, page = "cuda:0", 6, 2, 16
+    gen = torch.Generator().manual_seed(hs + n)
+    qkv = torch.randn(parts, n, (nh + 2 * g) * hs, generator=gen)
+    qkv = qkv.to(dev) if parts > 1 else qkv[0].to(dev, dtype)
+    positions = torch.arange(n, dtype=torch.int32, device=dev)
+    reqs = torch.zeros(n, dtype=torch.int32, device=dev)
+    reqs[-1] = -1
+    inv = torch.rand(hs // 2, generator=gen).to(dev)
+    pages = -(-n // page)
+    k_pool, v_pool = (torch.zeros(pages, g, page, hs, dtype=dtype, device=dev) for _ in range(2))
+    table = torch.arange(pages, dtype=torch.int32, device=dev)[None]
+    q = rope_kv_write(qkv, positions, reqs, inv, k_pool, v_pool, table, nh, g, hs, out_dtype=dtype)
+    rows = rotate_heads(qkv, positions, reqs, inv, nh + 2 * g, hs, turned=nh + g, out_dtype=dtype)
+    k, v = (p.permute(0, 2, 1, 3).reshape(-1, g * hs)[:n - 1] for p in (k_pool, v_pool))
+    assert torch.equal(rows[:-1], torch.cat([q[:-1], k, v], 1))
+    some = rotate_heads(qkv, positions, reqs, None, nh, hs, out_dtype=dtype)
+    assert torch.equal(some[:-1], (qkv.sum(0) if parts > 1 and parts < 3 else qkv[0] + qkv[1] + qkv[2] if parts == 3 else qkv)[:-1, :nh * hs].to(dtype))

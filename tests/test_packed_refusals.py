@@ -65,3 +65,12 @@ def test_options_of_a_packed_cache():
     request = PagedKV(8, 128, packable=True)
     assert group_page_bytes([request], [None], 64, 2, 4) == {"kv_all": 8 * 64 * (128 + 4)}
     assert group_page_bytes([request], [None], 64, 2) == {"kv_all": 8 * 64 * 512}
+
+
+def test_rotate_heads_refuses_cpu_tensors():
+    import torch
+    from yalis_b200.ops._lib import KernelError
+    from yalis_b200.ops.elementwise import rotate_heads
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(KernelError):
+        rotate_heads(torch.zeros(2, 64), i, i, None, 2, 16)

@@ -698,7 +698,7 @@ __global__ void rope_kv_write_kernel(const TS* src, int src_stride, int n_parts,
                                      const int32_t* req_of_token, const float* __restrict__ inv_freq,
                                      T* k_pool, T* v_pool,
                                      const int32_t* block_table, int table_width, int page_size,
-                                     int num_pages, int nh, int g, int hs, int32_t* bad_page) {
+                                     int num_pages, int nh, int g, int hs, int turned, int32_t* bad_page) {
   pdl_launch_dependents();
   pdl_wait();
   const int t = blockIdx.x, head = blockIdx.y;   // head: [0, nh) Q, [nh, nh+g) K, [nh+g, nh+2g) V
@@ -726,7 +726,7 @@ __global__ void rope_kv_write_kernel(const TS* src, int src_stride, int n_parts,
     const float x1 = sum_parts<TS>(row + i, n_parts, part_stride);
     const float x2 = sum_parts<TS>(row + i + half, n_parts, part_stride);
     float o1 = x1, o2 = x2;
-    if (!is_v && inv_freq) {
+    if (head < turned && inv_freq) {
       float sn, cs;
       sincosf((float)pos * inv_freq[i], &sn, &cs);
       rotate_pair(x1, x2, cs, sn, o1, o2);
@@ -745,7 +745,7 @@ __global__ void rope_kv_write_token_kernel(const TS* src, int src_stride, int n_
                                            const float* __restrict__ inv_freq, T* k_pool,
                                            T* v_pool, const int32_t* block_table,
                                            int table_width, int page_size, int num_pages, int nh, int g, int hs,
-                                           int32_t* bad_page) {
+                                           int turned, int32_t* bad_page) {
   extern __shared__ float cs[];   // cos[hs/2], sin[hs/2]
   pdl_launch_dependents();
   pdl_wait();
@@ -790,7 +790,7 @@ __global__ void rope_kv_write_token_kernel(const TS* src, int src_stride, int n_
     const float x1 = sum_parts<TS>(h + i, n_parts, part_stride);
     const float x2 = sum_parts<TS>(h + i + half, n_parts, part_stride);
     float o1 = x1, o2 = x2;
-    if (!is_v && inv_freq) {
+    if (head < turned && inv_freq) {
       const float c = cs[i], sn = cs[half + i];
       rotate_pair(x1, x2, c, sn, o1, o2);
     }
@@ -808,7 +808,7 @@ __global__ void rope_kv_write_token_vec_kernel(const TS* src, int src_stride, in
                                                const float* __restrict__ inv_freq, T* k_pool,
                                                T* v_pool, const int32_t* block_table,
                                                int table_width, int page_size, int num_pages, int nh, int g, int hs,
-                                               int32_t* bad_page) {
+                                               int turned, int32_t* bad_page) {
   extern __shared__ __align__(16) float cs[];   // cos[hs/2], sin[hs/2]
   pdl_launch_dependents();
   pdl_wait();
@@ -858,7 +858,7 @@ __global__ void rope_kv_write_token_vec_kernel(const TS* src, int src_stride, in
       x2.x += b.x; x2.y += b.y; x2.z += b.z; x2.w += b.w;
     }
     float4 o1 = x1, o2 = x2;
-    if (!is_v && inv_freq) {
+    if (head < turned && inv_freq) {
       const float4 c = *reinterpret_cast<const float4*>(cs + i), sn = *reinterpret_cast<const float4*>(cs + half + i);
       rotate_pair(x1.x, x2.x, c.x, sn.x, o1.x, o2.x);
       rotate_pair(x1.y, x2.y, c.y, sn.y, o1.y, o2.y);
@@ -870,12 +870,14 @@ __global__ void rope_kv_write_token_vec_kernel(const TS* src, int src_stride, in
   }
 }
 
-// src_dtype: the model type (n_parts must be 1) or YALIS_F32 partial sums [n_parts, N, src_stride].
-YALIS_API int yalis_rope_kv_write(const void* src, int src_dtype, int src_stride, int n_parts, long long part_stride,
-                                  void* q_out, int dtype, const int32_t* positions, const int32_t* req_of_token,
-                                  const float* inv_freq, void* k_pool, void* v_pool, const int32_t* block_table,
-                                  int table_width, int page_size, int num_pages, int nh, int g, int hs, int n_tokens,
-                                  int32_t* bad_page, cudaStream_t stream) {
+namespace {
+
+// src_dtype: the model type (n_parts must be 1) or YALIS_F32 partial sums [n_parts, N, src_stride].  Heads from `turned` on keep
+// their angle.
+int rope_kv_write(const void* src, int src_dtype, int src_stride, int n_parts, long long part_stride, void* q_out, int dtype,
+                  const int32_t* positions, const int32_t* req_of_token, const float* inv_freq, void* k_pool, void* v_pool,
+                  const int32_t* block_table, int table_width, int page_size, int num_pages, int nh, int g, int hs, int turned,
+                  int n_tokens, int32_t* bad_page, cudaStream_t stream) {
   if (n_tokens <= 0) return YALIS_OK;
   if (hs <= 0 || (hs & 1) || n_parts < 1) return YALIS_ERR_SHAPE;
   if (nh + 2 * g > 65535) return YALIS_ERR_SHAPE;
@@ -888,7 +890,7 @@ YALIS_API int yalis_rope_kv_write(const void* src, int src_dtype, int src_stride
   const bool vec_ok = hs % 8 == 0 && src_stride % 4 == 0 && part_stride % 4 == 0 && (ptrs & 15) == 0;
 #define YALIS_ROPE_ARGS(TS_)                                                                                         \
   (const TS_*)src, src_stride, n_parts, (size_t)part_stride, (T*)q_out, positions, req_of_token, inv_freq, (T*)k_pool, \
-      (T*)v_pool, block_table, table_width, page_size, num_pages, nh, g, hs, bad_page
+      (T*)v_pool, block_table, table_width, page_size, num_pages, nh, g, hs, turned, bad_page
   YALIS_DISPATCH_DTYPE(
       dtype, T,
       if (per_token && vec_ok) {
@@ -912,6 +914,26 @@ YALIS_API int yalis_rope_kv_write(const void* src, int src_dtype, int src_stride
       } else { return YALIS_ERR_DTYPE; });
 #undef YALIS_ROPE_ARGS
   return YALIS_OK;
+}
+
+}  // namespace
+
+// src_dtype: the model type (n_parts must be 1) or YALIS_F32 partial sums [n_parts, N, src_stride].
+YALIS_API int yalis_rope_kv_write(const void* src, int src_dtype, int src_stride, int n_parts, long long part_stride,
+                                  void* q_out, int dtype, const int32_t* positions, const int32_t* req_of_token,
+                                  const float* inv_freq, void* k_pool, void* v_pool, const int32_t* block_table,
+                                  int table_width, int page_size, int num_pages, int nh, int g, int hs, int n_tokens,
+                                  int32_t* bad_page, cudaStream_t stream) {
+  return rope_kv_write(src, src_dtype, src_stride, n_parts, part_stride, q_out, dtype, positions, req_of_token, inv_freq, k_pool, v_pool,
+                       block_table, table_width, page_size, num_pages, nh, g, hs, nh + g, n_tokens, bad_page, stream);
+}
+
+// The rows' first `heads` heads, the first `turned` of them rotated, as [N, heads * hs]; nothing goes to any cache.
+YALIS_API int yalis_rotate_heads(const void* src, int src_dtype, int src_stride, int n_parts, long long part_stride, void* out, int dtype,
+                                 const int32_t* positions, const int32_t* req_of_token, const float* inv_freq, int heads, int turned, int hs,
+                                 int n_tokens, cudaStream_t stream) {
+  return rope_kv_write(src, src_dtype, src_stride, n_parts, part_stride, out, dtype, positions, req_of_token, inv_freq, nullptr, nullptr,
+                       nullptr, 0, 1, 0, heads, 0, hs, turned, n_tokens, nullptr, stream);
 }
 
 // --------------------------------------------------------------------------

@@ -2,7 +2,6 @@
 
 from __future__ import annotations
 
-import ctypes
 from typing import Optional
 
 import torch
@@ -203,29 +202,28 @@ def rope_kv_write(qkv: torch.Tensor, positions: torch.Tensor, req_of_token: torc
 
 
 def rotate_heads(qkv: torch.Tensor, positions: torch.Tensor, req_of_token: torch.Tensor, inv_freq: Optional[torch.Tensor],
-                 first: int, heads: int, head_dim: int, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """Heads ``first`` ... ``first + heads - 1`` of the rows [N, width] (or float32 partial sums [S, N, width], added in order),
-    rotated by ``float(position) * inv_freq`` as ``rope_kv_write`` rotates them (None: not at all), as [N, heads * head_dim] in
-    ``out_dtype``: for caches that another kernel writes.  Tokens of no request (-1) are left out."""
+                 heads: int, head_dim: int, turned: Optional[int] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """The first ``heads`` heads of the rows [N, width] (or float32 partial sums [S, N, width], added in order) as
+    [N, heads * head_dim] in ``out_dtype``, the first ``turned`` of them (default all) rotated by ``float(position) * inv_freq`` as
+    ``rope_kv_write`` rotates them (None: not at all): for caches that another kernel writes.  Tokens of no request (-1) are left out."""
     name = "rotate_heads"
     need_cuda(name, qkv, positions, req_of_token, inv_freq)
-    need(qkv.is_contiguous() and qkv.dim() in (2, 3) and 0 <= first and 1 <= heads and (first + heads) * head_dim <= qkv.shape[-1], name,
-         "qkv must be contiguous [N, >= (first + heads) * head_dim] or [S, N, ...]")
+    need(qkv.is_contiguous() and qkv.dim() in (2, 3) and heads >= 1 and heads * head_dim <= qkv.shape[-1], name,
+         "qkv must be contiguous [N, >= heads * head_dim] or [S, N, ...]")
     need(qkv.dim() == 2 or qkv.dtype == torch.float32, name, "split partial sums must be float32")
     parts, (n, width) = qkv.shape[0] if qkv.dim() == 3 else 1, qkv.shape[-2:]
-    out_dtype = out_dtype or qkv.dtype
+    out_dtype, turned = out_dtype or qkv.dtype, heads if turned is None else turned
     need(qkv.dim() == 3 or qkv.dtype == out_dtype, name, "an unsplit qkv must have the output dtype")
-    need(head_dim % 2 == 0, name, f"head_dim {head_dim} must be even")
+    need(head_dim % 2 == 0 and 0 <= turned <= heads, name, f"head_dim {head_dim} must be even, and turned {turned} between 0 and heads")
     for t in (positions, req_of_token):
         need(t.dtype == torch.int32 and t.shape == (n,) and t.is_contiguous(), name, "positions/req_of_token: int32 [N]")
     if inv_freq is not None:
         need(inv_freq.dtype == torch.float32 and inv_freq.shape == (head_dim // 2,) and inv_freq.is_contiguous(), name,
              "inv_freq must be float32 [head_dim / 2]")
     out = torch.empty((n, heads * head_dim), dtype=out_dtype, device=qkv.device)
-    at = ctypes.c_void_p(qkv.data_ptr() + first * head_dim * qkv.element_size())
-    check(lib().yalis_rope_kv_write(at, i32(dtype_code(qkv.dtype)), i32(width), i32(parts), i64(n * width), ptr(out), i32(dtype_code(out_dtype)),
-                                    ptr(positions), ptr(req_of_token), ptr(inv_freq), ptr(None), ptr(None), ptr(None), i32(0), i32(1), i32(0),
-                                    i32(heads), i32(0), i32(head_dim), i32(n), ptr(None), stream()), name)
+    check(lib().yalis_rotate_heads(ptr(qkv), i32(dtype_code(qkv.dtype)), i32(width), i32(parts), i64(n * width), ptr(out), i32(dtype_code(out_dtype)),
+                                   ptr(positions), ptr(req_of_token), ptr(inv_freq), i32(heads), i32(turned),
+                                   i32(head_dim), i32(n), stream()), name)
     return out
 
 

@@ -63,13 +63,13 @@ def yarn_frequencies(dims: int, theta: float, factor: float, original: float, fa
 def _store_packed(qkv, inv_freq, num_heads, num_kv_heads, head_dim, ctx, cache: PackedKVCache, dtype):
     """``encode_and_store`` for a cache held in 4 bits: queries and keys are rotated together, keys and values packed from the
     rows in the model dtype.  The result's first heads * head_dim columns are the queries."""
-    heads = num_heads + num_kv_heads if cache.writable else num_heads
-    rows = rotate_heads(qkv, ctx.positions, ctx.req_of_token, inv_freq, 0, heads, head_dim, out_dtype=dtype)
+    turned = num_heads + num_kv_heads if cache.writable else num_heads
+    heads = turned + num_kv_heads if cache.writable and qkv.dim() == 3 else turned     # (partial sums: the values are added up with them)
+    rows = rotate_heads(qkv, ctx.positions, ctx.req_of_token, inv_freq, heads, head_dim, turned=turned, out_dtype=dtype)
     if cache.writable:
-        values = qkv[:, heads * head_dim:] if qkv.dim() == 2 else rotate_heads(qkv, ctx.positions, ctx.req_of_token, None, heads, num_kv_heads,
-                                                                             head_dim, out_dtype=dtype)
-        packed_kv_write(rows[:, num_heads * head_dim:], values, cache.pages, ctx.positions, ctx.req_of_token, ctx.block_tables[cache.group],
-                        error_flag=ctx.error_flag)
+        values = (rows if heads > turned else qkv)[:, turned * head_dim:(turned + num_kv_heads) * head_dim]
+        packed_kv_write(rows[:, num_heads * head_dim:turned * head_dim], values, cache.pages, ctx.positions, ctx.req_of_token,
+                        ctx.block_tables[cache.group], error_flag=ctx.error_flag)
     return rows
 
 

@@ -83,8 +83,8 @@ def attention(cache, q, q_start, positions, heads, window=None, scale=None):
     """float64: out [N, heads * dim], the sum of weights per pool place, and per output the sum of P |v| and, per row and head, the
     largest score error that float32 products of the codes can make (31 times the step times the sum of |q|, a rounding an
     element).  The sum of P |v| of bfloat16 queries has 2^8 times this on top, which half a step of bfloat16 turns into what weights
-    too small for float16 can lose: they are held as multiples of 2^-24 at least, at a scale at which the largest step of the
-    request's values is 64 to 128; half of that, 2^-25 / 64 of the largest step, times |code - zero| <= 15 for every key seen."""
+    too small for float16 can lose: weights times steps are held as multiples of 2^-24 at least, at a scale at which the row's largest
+    is 2^6 or more (where values' steps are 2^-80 or more); half of that, 2^-31 of the largest, times |code - zero| <= 15 for every key seen."""
     n, dim, g = q.shape[0], cache.dim, cache.g
     scale = 1 / math.sqrt(dim) if scale is None else scale
     out, size = torch.zeros(n, heads, dim).double(), torch.zeros(n, heads, dim).double()
@@ -99,15 +99,14 @@ def attention(cache, q, q_start, positions, heads, window=None, scale=None):
             at, row = cache.table[r, j // cache.page].long(), j % cache.page
             k, v = values(cache.k[at, :, row], cache.words[at, :, row, 0]), values(cache.v[at, :, row], cache.words[at, :, row, 1])
             k_step = step_zero(cache.words[at, :, row, 0])[0]
-            everything = torch.arange(int(positions[q_start[r + 1] - 1]) + 1)
-            v_step = step_zero(cache.words[cache.table[r, everything // cache.page].long(), :, everything % cache.page, 1])[0].nan_to_num(0)
+            v_step = step_zero(cache.words[at, :, row, 1])[0].nan_to_num(0)
             for h in range(heads):
                 kv = h // (heads // g)
                 x = q[t].double()[h * dim:(h + 1) * dim]
                 p = torch.softmax(k[:, kv] @ x * scale, 0)
                 out[t, h], size[t, h] = p @ v[:, kv], p @ v[:, kv].abs()
                 if q.dtype == torch.bfloat16:
-                    size[t, h] += 2.0 ** 8 * 15 * len(j) * 2.0 ** -31 * v_step[:, kv].max()
+                    size[t, h] += 2.0 ** 8 * 15 * len(j) * 2.0 ** -31 * (p * v_step[:, kv]).max().nan_to_num(0)
                 slack[t, h] = (dim + 16) * 2.0 ** -24 * 31 * k_step[:, kv].max() * x.abs().sum() * abs(scale)
                 sums[at, kv, row] += p
                 sum_slack[at, kv, row] += p * (2 * slack[t, h] + (len(j) + 32) * 2.0 ** -24)

@@ -227,6 +227,24 @@ def test_a_row_without_numbers_is_seen_only_by_those_that_see_it(dim):
             assert not bool(got[0, :9].isnan().any())                  # positions 10 .. 18
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim,n,window", [(64, 1, None), (128, 1, 40), (128, 5, None), (64, 9, 33), (24, 4, 20), (64, 40, None)])
+def test_values_of_another_size_that_have_no_weight(dtype, dim, n, window):
+    """Values 2^100 times as large as the others', at places that a row does not see (behind its window, after it, behind the last)
+    or gives no weight, take nothing from its accuracy."""
+    c = Cache([70 + n, 90 + n], 2, dim, 16, seed=dim + n)
+    large = lambda r, j: c.words[int(c.table[r, j // 16]), :, j % 16, 1].copy_(torch.tensor(2.0 ** 100).bfloat16().view(torch.int16) | 7)
+    q, pos, q_start = step_of(c, [n, n], dtype=dtype, heads=4)
+    if n > 1:
+        large(1, 90 + n - 1)                               # the last row's own place: its value is seen by nobody else
+    if window is not None:
+        large(0, 70 - window)                              # just behind the first row's window
+    else:                                                  # a key of scores about 140 or -140: all of a row's weight or none
+        c.words[int(c.table[0, 4]), :, 69 % 16, 0] = 0x4180
+        large(0, 69)
+    check_attention(c, q, pos, q_start, 4, window=window, sums=False)
+
+
 def test_attention_without_a_page():
     from yalis_b200.ops.packed import packed_attention
     for dim, n in ((64, 1), (128, 1), (24, 1), (64, 20)):

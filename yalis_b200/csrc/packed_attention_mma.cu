@@ -11,8 +11,9 @@
 // eight codes, (w >> s) & 0x00780078 | 0x41804180 is the pair 16 + c_i, 16 + c_(i + 4) in bfloat16.  For values 16 + zero is taken
 // away from the pairs (exact); for keys (16 + zero) sum(q) is taken away from the product, which is two instructions a score in
 // place of 64 a chunk (with float32 queries the pairs lose it too: the difference of two large sums would show).  With bfloat16 queries
-// values and weights meet in float16: two of a half word's codes then need no shift, and a weight keeps eleven bits; the values' steps
-// go in relative to the largest so far.  Elements of a V row pair up by key instead: the 16-bit halves of two keys' words are put side by side first.  The
+// values and weights meet in float16: two of a half word's codes then need no shift, and a weight keeps eleven bits; every column's
+// exponentials are then taken relative to its largest weight times step so far instead of its largest weight, so that a key that a column
+// does not see, or gives no weight, has no say in how its others are rounded.  Elements of a V row pair up by key instead: the 16-bit halves of two keys' words are put side by side first.  The
 // scores' accumulators, times step, are the softmax's scores; the weights times the values' steps are rounded to float16
 // (float32: to three bfloat16 parts) and turned from accumulator layout to operand layout by movmatrix.
 //
@@ -35,6 +36,8 @@ constexpr int kStages = 2;
 constexpr float kNone = -1e30f;  // the maximum of no scores
 constexpr float kUnset = -3e38f; // limit of a column that has seen no score yet: any will do
 constexpr float kLazy = 8.f;   // how far (log2) scores may rise above the maximum in use before the output is rescaled
+constexpr float kTarget = 6.f; // where (log2) the largest weight times its value's step lies in float16 after that: below 2^15 with kLazy more
+constexpr float kSmall = -80.f;  // steps of less (log2) count as this, which keeps the weights themselves within float32
 
 struct MmaParams {
   const void* q;               // [N, q_stride]
@@ -196,7 +199,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
   extern __shared__ __align__(128) unsigned char smem[];
   Stage<DIM>* ring = reinterpret_cast<Stage<DIM>*>(smem) + (threadIdx.x >> 5) * kStages;
   float4* terms = reinterpret_cast<float4*>(smem + sizeof(Stage<DIM>) * kStages * kWarps) + (threadIdx.x >> 5) * kChunk;
-  float4* merge_o = reinterpret_cast<float4*>(smem + sizeof(Stage<DIM>) * kStages * kWarps + kWarps * kChunk * 16);   // [kWarps][NT * MT][32]
+  float* height = reinterpret_cast<float*>(smem + sizeof(Stage<DIM>) * kStages * kWarps + kWarps * kChunk * 16) + (threadIdx.x >> 5) * kChunk;
+  float4* merge_o = reinterpret_cast<float4*>(smem + sizeof(Stage<DIM>) * kStages * kWarps + kWarps * kChunk * 20);   // [kWarps][NT * MT][32]
   float* merge_ml = reinterpret_cast<float*>(merge_o + kWarps * NT * MT * 32);                     // [kWarps][COLS][2]
   int* s_last = reinterpret_cast<int*>(merge_ml + kWarps * COLS * 2);
   int* s_deal = s_last + 1;                                                                        // pieces, blocks
@@ -335,10 +339,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       any_lo = min(any_lo, __shfl_xor_sync(0xffffffffu, any_lo, o));
     }
 
-    // Scores are taken relative to base; one above limit moves it.
+    // Scores are taken relative to base; one above limit (HALF: with the value's step, both in powers of two) moves it.
     float base[NT][2], limit[NT][2], l[NT][2], acc[NT][MT][4];
-    uint32_t v_top = 0u;                         // HALF: no step up to this needs another scale
-    float v_scale = 1.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       base[nt][0] = base[nt][1] = l[nt][0] = l[nt][1] = 0.f;
@@ -460,23 +462,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       const Stage<DIM>& st = ring[stage];
       const int key0 = first_key + c * kChunk;
       float4 own = terms_of(st.words[lane], p.scale_log2);
-      // HALF: the values' steps relative to the largest so far, as 64 to 128, so that weights stay below 2^15 (kLazy) and are whole
-      // to eleven bits down to 2^-14.
       if constexpr (HALF) {
-        const uint32_t largest = __reduce_max_sync(0xffffffffu, own.z == own.z ? __float_as_uint(own.z) : 0u);
-        if (__any_sync(0xffffffffu, largest > v_top)) {      // (the vote says that the whole warp goes one way)
-          const float fewer = v_scale;
-          v_top = largest | 0x007FFFFFu;
-          v_scale = __uint_as_float(0x82000000u - max(largest & 0x7F800000u, 0x04000000u));       // 2^(6 - e) for a step of 2^e and more
-          const float less = v_scale / fewer;    // (powers of two; nothing to rescale the first time)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) acc[nt][i][j] *= less;
-        }
-        own.z *= v_scale;
+        height[lane] = fmaxf((float)((int)(__float_as_uint(own.z) >> 23) - 127), kSmall);        // log2 of the value's step
         // 16 + zero / 64 and 16 + zero / 4 in float16
         own.w = __uint_as_float(0x4C004C00u | (st.words[lane] >> 16 & 15u) * 0x00100001u);
       }
@@ -486,10 +473,15 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       // ---- products with 32 keys ----
       float sc[NT][2][4];
       float4 term[2][2];
+      float rise[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         term[half][0] = terms[own_key + half * 16];
         term[half][1] = terms[own_key + half * 16 + 8];
+        if constexpr (HALF) {
+          rise[half][0] = height[own_key + half * 16];
+          rise[half][1] = height[own_key + half * 16 + 8];
+        }
         uint32_t wa[W], wb[W];
         const unsigned char* from = st.k + k_own + half * 16 * (DIM / 2);
         if constexpr (DIM == 128) {
@@ -547,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                   const int j = half * 16 + own_key + 8 * e;
-                  if (!MASK || key0 + j <= see_hi[nt][x])
+                  if ((!MASK || key0 + j <= see_hi[nt][x]) && key0 + j < p.score_stride)
                     to[j] = MASK && term[half][e].x == 0.f ? -INFINITY : term[half][e].x * sc[nt][half][2 * e + x];
                 }
             }
@@ -567,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
                 const int key = key0 + half * 16 + own_key + 8 * (i >> 1);
                 if (!(key <= see_hi[nt][i & 1] && key >= see_lo[nt][i & 1] && term[half][i >> 1].x != 0.f)) v = -INFINITY;
               }
-              most[nt][i & 1] = fmaxf(most[nt][i & 1], v);
+              most[nt][i & 1] = fmaxf(most[nt][i & 1], HALF ? v + rise[half][i >> 1] : v);
             }
         bool grow = false;
 #pragma unroll
@@ -581,11 +573,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
               float top = most[nt][x];
 #pragma unroll
               for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-              float up = fmaxf(top, 0.f);
+              constexpr float kTo = HALF ? kTarget : 0.f;
+              float up = fmaxf(top - kTo, 0.f);
               keep[x] = exp2_fast(-up);
               if (limit[nt][x] == kUnset) {        // nothing summed yet: the first maximum, wherever it lies
-                up = top == -INFINITY ? 0.f : top;
-                limit[nt][x] = top == -INFINITY ? kUnset : kLazy;
+                up = top == -INFINITY ? 0.f : top - kTo;
+                limit[nt][x] = top == -INFINITY ? kUnset : kTo + kLazy;
                 keep[x] = 1.f;
               }
               base[nt][x] += up;
@@ -705,16 +698,24 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (at >= end) pdl_launch_dependents();      // this block's last tile is there
 
-    if constexpr (HALF) {                        // codes were taken by 64 and by 4 too small, weights by the scale
-      const float even = 64.f / v_scale, odd = 4.f / v_scale;
+    if constexpr (HALF) {                        // codes were taken by 64 and by 4 too small
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          acc[nt][i][0] *= even; acc[nt][i][1] *= even;
-          acc[nt][i][2] *= odd; acc[nt][i][3] *= odd;
+          acc[nt][i][0] *= 64.f; acc[nt][i][1] *= 64.f;
+          acc[nt][i][2] *= 4.f; acc[nt][i][3] *= 4.f;
         }
     }
+    // A sum of weights on a base `by` higher.  HALF: bases may lie further apart than float32's powers of two, by the values' steps.
+    auto moved = [](float sum, float by) {
+      if constexpr (HALF) {
+        const float half = exp2f(0.5f * by);
+        return sum * half * half;
+      } else {
+        return sum * exp2f(by);
+      }
+    };
     // ---- the four warps' results together ----
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -754,8 +755,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
 #pragma unroll
         for (int k = 0; k < kWarps; ++k) {
           const float f0 = exp2f(ml[k][0].x - top[nt][0]), f1 = exp2f(ml[k][1].x - top[nt][1]);
-          norm[nt][0] += ml[k][0].y * f0;
-          norm[nt][1] += ml[k][1].y * f1;
+          norm[nt][0] += moved(ml[k][0].y, ml[k][0].x - top[nt][0]);
+          norm[nt][1] += moved(ml[k][1].y, ml[k][1].x - top[nt][1]);
 #pragma unroll
           for (int i = 0; i < OWN; ++i) {
             const float4 v = merge_o[(k * NT * MT + nt * MT + warp * OWN + i) * 32 + lane];
@@ -814,8 +815,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
               const float next = fmaxf(base[nt][x], ml.x);
               was[x] = exp2f(base[nt][x] - next);
               is[x] = exp2f(ml.x - next);
+              l[nt][x] = moved(l[nt][x], base[nt][x] - next) + moved(ml.y, ml.x - next);
               base[nt][x] = next;
-              l[nt][x] = l[nt][x] * was[x] + ml.y * is[x];
             }
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
@@ -856,7 +857,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
 template <typename T, int DIM, int NT, int PARTS, bool SCORES>
 int launch_mma_as(const MmaParams& p, int grid, cudaStream_t stream) {
   constexpr int MT = DIM / 16;
-  const size_t smem = sizeof(Stage<DIM>) * kStages * kWarps + kWarps * kChunk * 16 + (size_t)kWarps * NT * MT * 512 + (size_t)kWarps * 8 * NT * 8 + 16 +
+  const size_t smem = sizeof(Stage<DIM>) * kStages * kWarps + kWarps * kChunk * 20 + (size_t)kWarps * NT * MT * 512 + (size_t)kWarps * 8 * NT * 8 + 16 +
                       (size_t)(p.n_requests + 1) * 12;
   auto* kernel = packed_attention_mma_kernel<T, DIM, NT, PARTS, SCORES>;
   static int configured[64] = {0};

@@ -245,6 +245,25 @@ def test_values_of_another_size_that_have_no_weight(dtype, dim, n, window):
     check_attention(c, q, pos, q_start, 4, window=window, sums=False)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim,n", [(64, 1), (128, 7), (24, 3), (64, 70)])
+def test_scales_and_windows_at_their_limits(dtype, dim, n):
+    c = Cache([n, 90 + n], 2, dim, 16, seed=n)
+    q, pos, q_start = step_of(c, [n, n], dtype=dtype, heads=4)
+    for scale in (0.0, 1e-38, -0.2):                       # no weight differs from another; scales whose products with a step underflow
+        check_attention(c, q, pos, q_start, 4, scale=scale)
+    for window in (1, 2 ** 31 - 1, 2 ** 32 + 5):
+        check_attention(c, q, pos, q_start, 4, window=window)
+
+
+@pytest.mark.parametrize("dtype,n", [(torch.float32, 20), (torch.float32, 1), (torch.bfloat16, 1), (torch.bfloat16, 40)])
+def test_a_table_for_many_more_tokens_than_there_are(dtype, n):
+    c = Cache([30 + n, 90 + n], 2, 64, 64, seed=n)
+    c.table = torch.cat([c.table, torch.full((2, 70000), -1, dtype=torch.int32)], 1)
+    q, pos, q_start = step_of(c, [n, n], dtype=dtype, heads=4)
+    check_attention(c, q, pos, q_start, 4)
+
+
 def test_attention_without_a_page():
     from yalis_b200.ops.packed import packed_attention
     for dim, n in ((64, 1), (128, 1), (24, 1), (64, 20)):

@@ -157,7 +157,7 @@ struct Stage {
 };
 
 // What a key's word says, as the products use it: the key's step times scale, 16 + its zero, the value's step, 16 + its zero.
-// A key that is not there has steps of 0 (a row that is there has at least 2^-126).
+// A key that is not there has a value's step of 0 (a row that is there has at least 2^-126; times scale it may be 0).
 __device__ __forceinline__ float4 terms_of(uint32_t word, float scale_log2) {
   return make_float4(step_of(word & 0xFFFFu) * scale_log2, __uint_as_float(0x41800000u | (word & 15u) << 19), step_of(word >> 16),
                      __uint_as_float(0x41800000u | (word >> 16 & 15u) << 19));
@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
                 for (int e = 0; e < 2; ++e) {
                   const int j = half * 16 + own_key + 8 * e;
                   if ((!MASK || key0 + j <= see_hi[nt][x]) && key0 + j < p.score_stride)
-                    to[j] = MASK && term[half][e].x == 0.f ? -INFINITY : term[half][e].x * sc[nt][half][2 * e + x];
+                    to[j] = MASK && term[half][e].z == 0.f ? -INFINITY : term[half][e].x * sc[nt][half][2 * e + x];
                 }
             }
         }
@@ -557,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
               v = fmaf(term[half][i >> 1].x, v, -base[nt][i & 1]);
               if constexpr (MASK) {
                 const int key = key0 + half * 16 + own_key + 8 * (i >> 1);
-                if (!(key <= see_hi[nt][i & 1] && key >= see_lo[nt][i & 1] && term[half][i >> 1].x != 0.f)) v = -INFINITY;
+                if (!(key <= see_hi[nt][i & 1] && key >= see_lo[nt][i & 1] && term[half][i >> 1].z != 0.f)) v = -INFINITY;
               }
               most[nt][i & 1] = fmaxf(most[nt][i & 1], HALF ? v + rise[half][i >> 1] : v);
             }

@@ -249,7 +249,7 @@ packed_sums_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
           const bool masked = n_tok < p.tokens_per_tile || it.begin + t < key_lo + 31 ||
                               (p.window > 0 && it.begin + t + n_tok - 1 - p.window >= key_lo);
           // Row c sees this lane's key if lowest <= token < beyond.
-          const int lowest = key - it.begin - t, beyond = min(n_tok, p.window > 0 ? lowest + p.window : 0x3fffffff);
+          const int lowest = key - it.begin - t, beyond = p.window > 0 ? (int)min((long long)n_tok, (long long)lowest + p.window) : n_tok;
           auto add = [&](const float (&s)[32], int c0) {
             const float4* lse4 = reinterpret_cast<const float4*>(&lse_s[warp][c0]);
             if (masked) {

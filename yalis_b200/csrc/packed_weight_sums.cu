@@ -64,8 +64,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_weight_sums_kernel(const S
   __shared__ int last_s[COLUMNS];
   __shared__ float sum_s[CG > 1 ? CG : 1][CG > 1 ? KG * kKeys : 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int kvh = blockIdx.x, req = blockIdx.y, kg = warp / CG, cg = warp % CG;
-  const int block0 = blockIdx.z * KG * kKeys, key0 = block0 + kg * kKeys;
+  const int kvh = blockIdx.x % p.pages.g, req = blockIdx.y, kg = warp / CG, cg = warp % CG;
+  const int block0 = blockIdx.x / p.pages.g * (KG * kKeys), key0 = block0 + kg * kKeys;
   pdl_launch_dependents();
   pdl_wait();
   const int tok0 = p.q_start[req], n = p.q_start[req + 1] - tok0;
@@ -244,8 +244,9 @@ __global__ void __launch_bounds__(kThreads, 1) packed_weight_sums_kernel(const S
 
 template <typename T, int DIM, int PARTS>
 int launch_sums(const SumsParams& p, int n_requests, int max_kv_len, cudaStream_t stream) {
-  const dim3 grid(p.pages.g, n_requests, (max_kv_len + 2 * kKeys - 1) / (2 * kKeys));
-  if (grid.y > 65535 || grid.z > 65535) return YALIS_ERR_SHAPE;
+  const long long blocks = (max_kv_len + 2LL * kKeys - 1) / (2 * kKeys) * p.pages.g;
+  if (n_requests > 65535 || blocks > 0x7fffffff) return YALIS_ERR_SHAPE;
+  const dim3 grid((unsigned)blocks, n_requests);
   return yalis_launch(packed_weight_sums_kernel<T, DIM, PARTS, 2, 4, 64 / (PARTS == 1 ? 1 : 2)>, grid, dim3(kThreads), 0, stream, p);
 }
 
@@ -257,7 +258,7 @@ __global__ void __launch_bounds__(256) packed_sums_of_scores_kernel(const SumsPa
   const int tok0 = p.q_start[req], n = p.q_start[req + 1] - tok0;
   if (n <= 0 || (p.only_single && n > 1)) return;
   const int last = p.positions[tok0 + n - 1], begin = p.positions[tok0];
-  if (key > last || (p.window > 0 && key <= begin - p.window)) return;
+  if (key >= stride || key > last || (p.window > 0 && key <= begin - p.window)) return;
   int row;
   const int page = page_of(p.pages, p.block_table + (size_t)req * p.table_width, p.table_width, key, row);
   if (page < 0) return;
@@ -321,6 +322,6 @@ YALIS_API int yalis_packed_sums_of_scores(float* scores, long long score_stride,
   if (n_requests <= 0 || max_kv_len <= 0) return YALIS_OK;
   const SumsParams p = params_of(nullptr, 0, num_pages, page_size, g, dim, positions, q_start, block_table, table_width, nh, 1.f, window, only_single,
                                  lse2, sums);
-  return yalis_launch(packed_sums_of_scores_kernel, dim3((max_kv_len + 255) / 256, g, n_requests), dim3(256), 0, stream, p, (const float*)scores,
+  return yalis_launch(packed_sums_of_scores_kernel, dim3((unsigned)((max_kv_len + 255LL) / 256), g, n_requests), dim3(256), 0, stream, p, (const float*)scores,
                       score_stride);
 }

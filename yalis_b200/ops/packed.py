@@ -196,6 +196,7 @@ def packed_kv_read(pages: PackedPages, positions: torch.Tensor, req_of_token: to
     return both.unbind(0)
 
 
+_LONGEST = (1 << 31) - 1   # places are 32-bit numbers
 UNPACK_ROWS = 64          # query rows of a pair (tokens * heads of a KV head) beyond which portions are unpacked for the prompt kernel
 UNPACK_PAGE = 64          # keys of a page of the unpacked pools
 UNPACK_BYTES = 2 << 30    # of unpacked keys and values at a time
@@ -286,7 +287,9 @@ def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tenso
         scale = dim ** -0.5
     elif not math.isfinite(scale):
         raise KernelError(f"{name}: the scale must be finite")
-    r, reach, window, flag = q_start.shape[0] - 1, columns * page_size, window or 0, _flag_address(name, error_flag)
+    r, reach, flag = q_start.shape[0] - 1, min(columns * page_size, _LONGEST), _flag_address(name, error_flag)
+    if window is None or window >= reach:
+        window = 0                                      # (every place that the table has)
     max_kv_len = reach if max_kv_len is None or max_kv_len > reach else int(max_kv_len)
     lse2 = scores = None
     if weight_sums is not None:

@@ -306,7 +306,8 @@ def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tenso
     mma = (dim == 64 or dim == 128) and r <= 4096
     unpack = (max_q_len * per > UNPACK_ROWS and code == BF16 and (dim == 64 or dim == 128) and per <= 128 and scale > 0 and aligned
               and (out_at | out_step * 2) % 16 == 0)
-    single = unpack and mma and n > max_q_len          # single tokens may stand beside the portions: a kernel of their own
+    # Single tokens beside the portions get a kernel of their own where there may be any: with one, the others have all rows but it.
+    single = unpack and mma and max_q_len < n <= (r - 1) * max_q_len + 1
     if unpack:
         _attend_unpacked(name, device, (q_at, step, out_at, out_step), held, at, n, max_q_len, max_kv_len, num_heads, scale, window, single, lse2,
                          weight_sums, flag, raw)

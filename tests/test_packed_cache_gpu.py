@@ -106,6 +106,14 @@ def test_rows_without_a_page():
 
 # ---- attention ------------------------------------------------------------------------------------------------------
 
+@pytest.fixture(params=["by the rule", "always unpacked"])
+def portions_by_both(request, monkeypatch):
+    """Portions by whichever way the step's sizes choose, and by the prompt kernel wherever they have more rows than 64."""
+    from yalis_b200.ops import packed
+    if request.param == "always unpacked":
+        monkeypatch.setattr(packed, "UNPACK_FEW", 0)
+
+
 def step_of(cache, brought, seed=0, dtype=torch.bfloat16, heads=4, empty=()):
     """Rows of the requests' last ``brought`` tokens (0: a request that brings none)."""
     gen = torch.Generator().manual_seed(seed)
@@ -165,6 +173,7 @@ def test_single_tokens(dtype, heads, g, dim):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("heads,g,dim", LAYOUTS)
+@pytest.mark.usefixtures("portions_by_both")
 def test_portions(dtype, heads, g, dim):
     for page, window in ((16, None), (64, 20)):
         c = Cache([1, 5, 40, 130], g, dim, page, seed=page)
@@ -175,6 +184,7 @@ def test_portions(dtype, heads, g, dim):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("heads,g,dim,page", [(4, 1, 128, 64), (8, 2, 64, 16)])
 @pytest.mark.parametrize("window", [None, 50])
+@pytest.mark.usefixtures("portions_by_both")
 def test_whole_prompts_beside_single_tokens(dtype, heads, g, dim, page, window):
     c = Cache([200, 1, 333, 64, 65], g, dim, page, seed=3)
     q, pos, q_start = step_of(c, [200, 1, 1, 64, 1], dtype=dtype, heads=heads)
@@ -191,6 +201,7 @@ def test_one_long_request_and_many_short(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.usefixtures("portions_by_both")
 def test_rows_that_see_nothing(dtype):
     c = Cache([40, 3, 20], 2, 64, 16)
     q, pos, q_start = step_of(c, [1, 1, 1], dtype=dtype, heads=4, empty=(1,))
@@ -202,6 +213,7 @@ def test_rows_that_see_nothing(dtype):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("dim", [64, 128, 24])
+@pytest.mark.usefixtures("portions_by_both")
 def test_large_scores_and_rows_of_one_value(dtype, dim):
     c = Cache([150, 70], 1, dim, 16, seed=6)
     q, pos, q_start = step_of(c, [1, 4], dtype=dtype, heads=4)
@@ -213,6 +225,7 @@ def test_large_scores_and_rows_of_one_value(dtype, dim):
 
 
 @pytest.mark.parametrize("dim", [64, 24])
+@pytest.mark.usefixtures("portions_by_both")
 def test_a_row_without_numbers_is_seen_only_by_those_that_see_it(dim):
     from yalis_b200.ops.packed import packed_attention
     c = Cache([40, 40], 2, dim, 16)
@@ -229,6 +242,7 @@ def test_a_row_without_numbers_is_seen_only_by_those_that_see_it(dim):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("dim,n,window", [(64, 1, None), (128, 1, 40), (128, 5, None), (64, 9, 33), (24, 4, 20), (64, 40, None)])
+@pytest.mark.usefixtures("portions_by_both")
 def test_values_of_another_size_that_have_no_weight(dtype, dim, n, window):
     """Values 2^100 times as large as the others', at places that a row does not see (behind its window, after it, behind the last)
     or gives no weight, take nothing from its accuracy."""
@@ -247,6 +261,7 @@ def test_values_of_another_size_that_have_no_weight(dtype, dim, n, window):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("dim,n", [(64, 1), (128, 7), (24, 3), (64, 70)])
+@pytest.mark.usefixtures("portions_by_both")
 def test_scales_and_windows_at_their_limits(dtype, dim, n):
     c = Cache([n, 90 + n], 2, dim, 16, seed=n)
     q, pos, q_start = step_of(c, [n, n], dtype=dtype, heads=4)
@@ -257,6 +272,7 @@ def test_scales_and_windows_at_their_limits(dtype, dim, n):
 
 
 @pytest.mark.parametrize("dtype,n", [(torch.float32, 20), (torch.float32, 1), (torch.bfloat16, 1), (torch.bfloat16, 40)])
+@pytest.mark.usefixtures("portions_by_both")
 def test_a_table_for_many_more_tokens_than_there_are(dtype, n):
     c = Cache([30 + n, 90 + n], 2, 64, 64, seed=n)
     c.table = torch.cat([c.table, torch.full((2, 70000), -1, dtype=torch.int32)], 1)
@@ -264,6 +280,7 @@ def test_a_table_for_many_more_tokens_than_there_are(dtype, n):
     check_attention(c, q, pos, q_start, 4)
 
 
+@pytest.mark.usefixtures("portions_by_both")
 def test_attention_without_a_page():
     from yalis_b200.ops.packed import packed_attention
     for dim, n in ((64, 1), (128, 1), (24, 1), (64, 20)):
@@ -311,6 +328,7 @@ def test_a_replayed_step_follows_its_inputs():
         torch.testing.assert_close(sums.cpu().double(), 6 * a, rtol=1e-4, atol=1e-6)
 
 
+@pytest.mark.usefixtures("portions_by_both")
 def test_the_same_step_gives_the_same_bits():
     from yalis_b200.ops.packed import packed_attention
     c = Cache([1500, 7, 64, 800], 2, 64, 16, seed=9)
@@ -402,6 +420,7 @@ def test_eviction_without_a_page():
 # ---- together -------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.usefixtures("portions_by_both")
 def test_a_request_through_all_of_them(dtype):
     """A prompt in two portions, tokens one by one with their weights counted, the cache cut, and tokens behind the cut: as one
     attention over the same rows in 64 bits."""

@@ -39,10 +39,12 @@ def test_greedy_generation_equals_plain_float32(plain_packed, which, lengths, ne
     assert all(eng.engine.manager.free_pages(g.name) == g.num_pages for g in eng.engine.groups)
 
 
-@pytest.mark.parametrize("which", ["C", "D"])
-def test_bfloat16_recorded_steps_are_the_launched_ones(which):
+@pytest.mark.parametrize("which, few", [("C", None), ("C", 0), ("D", 0)])
+def test_bfloat16_recorded_steps_are_the_launched_ones(which, few, monkeypatch):
     """Decode steps replayed from recordings, prompts long enough for the unpacked form: the same tokens as launch by launch, and
     a cache of little more than a quarter of the bytes."""
+    if few is not None:
+        monkeypatch.setattr("yalis_b200.ops.packed.UNPACK_FEW", few)
     d = tiny_model_dir(which, 0.02)
     cfg = plain.read_config(d)
     prompts = prompts_for(cfg, [5, 90, 33, 64])
@@ -58,8 +60,11 @@ def test_bfloat16_recorded_steps_are_the_launched_ones(which):
     assert small * 2 * head * 2 == whole * (head + 4)
 
 
-def test_bfloat16_follows_the_oracle(plain_packed):
+@pytest.mark.parametrize("few", [None, 0])
+def test_bfloat16_follows_the_oracle(plain_packed, few, monkeypatch):
     """Every generated token is the oracle's best or within rounding of it."""
+    if few is not None:
+        monkeypatch.setattr("yalis_b200.ops.packed.UNPACK_FEW", few)
     d = tiny_model_dir("C", 0.02)
     cfg, w = plain.read_config(d), plain.read_weights(d)
     prompts = prompts_for(cfg, [5, 100, 33])

@@ -197,6 +197,6 @@ YALIS_API int yalis_packed_weight_sums_general(const void* q, long long q_stride
     return YALIS_ERR_SHAPE;
   if (n_requests <= 0 || max_kv_len <= 0) return YALIS_OK;
   p.lse2 = lse2; p.sums = sums;
-  YALIS_DISPATCH_DTYPE(dtype, T, return yalis_launch(packed_weight_sums_general_kernel<T>, dim3((unsigned)((max_kv_len + kThreads - 1LL) / kThreads), g, n_requests),
-                                                     dim3(kThreads), 0, stream, p));
+  YALIS_DISPATCH_DTYPE(dtype, T, return yalis_launch(packed_weight_sums_general_kernel<T>, dim3((unsigned)((max_kv_len + kThreads - 1LL) / kThreads), g,
+                                                                                                  n_requests), dim3(kThreads), 0, stream, p));
 }

@@ -13,7 +13,8 @@
 // place of 64 a chunk (with float32 queries the pairs lose it too: the difference of two large sums would show).  With bfloat16 queries
 // values and weights meet in float16: two of a half word's codes then need no shift, and a weight keeps eleven bits; every column's
 // exponentials are then taken relative to its largest weight times step so far instead of its largest weight, so that a key that a column
-// does not see, or gives no weight, has no say in how its others are rounded.  Elements of a V row pair up by key instead: the 16-bit halves of two keys' words are put side by side first.  The
+// does not see, or gives no weight, has no say in how its others are rounded.  Elements of a V row pair up by key instead: the 16-bit
+// halves of two keys' words are put side by side first.  The
 // scores' accumulators, times step, are the softmax's scores; the weights times the values' steps are rounded to float16
 // (float32: to three bfloat16 parts) and turned from accumulator layout to operand layout by movmatrix.
 //
@@ -22,6 +23,8 @@
 // dealt to a fixed grid by the step's lengths (choose_deal), so that a recorded launch serves other lengths too; a pair cut between
 // blocks is added up, in the blocks' order, by whichever of them comes last (a counter per pair, left at zero).  Nothing waits for
 // another block.
+// Bound by instructions, about 500 a chunk and warp: 8 requests of 16,000 to 32,000 keys, 24 heads of 128 over 8: 63 us, 212 MB at
+// 3.4 TB/s, issue slots busy 0.56; 64 requests of 520 to 1,040, 32 heads: 24 us (the general form: 4,640 and 280).
 #include <cuda_fp16.h>
 
 #include <type_traits>

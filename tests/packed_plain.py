@@ -84,7 +84,8 @@ def attention(cache, q, q_start, positions, heads, window=None, scale=None):
     largest score error that float32 products of the codes can make (31 times the step times the sum of |q|, a rounding an
     element).  The sum of P |v| of bfloat16 queries has 2^8 times this on top, which half a step of bfloat16 turns into what weights
     too small for float16 can lose: weights times steps are held as multiples of 2^-24 at least, at a scale at which the row's largest
-    is 2^6 or more (where values' steps are 2^-80 or more); half of that, 2^-31 of the largest, times |code - zero| <= 15 for every key seen."""
+    is 2^6 or more (where values' steps are 2^-80 or more); half of that, 2^-31 of the largest, times |code - zero| <= 15 for every key seen.  And what float32 sums
+    lose when codes and zeros are multiplied out apart, sum P t c - sum P t z with each at most 15 sum P t: 300 roundings of 2^-24 of that."""
     n, dim, g = q.shape[0], cache.dim, cache.g
     scale = 1 / math.sqrt(dim) if scale is None else scale
     out, size = torch.zeros(n, heads, dim).double(), torch.zeros(n, heads, dim).double()
@@ -106,7 +107,8 @@ def attention(cache, q, q_start, positions, heads, window=None, scale=None):
                 p = torch.softmax(k[:, kv] @ x * scale, 0)
                 out[t, h], size[t, h] = p @ v[:, kv], p @ v[:, kv].abs()
                 if q.dtype == torch.bfloat16:
-                    size[t, h] += 2.0 ** 8 * 15 * len(j) * 2.0 ** -31 * (p * v_step[:, kv]).max().nan_to_num(0)
+                    weighted = (p * v_step[:, kv]).nan_to_num(0)
+                    size[t, h] += 2.0 ** 8 * 15 * (len(j) * 2.0 ** -31 * weighted.max() + 300 * 2.0 ** -24 * weighted.sum())
                 slack[t, h] = (dim + 16) * 2.0 ** -24 * 31 * k_step[:, kv].max() * x.abs().sum() * abs(scale)
                 sums[at, kv, row] += p
                 sum_slack[at, kv, row] += p * (2 * slack[t, h] + (len(j) + 32) * 2.0 ** -24)

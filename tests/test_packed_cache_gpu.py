@@ -260,6 +260,20 @@ def test_values_of_another_size_that_have_no_weight(dtype, dim, n, window):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim,n", [(64, 1), (128, 5), (64, 9)])
+def test_queries_of_other_sizes(dtype, dim, n):
+    """Heads, and elements of a head, that lie many powers of two apart; rows of zeros."""
+    c = Cache([n, 90 + n], 2, dim, 16, seed=n)
+    q, pos, q_start = step_of(c, [n, n], dtype=dtype, heads=8)
+    q = q.view(2 * n, 8, dim)
+    q *= (2.0 ** torch.tensor([0, -60, -14, 3, -110, -24, 0, 1])).to(dtype)[:, None]
+    q[:, 0, ::2] *= 2.0 ** -13
+    q[:, 3, 5] = 2.0 ** 7
+    q[0, 6] = 0
+    check_attention(c, q.view(2 * n, 8 * dim), pos, q_start, 8)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("dim,n", [(64, 1), (128, 7), (24, 3), (64, 70)])
 @pytest.mark.usefixtures("portions_by_both")
 def test_scales_and_windows_at_their_limits(dtype, dim, n):

@@ -3,28 +3,32 @@
 //
 // A pair is a KV head of a request with up to 8 NT of its query rows (row = token * heads per KV head + head), which are the columns
 // here: both products are taken transposed, so that the codes are the operand of 16 rows and a lane turns the codes it has loaded
-// into bfloat16 pairs in registers, with nothing in between:
+// into pairs of numbers in registers, with nothing in between:
 //
 //   S^T [keys, columns] = C_K [16 keys x 16 elements] q^T       O^T [elements, columns] += C_V^T [16 elements x 16 keys] W^T
 //
-// The order of a product's inner index is free as long as both operands agree, so a lane takes neighbouring codes: with a word of
-// eight codes, (w >> s) & 0x00780078 | 0x41804180 is the pair 16 + c_i, 16 + c_(i + 4) in bfloat16.  For values 16 + zero is taken
-// away from the pairs (exact); for keys (16 + zero) sum(q) is taken away from the product, which is two instructions a score in
-// place of 64 a chunk (with float32 queries the pairs lose it too: the difference of two large sums would show).  With bfloat16 queries
-// values and weights meet in float16: two of a half word's codes then need no shift, and a weight keeps eleven bits; every column's
-// exponentials are then taken relative to its largest weight times step so far instead of its largest weight, so that a key that a column
-// does not see, or gives no weight, has no say in how its others are rounded.  Elements of a V row pair up by key instead: the 16-bit
-// halves of two keys' words are put side by side first.  The
-// scores' accumulators, times step, are the softmax's scores; the weights times the values' steps are rounded to float16
-// (float32: to three bfloat16 parts) and turned from accumulator layout to operand layout by movmatrix.
+// The order of a product's inner index is free as long as both operands agree, so a lane takes neighbouring codes.
+//
+// bfloat16 queries: both products are taken in float16, where a code needs nothing but a mask.  Four bits c at the bottom of a 16-bit half
+// are the float16 number c 2^-24, the next four c 2^-20 (numbers below 2^-14 are linear in their bits), so two of a half word's four codes
+// need no shift.  Zeros are multiplied out apart: for keys zero sum(q) is taken from the product, for values the weights' product with the
+// zeros (a tile of its own) from the output, in place of 64 subtractions a chunk each.  Queries go in by a power of two that puts a row's
+// largest near the top of float16, which loses no bit of anything above 2^-28 of it; weights keep eleven bits: every column's exponentials
+// are taken relative to its largest weight times value's step so far instead of its largest weight, so that a key that a column does not
+// see, or gives no weight, has no say in how its others are rounded.
+// float32 queries: codes become bfloat16 pairs, with a word of eight codes (w >> s) & 0x00780078 | 0x41804180 is 16 + c_i, 16 + c_(i + 4),
+// less 16 + zero; queries and weights go in as three bfloat16 parts (sums of large numbers that cancel would show here).
+// Elements of a V row pair up by key: the 16-bit halves of two keys' words are put side by side first.  The scores' accumulators, times
+// step, are the softmax's scores; weights are turned from accumulator layout to operand layout by movmatrix.
 //
 // A warp takes 32 keys at a time (a chunk) through a ring of its own in shared memory, filled by 16-byte asynchronous copies, and
 // keeps a softmax and an output of its own; the four warps of a block come together at the end of a pair.  Chunks are
 // dealt to a fixed grid by the step's lengths (choose_deal), so that a recorded launch serves other lengths too; a pair cut between
 // blocks is added up, in the blocks' order, by whichever of them comes last (a counter per pair, left at zero).  Nothing waits for
 // another block.
-// Bound by instructions, about 500 a chunk and warp: 8 requests of 16,000 to 32,000 keys, 24 heads of 128 over 8: 63 us, 212 MB at
-// 3.4 TB/s, issue slots busy 0.56; 64 requests of 520 to 1,040, 32 heads: 24 us (the general form: 4,640 and 280).
+// Bound by instructions, about 490 a chunk and warp (620 and 9 % more time with shifts and subtractions for every pair): 8 requests of
+// 16,000 to 32,000 keys, 24 heads of 128 over 8: 58 us, 212 MB at 3.7 TB/s; 64 requests of 520 to 1,040, 32 heads: 23 us (the general
+// form: 4,640 and 280).
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -85,18 +89,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
 __device__ __forceinline__ uint32_t pair_f16(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ uint32_t minus_f16(uint32_t a, uint32_t b) {
-  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-// Codes of a pair in float16, where two of a 16-bit half's four need no shift: 16 + c / 64 from the lowest bits, 16 + c / 4 from the next.
-template <int SHIFT>
-__device__ __forceinline__ uint32_t code_pair_f16(uint32_t w, uint32_t sixteens) {
-  uint32_t r;
-  if constexpr (SHIFT == 0) asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(r) : "r"(w), "r"(sixteens));
-  else asm("lop3.b32 %0, %1, 0x00F000F0, %2, 0xEA;" : "=r"(r) : "r"(w), "r"(sixteens));
-  return r;
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
   uint32_t r;
@@ -159,7 +151,8 @@ struct Stage {
   uint32_t words[kChunk];
 };
 
-// What a key's word says, as the products use it: the key's step times scale, 16 + its zero, the value's step, 16 + its zero.
+// What a key's word says, as the products with bfloat16 pairs use it: the key's step times scale, 16 + its zero, the value's step, 16 +
+// its zero.
 // A key that is not there has a value's step of 0 (a row that is there has at least 2^-126; times scale it may be 0).
 __device__ __forceinline__ float4 terms_of(uint32_t word, float scale_log2) {
   return make_float4(step_of(word & 0xFFFFu) * scale_log2, __uint_as_float(0x41800000u | (word & 15u) << 19), step_of(word >> 16),
@@ -198,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
   constexpr int PIECES = DIM / 32;             // 16-byte pieces of a row
   constexpr int COPIES = PIECES;               // of K (and as many of V) that a lane asks for per chunk
   constexpr int PART_FLOATS = NT * MT * 128 + 2 * COLS;
-  constexpr bool SIGNED = PARTS > 1, HALF = PARTS == 1;        // HALF: values and weights meet in float16
+  constexpr bool HALF = PARTS == 1;            // products in float16
   extern __shared__ __align__(128) unsigned char smem[];
   Stage<DIM>* ring = reinterpret_cast<Stage<DIM>*>(smem) + (threadIdx.x >> 5) * kStages;
   float4* terms = reinterpret_cast<float4*>(smem + sizeof(Stage<DIM>) * kStages * kWarps) + (threadIdx.x >> 5) * kChunk;
@@ -218,8 +211,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
   const int k_own = DIM == 128 ? piece_at<DIM>(own_key, t) : own_key * (DIM / 2) + t * 8;
   const int v_own[2] = {DIM == 128 ? piece_at<DIM>(v_key[0], g >> 1) + (g & 1) * 8 : v_key[0] * (DIM / 2) + g * 4,
                         DIM == 128 ? piece_at<DIM>(v_key[1], g >> 1) + (g & 1) * 8 : v_key[1] * (DIM / 2) + g * 4};
-  uint32_t sixteens_f16;
-  asm volatile("mov.b32 %0, 0x4C004C00;" : "=r"(sixteens_f16));
   pdl_wait();
 
   // ---- the chunks of every request (KV heads, blocks of columns and chunks of 32 keys), their running sum, this block's share ----
@@ -342,16 +333,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       any_lo = min(any_lo, __shfl_xor_sync(0xffffffffu, any_lo, o));
     }
 
-    // Scores are taken relative to base; one above limit (HALF: with the value's step, both in powers of two) moves it.
-    float base[NT][2], limit[NT][2], l[NT][2], acc[NT][MT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      base[nt][0] = base[nt][1] = l[nt][0] = l[nt][1] = 0.f;
-      limit[nt][0] = limit[nt][1] = kUnset;
-#pragma unroll
-      for (int i = 0; i < MT; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
-    }
-
     // Chunks of this warp that any column sees: one in kWarps.
     int c = lo + warp, c_end = hi;
     if (any_hi < 0) c_end = 0;
@@ -421,39 +402,78 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
     if (c + kWarps < c_end) row = lookup(c + kWarps);
 
     // ---- queries in registers as the products' right operand, while the first copies are under way ----
+    // HALF: in float16, by a power of two (unit takes it out again) so high that a column's largest is 2^11 to 2^12: no bit is lost of
+    // anything above 2^-28 of it.  The pairs whose codes lie in the lowest bits go in sixteenfold.
     uint32_t qf[NT][2 * W][2][PARTS];
-    float q_sum[NT][2];                          // sum(q) of the columns 2t, 2t + 1
+    float q_sum[NT][2], unit[NT][2];             // sum(q) of the columns 2t, 2t + 1
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int row = column0 + nt * 8 + g;
       const bool real = row < n_rows;
       const int token = tok0 + (real ? row / p.per : 0), head = kvh * p.per + (real ? row % p.per : 0);
       const T* src = static_cast<const T*>(p.q) + (long long)token * p.q_stride + (long long)head * DIM + t * (DIM / 4);
-      float own = 0.f;
+      float x[W][8], own = 0.f, own_unit = 1.f;
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        float x[8];
         if (!real) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = 0.f;
+          for (int i = 0; i < 8; ++i) x[w][i] = 0.f;
         } else if (p.q_vector) {
           const float4 a = load4_f32(src + 8 * w), b = load4_f32(src + 8 * w + 4);
-          x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-          x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+          x[w][0] = a.x; x[w][1] = a.y; x[w][2] = a.z; x[w][3] = a.w;
+          x[w][4] = b.x; x[w][5] = b.y; x[w][6] = b.z; x[w][7] = b.w;
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(src[8 * w + i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          parts_of<PARTS>(x[i], x[i + 4], qf[nt][2 * w + (i >> 1)][i & 1]);
-          own += x[i] + x[i + 4];
+          for (int i = 0; i < 8; ++i) x[w][i] = to_f32<T>(src[8 * w + i]);
         }
       }
+      float scale = 1.f;
+      if constexpr (HALF) {
+        uint32_t most = 0u;
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[w][i]) & 0x7FFFFFFFu);
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2)) >> 23;
+        const uint32_t up = min(254u, 265u - most);
+        const bool fits = most < 246u;           // (nothing from 2^119 on is computed with)
+        scale = fits ? __uint_as_float(up << 23) : NAN;
+        own_unit = fits ? __uint_as_float((274u - up) << 23) : 1.f;             // 2^20 / scale: codes are 2^-24 and 2^-20 of their numbers
+      }
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (HALF) {
+            const float a = x[w][i] * scale, b = x[w][i + 4] * scale;
+            own += a + b;
+            qf[nt][2 * w + (i >> 1)][i & 1][0] = i & 1 ? pair_f16(a, b) : pair_f16(16.f * a, 16.f * b);
+          } else {
+            parts_of<PARTS>(x[w][i], x[w][i + 4], qf[nt][2 * w + (i >> 1)][i & 1]);
+            own += x[w][i] + x[w][i + 4];
+          }
+        }
+      }
+      if constexpr (HALF) own *= 9.5367431640625e-7f;          // 2^-20: in the products' unit
       own += __shfl_xor_sync(0xffffffffu, own, 1);
       own += __shfl_xor_sync(0xffffffffu, own, 2);             // column g, in its four lanes
 #pragma unroll
-      for (int e = 0; e < 2; ++e) q_sum[nt][e] = __shfl_sync(0xffffffffu, own, (2 * t + e) * 4);
+      for (int e = 0; e < 2; ++e) {
+        q_sum[nt][e] = __shfl_sync(0xffffffffu, own, (2 * t + e) * 4);
+        unit[nt][e] = HALF ? __shfl_sync(0xffffffffu, own_unit, (2 * t + e) * 4) : 1.f;
+      }
+    }
+
+    // Scores are taken relative to base; one above limit (HALF: with the value's step, both in powers of two) moves it.
+    float base[NT][2], limit[NT][2], l[NT][2], acc[NT][MT][4], acc_z[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      base[nt][0] = base[nt][1] = l[nt][0] = l[nt][1] = 0.f;
+      limit[nt][0] = limit[nt][1] = kUnset;
+      acc_z[nt][0] = acc_z[nt][1] = acc_z[nt][2] = acc_z[nt][3] = 0.f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
     }
 
     for (int stage = 0; c < c_end; c += kWarps, stage ^= 1) {
@@ -466,9 +486,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       const int key0 = first_key + c * kChunk;
       float4 own = terms_of(st.words[lane], p.scale_log2);
       if constexpr (HALF) {
+        own.y -= 16.f;                           // (no sixteens in the keys' codes)
         height[lane] = fmaxf((float)((int)(__float_as_uint(own.z) >> 23) - 127), kSmall);        // log2 of the value's step
-        // 16 + zero / 64 and 16 + zero / 4 in float16
-        own.w = __uint_as_float(0x4C004C00u | (st.words[lane] >> 16 & 15u) * 0x00100001u);
+        own.w = __uint_as_float(st.words[lane] >> 16 & 15u);   // the value's zero times 2^-24 in float16
       }
       terms[lane] = own;
       __syncwarp();
@@ -498,9 +518,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
         for (int nt = 0; nt < NT; ++nt) sc[nt][half][0] = sc[nt][half][1] = sc[nt][half][2] = sc[nt][half][3] = 0.f;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          uint32_t lo[4] = {code_pair<0>(wa[w], sixteens), code_pair<0>(wb[w], sixteens), code_pair<1>(wa[w], sixteens), code_pair<1>(wb[w], sixteens)};
-          uint32_t hi[4] = {code_pair<2>(wa[w], sixteens), code_pair<2>(wb[w], sixteens), code_pair<3>(wa[w], sixteens), code_pair<3>(wb[w], sixteens)};
-          if constexpr (SIGNED) {
+          uint32_t lo[4], hi[4];
+          if constexpr (HALF) {                  // as they lie: c in the lowest bits is c 2^-24 in float16, c in the next c 2^-20
+            const uint32_t wa8 = wa[w] >> 8, wb8 = wb[w] >> 8;
+            lo[0] = wa[w] & 0x000F000Fu; lo[1] = wb[w] & 0x000F000Fu; lo[2] = wa[w] & 0x00F000F0u; lo[3] = wb[w] & 0x00F000F0u;
+            hi[0] = wa8 & 0x000F000Fu; hi[1] = wb8 & 0x000F000Fu; hi[2] = wa8 & 0x00F000F0u; hi[3] = wb8 & 0x00F000F0u;
+          } else {
+            lo[0] = code_pair<0>(wa[w], sixteens); lo[1] = code_pair<0>(wb[w], sixteens); lo[2] = code_pair<1>(wa[w], sixteens); lo[3] = code_pair<1>(wb[w], sixteens);
+            hi[0] = code_pair<2>(wa[w], sixteens); hi[1] = code_pair<2>(wb[w], sixteens); hi[2] = code_pair<3>(wa[w], sixteens); hi[3] = code_pair<3>(wb[w], sixteens);
             const uint32_t za = __byte_perm(__float_as_uint(term[half][0].y), 0, 0x3232), zb = __byte_perm(__float_as_uint(term[half][1].y), 0, 0x3232);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -512,14 +537,19 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int i = PARTS - 1; i >= 0; --i) {
-              mma_bf16(sc[nt][half], lo, qf[nt][2 * w][0][i], qf[nt][2 * w][1][i]);
-              mma_bf16(sc[nt][half], hi, qf[nt][2 * w + 1][0][i], qf[nt][2 * w + 1][1][i]);
+              if constexpr (HALF) {
+                mma_f16(sc[nt][half], lo, qf[nt][2 * w][0][i], qf[nt][2 * w][1][i]);
+                mma_f16(sc[nt][half], hi, qf[nt][2 * w + 1][0][i], qf[nt][2 * w + 1][1][i]);
+              } else {
+                mma_bf16(sc[nt][half], lo, qf[nt][2 * w][0][i], qf[nt][2 * w][1][i]);
+                mma_bf16(sc[nt][half], hi, qf[nt][2 * w + 1][0][i], qf[nt][2 * w + 1][1][i]);
+              }
             }
           }
         }
       }
       // ---- softmax: scores in powers of two, less the maximum in use ----
-      if constexpr (!SIGNED) {
+      if constexpr (HALF) {
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -543,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
                 for (int e = 0; e < 2; ++e) {
                   const int j = half * 16 + own_key + 8 * e;
                   if ((!MASK || key0 + j <= see_hi[nt][x]) && key0 + j < p.score_stride)
-                    to[j] = MASK && term[half][e].z == 0.f ? -INFINITY : term[half][e].x * sc[nt][half][2 * e + x];
+                    to[j] = MASK && term[half][e].z == 0.f ? -INFINITY : term[half][e].x * unit[nt][x] * sc[nt][half][2 * e + x];
                 }
             }
         }
@@ -557,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               float& v = sc[nt][half][i];
-              v = fmaf(term[half][i >> 1].x, v, -base[nt][i & 1]);
+              v = fmaf(HALF ? term[half][i >> 1].x * unit[nt][i & 1] : term[half][i >> 1].x, v, -base[nt][i & 1]);
               if constexpr (MASK) {
                 const int key = key0 + half * 16 + own_key + 8 * (i >> 1);
                 if (!(key <= see_hi[nt][i & 1] && key >= see_lo[nt][i & 1] && term[half][i >> 1].z != 0.f)) v = -INFINITY;
@@ -596,6 +626,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
               acc[nt][i][0] *= keep[0]; acc[nt][i][1] *= keep[1];
               acc[nt][i][2] *= keep[0]; acc[nt][i][3] *= keep[1];
             }
+            acc_z[nt][0] *= keep[0]; acc_z[nt][1] *= keep[1];
+            acc_z[nt][2] *= keep[0]; acc_z[nt][3] *= keep[1];
           }
         }
 #pragma unroll
@@ -645,18 +677,18 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
           }
         }
         if constexpr (HALF) {
-          const uint32_t lo01 = __byte_perm(__float_as_uint(z[0]), __float_as_uint(z[1]), 0x5410), hi01 = __byte_perm(__float_as_uint(z[0]), __float_as_uint(z[1]), 0x7632);
-          const uint32_t lo23 = __byte_perm(__float_as_uint(z[2]), __float_as_uint(z[3]), 0x5410), hi23 = __byte_perm(__float_as_uint(z[2]), __float_as_uint(z[3]), 0x7632);
+          const uint32_t z01 = __byte_perm(__float_as_uint(z[0]), __float_as_uint(z[1]), 0x5410), z23 = __byte_perm(__float_as_uint(z[2]), __float_as_uint(z[3]), 0x5410);
+          const uint32_t zeros[4] = {z01, z01, z23, z23};      // every row of a tile of its own
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(acc_z[nt], zeros, wf[nt][half][0][0], wf[nt][half][1][0]);
 #pragma unroll
           for (int u = 0; u < U; ++u) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const uint32_t a = __byte_perm(vw[0][u], vw[1][u], h ? 0x7632 : 0x5410), b = __byte_perm(vw[2][u], vw[3][u], h ? 0x7632 : 0x5410);
               const uint32_t a8 = a >> 8, b8 = b >> 8;
-              const uint32_t f0[4] = {minus_f16(code_pair_f16<0>(a, sixteens_f16), lo01), minus_f16(code_pair_f16<4>(a, sixteens_f16), hi01),
-                                      minus_f16(code_pair_f16<0>(b, sixteens_f16), lo23), minus_f16(code_pair_f16<4>(b, sixteens_f16), hi23)};
-              const uint32_t f1[4] = {minus_f16(code_pair_f16<0>(a8, sixteens_f16), lo01), minus_f16(code_pair_f16<4>(a8, sixteens_f16), hi01),
-                                      minus_f16(code_pair_f16<0>(b8, sixteens_f16), lo23), minus_f16(code_pair_f16<4>(b8, sixteens_f16), hi23)};
+              const uint32_t f0[4] = {a & 0x000F000Fu, a & 0x00F000F0u, b & 0x000F000Fu, b & 0x00F000F0u};
+              const uint32_t f1[4] = {a8 & 0x000F000Fu, a8 & 0x00F000F0u, b8 & 0x000F000Fu, b8 & 0x00F000F0u};
               const int tile = 4 * u + 2 * h;
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
@@ -701,13 +733,15 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (at >= end) pdl_launch_dependents();      // this block's last tile is there
 
-    if constexpr (HALF) {                        // codes were taken by 64 and by 4 too small
+    if constexpr (HALF) {                        // codes and zeros were taken by 2^24 too small, those of odd elements by 2^20
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          acc[nt][i][0] *= 64.f; acc[nt][i][1] *= 64.f;
-          acc[nt][i][2] *= 4.f; acc[nt][i][3] *= 4.f;
+          acc[nt][i][0] = (acc[nt][i][0] - acc_z[nt][0]) * 16777216.f;
+          acc[nt][i][1] = (acc[nt][i][1] - acc_z[nt][1]) * 16777216.f;
+          acc[nt][i][2] = (acc[nt][i][2] - 16.f * acc_z[nt][2]) * 1048576.f;
+          acc[nt][i][3] = (acc[nt][i][3] - 16.f * acc_z[nt][3]) * 1048576.f;
         }
     }
     // A sum of weights on a base `by` higher.  HALF: bases may lie further apart than float32's powers of two, by the values' steps.

@@ -38,6 +38,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "slots.cuh"
 #include "tcgen05.cuh"
 
 namespace {
@@ -986,3 +987,5 @@ YALIS_API int yalis_prefill_attention_tcgen05_unpacked(
   return window > 0 ? launch_prefill<true>(p, q, (int)q_stride, k_pool, v_pool, n_tokens, hs, 1, stream, true)
                     : launch_prefill<false>(p, q, (int)q_stride, k_pool, v_pool, n_tokens, hs, n_splits, stream, true);
 }
+
+YALIS_SLOTS(yalis_prefill_attention_tcgen05_unpacked)

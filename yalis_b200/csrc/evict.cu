@@ -11,6 +11,7 @@
 // Bound by memory: the sums are read once, a row that moves is read and written once (32 requests of 4,160 tokens to 2,048, 8 KV heads of
 // 128 in bfloat16: 101 us, 495 MB at 4.9 TB/s; with nothing to move 27; one request of 700 tokens: 12 us).
 #include "common.cuh"
+#include "slots.cuh"
 
 namespace {
 
@@ -269,3 +270,5 @@ YALIS_API int yalis_evict_tokens(void* const* pools, const int* row_bytes, int n
   }
   return yalis_launch(evict_tokens_kernel, dim3(g, n_requests), dim3(kThreads), smem, stream, p);
 }
+
+YALIS_SLOTS(yalis_evict_tokens)

@@ -8,6 +8,7 @@
 // and sums in float32.  It takes every size; its weights' normaliser, log2(sum exp S), goes to memory for the sums, which a second
 // kernel adds key by key in the order of the rows.
 #include "packed.cuh"
+#include "slots.cuh"
 
 namespace {
 
@@ -200,3 +201,6 @@ YALIS_API int yalis_packed_weight_sums_general(const void* q, long long q_stride
   YALIS_DISPATCH_DTYPE(dtype, T, return yalis_launch(packed_weight_sums_general_kernel<T>, dim3((unsigned)((max_kv_len + kThreads - 1LL) / kThreads), g,
                                                                                                   n_requests), dim3(kThreads), 0, stream, p));
 }
+
+YALIS_SLOTS(yalis_packed_attention_general)
+YALIS_SLOTS(yalis_packed_weight_sums_general)

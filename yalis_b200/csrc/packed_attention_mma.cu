@@ -34,6 +34,7 @@
 #include <type_traits>
 
 #include "packed.cuh"
+#include "slots.cuh"
 
 namespace {
 
@@ -951,3 +952,5 @@ YALIS_API int yalis_packed_attention_mma(const void* q, long long q_stride, int 
     return dim == 64 ? launch_mma<float, 64, 1, 3>(p, (int)grid, stream) : launch_mma<float, 128, 1, 3>(p, (int)grid, stream);
   return YALIS_ERR_DTYPE;
 }
+
+YALIS_SLOTS(yalis_packed_attention_mma)

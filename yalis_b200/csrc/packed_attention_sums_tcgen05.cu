@@ -20,6 +20,7 @@
 // every tile of a block, and a block per item left half of the time to the one with the most rows.
 // All waits are bounded (error word, tensor memory freed).
 #include "packed.cuh"
+#include "slots.cuh"
 #include "tcgen05.cuh"
 
 namespace {
@@ -404,3 +405,5 @@ YALIS_API int yalis_packed_sums_tcgen05(const void* q, long long q_stride, const
   if (!encode(&mq, 3, q, q_sizes, q_strides, q_box) || !encode(&mk, 2, k_unpacked, k_sizes, k_strides, k_box)) return YALIS_ERR_LAUNCH;
   return dim == 64 ? launch_sums<64>(mq, mk, p, stream) : launch_sums<128>(mq, mk, p, stream);
 }
+
+YALIS_SLOTS(yalis_packed_sums_tcgen05)

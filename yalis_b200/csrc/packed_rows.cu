@@ -7,6 +7,7 @@
 // 2 dim values read and dim + 4 bytes written a token and KV head (bfloat16: 512 -> 132 B at 128).  Bound by instructions: 12,003 tokens,
 // 8 KV heads of 128 (62 MB): 25 us to write (2.4 TB/s, issue slots busy 0.78), 14 to read back (4.4 TB/s, 0.70).
 #include "packed.cuh"
+#include "slots.cuh"
 
 namespace {
 
@@ -362,3 +363,6 @@ YALIS_API int yalis_packed_unpack(void* k_codes, void* v_codes, void* words, int
   const long long most = (long long)width * g * n_requests, resident = 4LL * yalis_sm_count();
   return yalis_launch(packed_unpack_kernel, dim3((unsigned)(most < resident ? most : resident)), dim3(kUnpackThreads), 0, stream, p);
 }
+
+YALIS_SLOTS(yalis_packed_rows)
+YALIS_SLOTS(yalis_packed_unpack)

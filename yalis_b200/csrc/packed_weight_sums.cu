@@ -12,6 +12,7 @@
 // a thread per key.  That moves 8 bytes a row and key, where taking the products once more reads the keys' codes again (16 requests of
 // 2,000 to 4,000 tokens, 32 heads of 128 over 8: 58 us by products, 8.5 by scores).
 #include "packed.cuh"
+#include "slots.cuh"
 
 namespace {
 
@@ -325,3 +326,6 @@ YALIS_API int yalis_packed_sums_of_scores(float* scores, long long score_stride,
   return yalis_launch(packed_sums_of_scores_kernel, dim3((unsigned)((max_kv_len + 255LL) / 256), g, n_requests), dim3(256), 0, stream, p, (const float*)scores,
                       score_stride);
 }
+
+YALIS_SLOTS(yalis_packed_weight_sums)
+YALIS_SLOTS(yalis_packed_sums_of_scores)

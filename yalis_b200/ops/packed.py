@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import struct
 from dataclasses import dataclass
 from typing import Optional, Sequence, Tuple
 
@@ -20,18 +21,25 @@ from ._lib import BF16, F32, KernelError, check, dtype_code, lib, need
 from .attention import (PREFILL_SPLIT_GAIN, PREFILL_SPLIT_MIN_TILES, PREFILL_SPLIT_START_UP, PREFILL_SPLIT_UNSHARED, _policy_lib,
                         sm_count)
 
-_TYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
+_TYPES = {"i": ctypes.c_int, "s": ctypes.c_char_p}
 _entries = {}
 
 
-def _entry(name: str, signature: str, result=ctypes.c_int):
-    """The library's function with its argument types set once: plain numbers are handed over as they are (these calls are made
-    for every layer of a step, and converting thirty arguments one by one takes longer than the smaller kernels run)."""
+def _function(name: str, signature: str, result=ctypes.c_int):
+    """The library's function with its argument types set."""
+    fn = getattr(lib(), name)
+    fn.argtypes, fn.restype = [_TYPES[c] for c in signature], result
+    return fn
+
+
+def _entry(name: str, signature: str):
+    """The library's launch of that name, called with plain numbers in one array of slots (``csrc/slots.cuh``): these calls are made for
+    every layer of a step, and handing thirty arguments over one by one takes longer than the smaller kernels run."""
     fn = _entries.get(name)
     if fn is None:
-        fn = getattr(lib(), name)
-        fn.argtypes, fn.restype = [_TYPES[c] for c in signature], result
-        _entries[name] = fn
+        launch = _function(name + "_slots", "s")
+        pack = struct.Struct("".join("d" if c == "f" else "q" for c in signature)).pack
+        fn = _entries[name] = lambda *arguments: launch(pack(*arguments))
     return fn
 
 
@@ -150,8 +158,8 @@ def _mma_launch(device: int, code: int, dim: int, columns: int) -> Tuple[int, in
     key = (device, code, dim, columns)
     found = _mma_launches.get(key)
     if found is None:
-        blocks = _entry("yalis_packed_attention_mma_blocks", "iii")(code, dim, columns)
-        floats = _entry("yalis_packed_attention_mma_scratch_floats", "iii", ctypes.c_longlong)(blocks, dim, columns)
+        blocks = _function("yalis_packed_attention_mma_blocks", "iii")(code, dim, columns)
+        floats = _function("yalis_packed_attention_mma_scratch_floats", "iii", ctypes.c_longlong)(blocks, dim, columns)
         found = _mma_launches[key] = (blocks, floats)
     return found
 
@@ -189,7 +197,7 @@ def packed_kv_read(pages: PackedPages, positions: torch.Tensor, req_of_token: to
     held, n, code = _pages_arguments(name, pages), positions.shape[0] if positions.dim() else -1, dtype_code(dtype)
     _, columns = _check_index(name, n, block_table, positions, req_of_token)
     flag, width = _flag_address(name, error_flag), held[5] * held[6]
-    both = torch.empty((2, n, width), dtype=dtype, device=device)        # one allocation
+    both = torch.empty(2, n, width, dtype=dtype, device=device)        # one allocation
     at = both.data_ptr()
     check(_rows_entry()(0, at, at + n * width * both.element_size(), width, width, code, *held, positions.data_ptr(), req_of_token.data_ptr(),
                         block_table.data_ptr(), columns, n, True, flag, _raw_stream(device)), name)
@@ -378,9 +386,9 @@ def evict_tokens(pools: Sequence[torch.Tensor], weight_sums: torch.Tensor, lengt
         raise KernelError(f"{name}: block_table has fewer rows than requests")
     if keep < 1 or not 0 <= recent <= keep:
         raise KernelError(f"{name}: keep must be at least 1 and recent between 0 and keep")
-    kept = torch.empty((r, g, keep), dtype=torch.int32, device=device)
+    kept = torch.empty(r, g, keep, dtype=torch.int32, device=device)
     check(_entry("yalis_evict_tokens", "ppippp" + "iiiiiii" + "ppp")(
-        addresses, row_bytes, len(pools), weight_sums.data_ptr(), lengths.data_ptr(), block_table.data_ptr(), columns, page_size, pages, g, r, keep,
+        ctypes.addressof(addresses), ctypes.addressof(row_bytes), len(pools), weight_sums.data_ptr(), lengths.data_ptr(), block_table.data_ptr(), columns, page_size, pages, g, r, keep,
         recent, kept.data_ptr(), flag, _raw_stream(device)), name)
     return kept
 

@@ -342,6 +342,30 @@ def test_a_replayed_step_follows_its_inputs():
         torch.testing.assert_close(sums.cpu().double(), 6 * a, rtol=1e-4, atol=1e-6)
 
 
+def test_calls_on_two_streams_at_once():
+    """Steps of different requests on two streams, neither waiting for the other, with workspaces that grow on the way."""
+    from yalis_b200.ops.packed import packed_attention
+    streams, want, got = [torch.cuda.Stream() for _ in range(2)], [], [[], []]
+    inputs = []
+    for i in range(2):
+        c = Cache([900 + 300 * i, 90, 500], 2, 128, 16, seed=20 + i)
+        for brought, heads in (([1, 1, 1], 4), ([1, 3, 2], 16), ([60, 1, 70], 8)):
+            q, pos, q_start = step_of(c, brought, heads=heads, seed=i)
+            pages, table = c.to(DEV)
+            inputs.append((i, q.to(DEV), pages, pos.to(DEV), i32(q_start), table, max(brought), heads))
+    for i, *args in inputs:
+        want.append(packed_attention(*args))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i, *args in inputs:
+            with torch.cuda.stream(streams[i]):
+                got[i].append(packed_attention(*args))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for k, out in enumerate(got[i]):
+            assert torch.equal(out, want[3 * i + k % 3])
+
+
 @pytest.mark.usefixtures("portions_by_both")
 def test_the_same_step_gives_the_same_bits():
     from yalis_b200.ops.packed import packed_attention

@@ -105,3 +105,53 @@ def test_rotate_heads_gives_the_bits_of_the_cache_write(dtype, parts, n, hs):
     assert torch.equal(rows[:-1], torch.cat([q[:-1], k, v], 1))
     some = rotate_heads(qkv, positions, reqs, None, nh, hs, out_dtype=dtype)
     assert torch.equal(some[:-1], (qkv.sum(0) if parts > 1 and parts < 3 else qkv[0] + qkv[1] + qkv[2] if parts == 3 else qkv)[:-1, :nh * hs].to(dtype))
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+@pytest.mark.parametrize("head_dim", [16, 64])
+def test_windows_and_caches_that_two_layers_read(plain_packed, head_dim, graphs):
+    """A layer over a window, whose pages are given back behind it, and one run twice over one cache, cut every way."""
+    import tempfile
+
+    import traces
+    from test_toy_parts_gpu import plain_toy, setup_module, toy_config
+    from yalis_b200.engine.engine import Engine
+    from yalis_b200.engine.replay import Replayer
+    from yalis_b200.weights.loader import write_random_model
+    setup_module(None)
+    c = toy_config(["window_attention", "attention"], [(0, None), (1, None), (1, 1)], window=20, head_dim=head_dim)
+    with tempfile.TemporaryDirectory() as d:
+        write_random_model(c, d, seed=5, std=0.2)
+        w = plain.read_weights(d)
+        g = torch.Generator().manual_seed(2)
+        requests = {f"r{i}": torch.randint(0, c["vocab"], (n,), generator=g).tolist() for i, n in enumerate([150, 33, 97])}
+        want = {rid: plain_toy(t, w, c).numpy() for rid, t in requests.items()}
+        for build in (traces.whole, traces.tail_decoded, traces.portions, traces.mixed):
+            steps = traces.number(build(requests))
+            tokens = traces.peak_tokens(steps)
+            rep = Replayer(d, "float32", tokens, page_size=8, graphs=graphs,
+                           engine=Engine(d, dtype="float32", page_size=8, num_pages=-(-tokens // 64) * 8, max_slots=4, cache_bits=4))
+            assert sorted(x.name for x in rep.engine.groups) == ["kv_all", "kv_window_20"]
+            out = {}
+            for s in steps:
+                r = rep.run_step(s)
+                if r is not None:
+                    out[s["step"]] = r
+            got = traces.collect(steps, out, c["vocab"])
+            for rid in want:
+                assert np.abs(got[rid] - want[rid]).max() <= 1e-4 * np.abs(want[rid]).max(), (build.__name__, rid)
+            rep.engine.manager.check()
+
+
+def test_position_encodings_that_store_by_themselves_are_refused():
+    import tempfile
+
+    from test_toy_parts_gpu import setup_module, toy_config
+    from yalis_b200.engine.engine import Engine
+    from yalis_b200.weights.loader import write_random_model
+    setup_module(None)
+    c = toy_config(["attention"], [(0, None)], positions=["decay"])
+    with tempfile.TemporaryDirectory() as d:
+        write_random_model(c, d, seed=5, std=0.2)
+        with pytest.raises(ValueError, match="4 bits"):
+            Engine(d, dtype="float32", page_size=8, num_pages=8, max_slots=2, cache_bits=4)

@@ -124,8 +124,8 @@ class CacheStorage:
             rows = g.page_size // req.pool
             if self._cache_bits is not None:
                 if not req.packable or req.pool != 1 or req.value_dim != req.head_dim or req.head_dim % 8:
-                    raise ValueError(f"schedule entry {i}: its cache cannot be held in 4 bits (only plain paged attention's, with head sizes "
-                                     "that are multiples of 8)")
+                    raise ValueError(f"schedule entry {i}: its cache cannot be held in 4 bits (only plain paged attention's, with rotary or "
+                                     "no positions and head sizes that are multiples of 8)")
                 pages = PackedPages.empty(g.num_pages, req.num_kv_heads, rows, req.head_dim, self._device)
                 self.bytes += sum(t.numel() * t.element_size() for t in pages.pools())
                 return PackedKVCache(pages, g.name)

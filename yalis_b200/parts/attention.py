@@ -60,7 +60,7 @@ class PagedAttention(Mixer):
         self.w_o = tensors["o_proj"].contiguous()
 
     def cache_request(self) -> PagedKV:
-        return PagedKV(self.g, self.hs, self.window, packable=True)
+        return PagedKV(self.g, self.hs, self.window, packable=self.position.packs)
 
     def capture_key(self, host):
         # everything the choice of kernel and its launch depend on besides the shapes of the step's tensors

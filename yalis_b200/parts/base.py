@@ -322,6 +322,7 @@ NOT_ROTARY = object()     # answer of PositionEncoding.rotary_frequencies for en
 
 class PositionEncoding(Part):
     category = "position"
+    packs = False            # whether ``encode_and_store`` also takes a ``PackedKVCache`` (the result may then be wider than the queries)
 
     def encode_and_store(self, qkv, num_heads, num_kv_heads, head_dim, ctx, cache: PagedKVCache, dtype=None):
         raise NotImplementedError

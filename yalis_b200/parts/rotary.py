@@ -81,6 +81,8 @@ class RotaryEncoding(PositionEncoding):
     otherwise).  The kernels of ``encode_and_store`` turn the half layout only; mixers that prepare their heads
     themselves read ``inv_freq``, ``interleaved`` and ``magnitude``."""
 
+    packs = True
+
     def __init__(self, spec: PartSpec):
         super().__init__(spec)
         self.head_dim = int(spec.params["head_dim"])
@@ -142,6 +144,8 @@ class RotaryEncoding(PositionEncoding):
 
 class NoPositionEncoding(PositionEncoding):
     """Stores K and V unrotated (a mixer that wants positions handled elsewhere)."""
+
+    packs = True
 
     def rotary_frequencies(self, head_dim: int, device):
         return None

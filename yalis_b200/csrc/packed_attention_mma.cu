@@ -45,7 +45,7 @@ constexpr float kNone = -1e30f;  // the maximum of no scores
 constexpr float kUnset = -3e38f; // limit of a column that has seen no score yet: any will do
 constexpr float kLazy = 8.f;   // how far (log2) scores may rise above the maximum in use before the output is rescaled
 constexpr float kTarget = 6.f; // where (log2) the largest weight times its value's step lies in float16 after that: below 2^15 with kLazy more
-constexpr float kSmall = -80.f;  // steps of less (log2) count as this, which keeps the weights themselves within float32
+constexpr float kSmall = -80.f;  // steps of less (log2) count as this, which keeps the weights themselves within float32; so do steps that are no numbers
 
 struct MmaParams {
   const void* q;               // [N, q_stride]
@@ -488,7 +488,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       float4 own = terms_of(st.words[lane], p.scale_log2);
       if constexpr (HALF) {
         own.y -= 16.f;                           // (no sixteens in the keys' codes)
-        height[lane] = fmaxf((float)((int)(__float_as_uint(own.z) >> 23) - 127), kSmall);        // log2 of the value's step
+        // log2 of the value's step.  (Where that is no number its rows have no results, but their weights' sums are as ever.)
+        height[lane] = own.z <= 3.4e38f ? fmaxf((float)((int)(__float_as_uint(own.z) >> 23) - 127), kSmall) : kSmall;
         own.w = __uint_as_float(st.words[lane] >> 16 & 15u);   // the value's zero times 2^-24 in float16
       }
       terms[lane] = own;

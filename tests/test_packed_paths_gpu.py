@@ -88,6 +88,20 @@ def check(cache, q, pos, q_start, heads, window=None, sums=True, flag=0, **optio
 # ---- values without numbers -----------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,g,dim,page,window", [(4, 2, 64, 16, None), (4, 2, 64, 64, 40), (8, 1, 128, 16, 70), (4, 2, 128, 64, None), (4, 2, 24, 16, 40)])
+def test_a_value_without_numbers_is_seen_only_by_those_that_see_it(both_forms, dtype, heads, g, dim, page, window):
+    """One value row in the middle of a portion, one that some windows have passed, one before a window's first key: rows that do not
+    see it keep their numbers, however many there are, and the weights' sums go by the keys alone."""
+    c = Cache([100, 300, 200, 90], g, dim, page, seed=dim + page)
+    for r, j in ((0, 50), (1, 160), (2, 3)):
+        c.words[int(c.table[r, j // page]), g - 1, j % page, 1] = NAN_WORD
+    q, pos, q_start = step_of(c, [100, 170, 130, 1], dtype=dtype, heads=heads)
+    got = check(c, q, pos, q_start, heads, window)
+    assert bool(got.isnan().any()) and bool((~got.isnan()).any())
+    both_forms += ["expects_unpacking"] * (dtype == torch.bfloat16 and dim != 24)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("dim,n", [(64, 1), (128, 1), (128, 7), (24, 1)])
 def test_sums_where_a_value_without_numbers_is_seen(dtype, dim, n):
     """Its weight and everybody else's are softmax weights as ever, though the row's result is none: here it gets nearly all of a

@@ -36,6 +36,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "slots.cuh"
@@ -77,6 +78,9 @@ struct PrefillParams {
   float* part_o;               // [N, nh, n_splits, HS]
   float* part_ml;              // [N, nh, n_splits, 2]
   float* lse2;                 // [N, nh] the logarithm to base two of a row's sum of exponentials, or null
+  const unsigned char* marks;  // [pages, g, 64] of unpacked keys (packed_rows.cu), else null: 1 where a value holds no numbers
+  const int32_t* some_marked;  // `marked_by` if any key is marked (if none is, anything else, as a rule)
+  int marked_by;
   int32_t* error;
   // the general form (see attention_mma.cu, whose arithmetic of scores, sinks and gates this is)
   int window, chunk;           // 0: none
@@ -122,6 +126,7 @@ struct ItemDesc {
   int pos_first;    // absolute position of the first query token
   int hi_key;       // absolute position of the last one = the last visible key
   int lo_last;      // general form: the first key that the last token sees
+  int page_first;   // MARKS: the page of the first key tile
   int trace_row;
 };
 
@@ -138,7 +143,12 @@ __device__ __forceinline__ int first_visible(const PrefillParams& p, int pos) {
 // are left out at both ends.  Shares of an item's keys are for the plain form only.
 // Measured: the layer of 16 heads of 128 over 8 KV heads with chunks, sinks and a gate, 2,048 tokens: 346 us with the mma.sync
 // form (237 us of it that kernel), 172 us with this one.
-template <int HS, bool GEN>
+//
+// MARKS: pools unpacked for this launch, in pages of BN keys that follow one another, whose values without numbers lie there as zeros.
+// A row that sees such a value has no result; the others never meet it.  (A key is hidden by the weight 0, which is not enough where
+// the value is none.)  Marks are looked at only where the unpacking says that there are some: a load
+// and a vote for every tile, or a look at its pages' marks for every item, took 2 us of 40 to 74.
+template <int HS, bool GEN, bool MARKS>
 __global__ void __launch_bounds__(kThreads, 2)
 prefill_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                  const __grid_constant__ CUtensorMap map_v, const PrefillParams p) {
@@ -289,9 +299,11 @@ prefill_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, cons
       const int n_tok = min(p.tokens_per_tile, q_len - t0);
       const int n_rows = n_tok * p.per;
       const int pos_first = p.positions[tok0 + t0];
-      const int hi_key = p.positions[tok0 + t0 + n_tok - 1];
+      const int pos_last = p.positions[tok0 + t0 + n_tok - 1];
+      // (unpacked pools end with the table, and rows before place 0 see one tile of nothing, as rows at -1 do)
+      const int hi_key = MARKS ? max(-1, min(pos_last, p.table_width * BN - 1)) : pos_last;
       // This item's share of the key tiles (all of them without splits).
-      const int lo_key = GEN ? first_visible(p, pos_first) : 0, tile_lo = lo_key / BN;
+      const int lo_key = GEN ? first_visible(p, pos_first) : 0, tile_lo = (MARKS ? min(lo_key, max(hi_key, 0)) : lo_key) / BN;
       const int all_tiles = hi_key / BN + 1 - tile_lo;
       const int wanted = slots > 1 ? min(slots, (all_tiles + p.tiles_per_split - 1) / p.tiles_per_split) : 1;
       const int per_split = (all_tiles + wanted - 1) / wanted;
@@ -318,7 +330,8 @@ prefill_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, cons
         ItemDesc& it = descs[d];
         it.n_tiles = n_tiles; it.tile_base = tile_base; it.n_splits = n_splits; it.split = split; it.kvh = kvh;
         it.tok_first = tok0 + t0; it.n_rows = n_rows; it.pos_first = pos_first; it.hi_key = hi_key;
-        if (GEN) it.lo_last = first_visible(p, hi_key);
+        if (GEN) it.lo_last = first_visible(p, pos_last);
+        if (MARKS) it.page_first = req * p.table_width + tile_base;
         it.trace_row = in_share;
         mbar_arrive(&desc_full[d]);
         // Q, once the products of the item before, which read it, are done.
@@ -477,238 +490,257 @@ prefill_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, cons
     __syncwarp();
   } else {
     // ---------------------------------- softmax, one thread per row ----------------------------
-    const int r = threadIdx.x;                        // row of the tile = tensor-memory lane
-    const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16);
-    uint32_t T = 0;
-    bool ok = true;
-    for (int n = 0; ok; ++n) {
-      const int d = n & 1;
-      if (!warp_wait(&desc_full[d], (n >> 1) & 1, abort_flag, lane)) break;
-      const int n_tiles = descs[d].n_tiles;
-      if (n_tiles < 0) break;
-      const int tile_base = descs[d].tile_base, n_splits = descs[d].n_splits, split = descs[d].split;
-      const int kvh = descs[d].kvh, tok_first = descs[d].tok_first, n_rows = descs[d].n_rows;
-      const int pos_first = descs[d].pos_first, hi_key = descs[d].hi_key;
+    auto softmax = [&](auto with_marks) {
+      constexpr bool MARKED = decltype(with_marks)::value;
+      const int r = threadIdx.x;                        // row of the tile = tensor-memory lane
+      const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16);
+      uint32_t T = 0;
+      bool ok = true;
+      for (int n = 0; ok; ++n) {
+        const int d = n & 1;
+        if (!warp_wait(&desc_full[d], (n >> 1) & 1, abort_flag, lane)) break;
+        const int n_tiles = descs[d].n_tiles;
+        if (n_tiles < 0) break;
+        const int tile_base = descs[d].tile_base, n_splits = descs[d].n_splits, split = descs[d].split;
+        const int kvh = descs[d].kvh, tok_first = descs[d].tok_first, n_rows = descs[d].n_rows;
+        const int pos_first = descs[d].pos_first, hi_key = descs[d].hi_key;
 #ifdef YALIS_TRACE_CLOCKS
-      const int trace_row = descs[d].trace_row;
-      if (threadIdx.x == 0) { STAMP(63, 0); GSTAMP(0); }
+        const int trace_row = descs[d].trace_row;
+        if (threadIdx.x == 0) { STAMP(63, 0); GSTAMP(0); }
 #endif
-      const bool valid = r < n_rows;
-      const int t_in = r / p.per, head = r - t_in * p.per;
-      const int pos_row = valid ? p.positions[tok_first + t_in] : -1;
-      const int lo_row = GEN ? first_visible(p, max(pos_row, 0)) : 0, lo_last = GEN ? descs[d].lo_last : 0;
-      const int head_all = kvh * p.per + head;
-      const float slope2 = GEN && p.slopes ? p.slopes[head_all] * 1.4426950408889634f : 0.f;
-      // scores that are capped or fall off with the distance are brought to the exp2 domain one by one, others on the way
-      const bool one_by_one = GEN && (p.cap_log2 > 0.f || p.slopes != nullptr);
-      const float to_log2 = one_by_one ? 1.0f : p.scale_log2;
-      float m_run = -INFINITY, l_run = 0.f;
-      for (int j = 0; j < n_tiles && ok; ++j) {
-        const int b = (T + j) & 1;
-        const uint32_t ph = ((T + j) >> 1) & 1;
-        const int key0 = (tile_base + j) * BN;
-        if (lane == 0) STAMP(j, 0 + (warp ? 6 + warp * 6 : 0));
-        if (!warp_wait(&s_full[b], ph, abort_flag, lane)) { ok = false; break; }
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (lane == 0) STAMP(j, 1 + (warp ? 6 + warp * 6 : 0));
-        float sv[BN];
-        {
-          const uint32_t s_addr = lane_base + COL_S + b * BN;
-#pragma unroll
-          for (int c0 = 0; c0 < BN; c0 += 32) tmem_ld32(s_addr + c0, *reinterpret_cast<uint32_t(*)[32]>(&sv[c0]));
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        }
-        // S is in registers now; its buffer is written again only after P(j), which takes its place, has been used.
-        if (lane == 0) STAMP(j, 2 + (warp ? 6 + warp * 6 : 0));
-        if (GEN && one_by_one) {
-#pragma unroll
-          for (int c = 0; c < BN; ++c) {
-            const float off = slope2 * (float)(pos_row - (key0 + c));
-            if (p.cap_log2 > 0.f) {                            // c tanh(x / c), saturated where exp would overflow
-              const float x = fminf(sv[c] * p.scale_over_cap - off / p.cap_log2, 15.f);
-              sv[c] = p.cap_log2 * (1.0f - __fdividef(2.0f, __expf(2.0f * x) + 1.0f));
-            } else {
-              sv[c] = sv[c] * p.scale_log2 - off;
-            }
-          }
-        }
-        if (key0 + BN - 1 > pos_first || (GEN && key0 < lo_last) || !valid) {      // some key of the tile is hidden from some row
-#pragma unroll
-          for (int c = 0; c < BN; ++c)
-            if (!valid || key0 + c > pos_row || (GEN && key0 + c < lo_row)) sv[c] = -INFINITY;
-        }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < BN; c += 8) {                    // four chains of three-input maxima
-          mx[0] = max3(mx[0], sv[c], sv[c + 1]); mx[1] = max3(mx[1], sv[c + 2], sv[c + 3]);
-          mx[2] = max3(mx[2], sv[c + 4], sv[c + 5]); mx[3] = max3(mx[3], sv[c + 6], sv[c + 7]);
-        }
-        const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * to_log2;
-        const float m_new = fmaxf(m_run, m_tile);
-        if (lane == 0) STAMP(j, 3 + (warp ? 6 + warp * 6 : 0));
-        // Keep the older maximum unless the new one is more than 2^8 larger: exp2 of at most 8 is
-        // harmless in float32 and bfloat16, and O then needs no rescaling.
-        const bool grow = (m_new - m_run > 8.0f) || (m_run == -INFINITY && m_new != -INFINITY);
-        const float m_use = grow ? m_new : m_run;
-        const float mb = (m_use == -INFINITY) ? 0.f : m_use;
-        const float corr = grow ? ((m_run == -INFINITY) ? 0.f : ex2(m_run - mb)) : 1.f;
-        uint64_t ls2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
-        const uint64_t scale2 = pack2(to_log2, to_log2), nmb2 = pack2(-mb, -mb);
-        const uint32_t p_addr = lane_base + COL_S + b * BN;          // over the first half of S(j)
-#pragma unroll
-        for (int c0 = 0; c0 < BN; c0 += 32) {
-          uint32_t pk[16], lw[GEN ? 16 : 1];
-#pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            // scale and shift, and the row sums, two values to an instruction
-            float x0, x1, x2, x3;
-            unpack2(fma2(pack2(sv[c0 + c], sv[c0 + c + 1]), scale2, nmb2), x0, x1);
-            unpack2(fma2(pack2(sv[c0 + c + 2], sv[c0 + c + 3]), scale2, nmb2), x2, x3);
-            const float p0 = ex2(x0), p1 = ex2(x1), p2 = ex2(x2), p3 = ex2(x3);
-            ls2[0] = add2(ls2[0], pack2(p0, p1));
-            ls2[1] = add2(ls2[1], pack2(p2, p3));
-            pk[c >> 1] = pack_bf16(p0, p1);
-            pk[(c >> 1) + 1] = pack_bf16(p2, p3);
-            if constexpr (GEN) {
-              const uint32_t h0 = pk[c >> 1], h1 = pk[(c >> 1) + 1];
-              lw[c >> 1] = pack_bf16(p0 - __uint_as_float(h0 << 16), p1 - __uint_as_float(h0 & 0xffff0000u));
-              lw[(c >> 1) + 1] = pack_bf16(p2 - __uint_as_float(h1 << 16), p3 - __uint_as_float(h1 & 0xffff0000u));
-            }
-          }
-          tmem_st16(p_addr + (c0 >> 1), pk);
-          if constexpr (GEN) tmem_st16(p_addr + BN / 2 + (c0 >> 1), lw);
-        }
-        float ls[4];
-        unpack2(ls2[0], ls[0], ls[1]);
-        unpack2(ls2[1], ls[2], ls[3]);
-        l_run = l_run * corr + ((ls[0] + ls[1]) + (ls[2] + ls[3]));
-        if (lane == 0) STAMP(j, 4 + (warp ? 6 + warp * 6 : 0));
-        m_run = m_use;
-        // Rescale O in place if some row of this warp moved its maximum (never for the first tile).
-        if (j > 0 && __any_sync(0xffffffffu, grow)) {
-          if (!warp_wait(o_full, (T + j - 1) & 1, abort_flag, lane)) { ok = false; break; }     // P V of tile j-1 is done
+        const bool valid = r < n_rows;
+        const int t_in = r / p.per, head = r - t_in * p.per;
+        const int pos_row = valid ? p.positions[tok_first + t_in] : -1;
+        const int lo_row = GEN ? first_visible(p, max(pos_row, 0)) : 0, lo_last = GEN ? descs[d].lo_last : 0;
+        const int head_all = kvh * p.per + head;
+        const float slope2 = GEN && p.slopes ? p.slopes[head_all] * 1.4426950408889634f : 0.f;
+        // scores that are capped or fall off with the distance are brought to the exp2 domain one by one, others on the way
+        const bool one_by_one = GEN && (p.cap_log2 > 0.f || p.slopes != nullptr);
+        const float to_log2 = one_by_one ? 1.0f : p.scale_log2;
+        float m_run = -INFINITY, l_run = 0.f;
+        bool sees_none = false;                           // whether the row sees a value without numbers
+        for (int j = 0; j < n_tiles && ok; ++j) {
+          const int b = (T + j) & 1;
+          const uint32_t ph = ((T + j) >> 1) & 1;
+          const int key0 = (tile_base + j) * BN;
+          if (lane == 0) STAMP(j, 0 + (warp ? 6 + warp * 6 : 0));
+          if (!warp_wait(&s_full[b], ph, abort_flag, lane)) { ok = false; break; }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll 1
-          for (int c0 = 0; c0 < HS; c0 += 16) {
-            uint32_t o[16];
-            tmem_ld16(lane_base + COL_O + c0, o);
+          if (lane == 0) STAMP(j, 1 + (warp ? 6 + warp * 6 : 0));
+          float sv[BN];
+          {
+            const uint32_t s_addr = lane_base + COL_S + b * BN;
+#pragma unroll
+            for (int c0 = 0; c0 < BN; c0 += 32) tmem_ld32(s_addr + c0, *reinterpret_cast<uint32_t(*)[32]>(&sv[c0]));
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
-            tmem_st16(lane_base + COL_O + c0, o);
           }
-        }
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        if (key0 + BN - 1 > hi_key) {
-          // Last tile: rows of V past the last visible key may hold anything (even NaN); zero them
-          // once the tile has landed, and make the writes visible to the tensor core's reads.
-          if (!warp_wait(&v_full[b], ph, abort_flag, lane)) { ok = false; break; }
-          if (r < BN && key0 + r > hi_key) {
-            unsigned char* vt = v_s + b * KV_BYTES;
+          // S is in registers now; its buffer is written again only after P(j), which takes its place, has been used.
+          if (lane == 0) STAMP(j, 2 + (warp ? 6 + warp * 6 : 0));
+          if (GEN && one_by_one) {
 #pragma unroll
-            for (int h = 0; h < H2; ++h)
-#pragma unroll
-              for (int c = 0; c < 8; ++c)
-                *reinterpret_cast<uint4*>(vt + h * (BN * 128) + r * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[b]);
-        if (lane == 0) STAMP(j, 5 + (warp ? 6 + warp * 6 : 0));
-      }
-      // ---- O / l -> global --------------------------------------------------------------------
-      if (ok) ok = warp_wait(o_done, n & 1, abort_flag, lane);
-      if (!ok) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (n_splits > 1) {
-        // a share: unnormalised, with the maximum it is relative to and its sum
-        const size_t slot = ((size_t)(tok_first + (valid ? t_in : 0)) * p.nh + kvh * p.per + (valid ? head : 0)) * slots + split;
-        float* dst = p.part_o + slot * HS;
-        if (valid) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m_run, l_run);
-#pragma unroll 1
-        for (int c0 = 0; c0 < HS; c0 += 16) {
-          uint32_t o[16];
-          __syncwarp();                                       // rows without a token and rows with one part below
-          tmem_ld16(lane_base + COL_O + c0, o);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-          if (valid) {
-#pragma unroll
-            for (int c = 0; c < 16; c += 4)
-              *reinterpret_cast<uint4*>(dst + c0 + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
-          }
-        }
-      } else {
-        if (slots > 1 && valid) {                             // finished here: the second kernel leaves these rows alone
-          const size_t slot = ((size_t)(tok_first + t_in) * p.nh + kvh * p.per + head) * slots;
-          *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(INFINITY, 0.f);
-        }
-        float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
-        if (p.lse2 && valid) p.lse2[(size_t)(tok_first + t_in) * p.nh + kvh * p.per + head] = m_run + log2f(l_run);
-        const __nv_bfloat16* gate = nullptr;
-        if constexpr (GEN) {
-          if (p.sink) {                                         // the sums stand relative to m_run: the sink joins there
-            const float z = p.sink_logits ? p.sink_logits[head_all] * 1.4426950408889634f : 0.f, mf = fmaxf(m_run, z);
-            const float c = exp2f(m_run - mf);
-            inv = c / (l_run * c + exp2f(z - mf));
-          }
-          inv *= p.out_scale;
-          if (p.gate != nullptr && valid) {
-            gate = p.gate + (size_t)(tok_first + t_in) * p.gate_stride + (p.gate_per_head ? head_all : head_all * HS);
-            if (p.gate_per_head) inv *= 1.0f / (1.0f + __expf(-__bfloat162float(*gate)));
-          }
-        }
-        __nv_bfloat16* dst = p.out + (size_t)(tok_first + (valid ? t_in : 0)) * p.out_stride +
-                             (size_t)(kvh * p.per + (valid ? head : 0)) * HS;
-#pragma unroll 1
-        for (int c0 = 0; c0 < HS; c0 += 16) {
-          uint32_t o[16];
-          __syncwarp();                                       // rows without a token and rows with one part below
-          tmem_ld16(lane_base + COL_O + c0, o);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-          if constexpr (GEN) {
-            if (gate != nullptr && !p.gate_per_head) {
-              const uint4 ga = *reinterpret_cast<const uint4*>(gate + c0), gb = *reinterpret_cast<const uint4*>(gate + c0 + 8);
-              const uint32_t gw[8] = {ga.x, ga.y, ga.z, ga.w, gb.x, gb.y, gb.z, gb.w};
-#pragma unroll
-              for (int c = 0; c < 8; ++c) {
-                o[2 * c] = __float_as_uint(__uint_as_float(o[2 * c]) * (1.0f / (1.0f + __expf(-__uint_as_float(gw[c] << 16)))));
-                o[2 * c + 1] = __float_as_uint(__uint_as_float(o[2 * c + 1]) *
-                                               (1.0f / (1.0f + __expf(-__uint_as_float(gw[c] & 0xffff0000u)))));
+            for (int c = 0; c < BN; ++c) {
+              const float off = slope2 * (float)(pos_row - (key0 + c));
+              if (p.cap_log2 > 0.f) {                            // c tanh(x / c), saturated where exp would overflow
+                const float x = fminf(sv[c] * p.scale_over_cap - off / p.cap_log2, 15.f);
+                sv[c] = p.cap_log2 * (1.0f - __fdividef(2.0f, __expf(2.0f * x) + 1.0f));
+              } else {
+                sv[c] = sv[c] * p.scale_log2 - off;
               }
             }
           }
-          if (valid) {
-            uint4 v0, v1;
-            v0.x = pack_bf16(__uint_as_float(o[0]) * inv, __uint_as_float(o[1]) * inv);
-            v0.y = pack_bf16(__uint_as_float(o[2]) * inv, __uint_as_float(o[3]) * inv);
-            v0.z = pack_bf16(__uint_as_float(o[4]) * inv, __uint_as_float(o[5]) * inv);
-            v0.w = pack_bf16(__uint_as_float(o[6]) * inv, __uint_as_float(o[7]) * inv);
-            v1.x = pack_bf16(__uint_as_float(o[8]) * inv, __uint_as_float(o[9]) * inv);
-            v1.y = pack_bf16(__uint_as_float(o[10]) * inv, __uint_as_float(o[11]) * inv);
-            v1.z = pack_bf16(__uint_as_float(o[12]) * inv, __uint_as_float(o[13]) * inv);
-            v1.w = pack_bf16(__uint_as_float(o[14]) * inv, __uint_as_float(o[15]) * inv);
-            *reinterpret_cast<uint4*>(dst + c0) = v0;
-            *reinterpret_cast<uint4*>(dst + c0 + 8) = v1;
+          if (key0 + BN - 1 > pos_first || (GEN && key0 < lo_last) || !valid || MARKED) {      // some key of the tile is hidden from some row
+#pragma unroll
+            for (int c = 0; c < BN; ++c)
+              if (!valid || key0 + c > pos_row || (GEN && key0 + c < lo_row)) sv[c] = -INFINITY;
+            if constexpr (MARKED) {
+              const uint32_t* mark = reinterpret_cast<const uint32_t*>(p.marks + ((size_t)(descs[d].page_first + j) * p.g + kvh) * BN);
+#pragma unroll
+              for (int c = 0; c < BN; c += 4) {
+                const uint32_t four = mark[c / 4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sees_none |= (four >> (8 * i) & 1u) && sv[c + i] != -INFINITY;
+              }
+            }
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < BN; c += 8) {                    // four chains of three-input maxima
+            mx[0] = max3(mx[0], sv[c], sv[c + 1]); mx[1] = max3(mx[1], sv[c + 2], sv[c + 3]);
+            mx[2] = max3(mx[2], sv[c + 4], sv[c + 5]); mx[3] = max3(mx[3], sv[c + 6], sv[c + 7]);
+          }
+          const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * to_log2;
+          const float m_new = fmaxf(m_run, m_tile);
+          if (lane == 0) STAMP(j, 3 + (warp ? 6 + warp * 6 : 0));
+          // Keep the older maximum unless the new one is more than 2^8 larger: exp2 of at most 8 is
+          // harmless in float32 and bfloat16, and O then needs no rescaling.
+          const bool grow = (m_new - m_run > 8.0f) || (m_run == -INFINITY && m_new != -INFINITY);
+          const float m_use = grow ? m_new : m_run;
+          const float mb = (m_use == -INFINITY) ? 0.f : m_use;
+          const float corr = grow ? ((m_run == -INFINITY) ? 0.f : ex2(m_run - mb)) : 1.f;
+          uint64_t ls2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+          const uint64_t scale2 = pack2(to_log2, to_log2), nmb2 = pack2(-mb, -mb);
+          const uint32_t p_addr = lane_base + COL_S + b * BN;          // over the first half of S(j)
+#pragma unroll
+          for (int c0 = 0; c0 < BN; c0 += 32) {
+            uint32_t pk[16], lw[GEN ? 16 : 1];
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+              // scale and shift, and the row sums, two values to an instruction
+              float x0, x1, x2, x3;
+              unpack2(fma2(pack2(sv[c0 + c], sv[c0 + c + 1]), scale2, nmb2), x0, x1);
+              unpack2(fma2(pack2(sv[c0 + c + 2], sv[c0 + c + 3]), scale2, nmb2), x2, x3);
+              const float p0 = ex2(x0), p1 = ex2(x1), p2 = ex2(x2), p3 = ex2(x3);
+              ls2[0] = add2(ls2[0], pack2(p0, p1));
+              ls2[1] = add2(ls2[1], pack2(p2, p3));
+              pk[c >> 1] = pack_bf16(p0, p1);
+              pk[(c >> 1) + 1] = pack_bf16(p2, p3);
+              if constexpr (GEN) {
+                const uint32_t h0 = pk[c >> 1], h1 = pk[(c >> 1) + 1];
+                lw[c >> 1] = pack_bf16(p0 - __uint_as_float(h0 << 16), p1 - __uint_as_float(h0 & 0xffff0000u));
+                lw[(c >> 1) + 1] = pack_bf16(p2 - __uint_as_float(h1 << 16), p3 - __uint_as_float(h1 & 0xffff0000u));
+              }
+            }
+            tmem_st16(p_addr + (c0 >> 1), pk);
+            if constexpr (GEN) tmem_st16(p_addr + BN / 2 + (c0 >> 1), lw);
+          }
+          float ls[4];
+          unpack2(ls2[0], ls[0], ls[1]);
+          unpack2(ls2[1], ls[2], ls[3]);
+          l_run = l_run * corr + ((ls[0] + ls[1]) + (ls[2] + ls[3]));
+          if (lane == 0) STAMP(j, 4 + (warp ? 6 + warp * 6 : 0));
+          m_run = m_use;
+          // Rescale O in place if some row of this warp moved its maximum (never for the first tile).
+          if (j > 0 && __any_sync(0xffffffffu, grow)) {
+            if (!warp_wait(o_full, (T + j - 1) & 1, abort_flag, lane)) { ok = false; break; }     // P V of tile j-1 is done
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+            for (int c0 = 0; c0 < HS; c0 += 16) {
+              uint32_t o[16];
+              tmem_ld16(lane_base + COL_O + c0, o);
+              asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+              for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
+              tmem_st16(lane_base + COL_O + c0, o);
+            }
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          if (key0 + BN - 1 > hi_key) {
+            // Last tile: rows of V past the last visible key may hold anything (even NaN); zero them
+            // once the tile has landed, and make the writes visible to the tensor core's reads.
+            if (!warp_wait(&v_full[b], ph, abort_flag, lane)) { ok = false; break; }
+            if (r < BN && key0 + r > hi_key) {
+              unsigned char* vt = v_s + b * KV_BYTES;
+#pragma unroll
+              for (int h = 0; h < H2; ++h)
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                  *reinterpret_cast<uint4*>(vt + h * (BN * 128) + r * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          }
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[b]);
+          if (lane == 0) STAMP(j, 5 + (warp ? 6 + warp * 6 : 0));
+        }
+        // ---- O / l -> global --------------------------------------------------------------------
+        if (ok) ok = warp_wait(o_done, n & 1, abort_flag, lane);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (n_splits > 1) {
+          // a share: unnormalised, with the maximum it is relative to and its sum
+          const size_t slot = ((size_t)(tok_first + (valid ? t_in : 0)) * p.nh + kvh * p.per + (valid ? head : 0)) * slots + split;
+          float* dst = p.part_o + slot * HS;
+          if (valid) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m_run, l_run);
+#pragma unroll 1
+          for (int c0 = 0; c0 < HS; c0 += 16) {
+            uint32_t o[16];
+            __syncwarp();                                       // rows without a token and rows with one part below
+            tmem_ld16(lane_base + COL_O + c0, o);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            if (valid) {
+              if (MARKED && sees_none)
+#pragma unroll
+                for (int c = 0; c < 16; ++c) o[c] = 0x7FFFFFFFu;
+#pragma unroll
+              for (int c = 0; c < 16; c += 4)
+                *reinterpret_cast<uint4*>(dst + c0 + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+            }
+          }
+        } else {
+          if (slots > 1 && valid) {                             // finished here: the second kernel leaves these rows alone
+            const size_t slot = ((size_t)(tok_first + t_in) * p.nh + kvh * p.per + head) * slots;
+            *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(INFINITY, 0.f);
+          }
+          float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
+          if (p.lse2 && valid) p.lse2[(size_t)(tok_first + t_in) * p.nh + kvh * p.per + head] = m_run + log2f(l_run);
+          const __nv_bfloat16* gate = nullptr;
+          if constexpr (GEN) {
+            if (p.sink) {                                         // the sums stand relative to m_run: the sink joins there
+              const float z = p.sink_logits ? p.sink_logits[head_all] * 1.4426950408889634f : 0.f, mf = fmaxf(m_run, z);
+              const float c = exp2f(m_run - mf);
+              inv = c / (l_run * c + exp2f(z - mf));
+            }
+            inv *= p.out_scale;
+            if (p.gate != nullptr && valid) {
+              gate = p.gate + (size_t)(tok_first + t_in) * p.gate_stride + (p.gate_per_head ? head_all : head_all * HS);
+              if (p.gate_per_head) inv *= 1.0f / (1.0f + __expf(-__bfloat162float(*gate)));
+            }
+          }
+          if (MARKED && sees_none) inv = NAN;
+          __nv_bfloat16* dst = p.out + (size_t)(tok_first + (valid ? t_in : 0)) * p.out_stride +
+                               (size_t)(kvh * p.per + (valid ? head : 0)) * HS;
+#pragma unroll 1
+          for (int c0 = 0; c0 < HS; c0 += 16) {
+            uint32_t o[16];
+            __syncwarp();                                       // rows without a token and rows with one part below
+            tmem_ld16(lane_base + COL_O + c0, o);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            if constexpr (GEN) {
+              if (gate != nullptr && !p.gate_per_head) {
+                const uint4 ga = *reinterpret_cast<const uint4*>(gate + c0), gb = *reinterpret_cast<const uint4*>(gate + c0 + 8);
+                const uint32_t gw[8] = {ga.x, ga.y, ga.z, ga.w, gb.x, gb.y, gb.z, gb.w};
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                  o[2 * c] = __float_as_uint(__uint_as_float(o[2 * c]) * (1.0f / (1.0f + __expf(-__uint_as_float(gw[c] << 16)))));
+                  o[2 * c + 1] = __float_as_uint(__uint_as_float(o[2 * c + 1]) *
+                                                 (1.0f / (1.0f + __expf(-__uint_as_float(gw[c] & 0xffff0000u)))));
+                }
+              }
+            }
+            if (valid) {
+              uint4 v0, v1;
+              v0.x = pack_bf16(__uint_as_float(o[0]) * inv, __uint_as_float(o[1]) * inv);
+              v0.y = pack_bf16(__uint_as_float(o[2]) * inv, __uint_as_float(o[3]) * inv);
+              v0.z = pack_bf16(__uint_as_float(o[4]) * inv, __uint_as_float(o[5]) * inv);
+              v0.w = pack_bf16(__uint_as_float(o[6]) * inv, __uint_as_float(o[7]) * inv);
+              v1.x = pack_bf16(__uint_as_float(o[8]) * inv, __uint_as_float(o[9]) * inv);
+              v1.y = pack_bf16(__uint_as_float(o[10]) * inv, __uint_as_float(o[11]) * inv);
+              v1.z = pack_bf16(__uint_as_float(o[12]) * inv, __uint_as_float(o[13]) * inv);
+              v1.w = pack_bf16(__uint_as_float(o[14]) * inv, __uint_as_float(o[15]) * inv);
+              *reinterpret_cast<uint4*>(dst + c0) = v0;
+              *reinterpret_cast<uint4*>(dst + c0 + 8) = v1;
+            }
           }
         }
-      }
 #ifdef YALIS_TRACE_CLOCKS
-      if (threadIdx.x == 0) {
-        GSTAMP(1);
-        unsigned sm_;
-        asm volatile("mov.u32 %0, %%smid;" : "=r"(sm_));
-        if (p.trace) p.trace[((size_t)trace_row * 64 + 62) * 32 + 2] = sm_ + 1;
-      }
+        if (threadIdx.x == 0) {
+          GSTAMP(1);
+          unsigned sm_;
+          asm volatile("mov.u32 %0, %%smid;" : "=r"(sm_));
+          if (p.trace) p.trace[((size_t)trace_row * 64 + 62) * 32 + 2] = sm_ + 1;
+        }
 #endif
-      T += (uint32_t)n_tiles;
-      // The O of this item is in registers or written: the next item's first P V may overwrite it (it waits for
-      // this warp's next arrival at p_full, which comes after this point).
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&desc_empty[d]);
-    }
+        T += (uint32_t)n_tiles;
+        // The O of this item is in registers or written: the next item's first P V may overwrite it (it waits for
+        // this warp's next arrival at p_full, which comes after this point).
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&desc_empty[d]);
+      }
+    };
+    if (MARKS && *p.some_marked == p.marked_by) softmax(std::bool_constant<MARKS>());
+    else softmax(std::false_type());
   }
 
   // ---- exit: drain on abort, hand the counter back, free tensor memory -------------------------------------
@@ -808,23 +840,23 @@ __global__ void prefill_merge_splits_kernel(const float* part_o, const float* pa
   }
 }
 
-template <int HS, bool GEN>
+template <int HS, bool GEN, bool MARKS>
 int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const PrefillParams& p, int n_splits,
-           int n_tokens, bool rows_of_requests, cudaStream_t stream) {
+           int n_tokens, cudaStream_t stream) {
   const size_t smem = 1024 + (size_t)BM * HS * 2 + (size_t)4 * BN * HS * 2 + kBarriers * 8 + 8 + 2 * sizeof(ItemDesc);
   static bool configured = false;
   if (!configured) {
-    if (cudaFuncSetAttribute(prefill_attention_tcgen05_kernel<HS, GEN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(prefill_attention_tcgen05_kernel<HS, GEN, MARKS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (int)smem) != cudaSuccess)
       return YALIS_ERR_LAUNCH;
     configured = true;
   }
   // Two blocks to an SM for the whole launch (fewer if the step has fewer items).
   dim3 grid((unsigned)std::min<long long>(p.n_items, 2LL * yalis_sm_count()), 1, 1);
-  int st = yalis_launch(prefill_attention_tcgen05_kernel<HS, GEN>, grid, dim3(kThreads), smem, stream, mq, mk, mv, p);
+  int st = yalis_launch(prefill_attention_tcgen05_kernel<HS, GEN, MARKS>, grid, dim3(kThreads), smem, stream, mq, mk, mv, p);
   if (st != YALIS_OK || n_splits == 1) return st;
   return yalis_launch(prefill_merge_splits_kernel, dim3(n_tokens), dim3(256), 0, stream, (const float*)p.part_o,
-                      (const float*)p.part_ml, p.out, p.out_stride, p.nh, HS, n_splits, rows_of_requests ? p.q_start : (const int32_t*)nullptr,
+                      (const float*)p.part_ml, p.out, p.out_stride, p.nh, HS, n_splits, MARKS ? p.q_start : (const int32_t*)nullptr,
                       p.n_requests, p.lse2);
 }
 
@@ -841,16 +873,16 @@ bool count_items(PrefillParams& p, int n_tokens, int max_q_len, int n_splits) {
   return true;
 }
 
-template <bool GEN>
+template <bool GEN, bool MARKS = false>
 int launch_prefill(const PrefillParams& p, const void* q, int q_stride, const void* k_pool, const void* v_pool, int n_tokens,
-                   int hs, int n_splits, cudaStream_t stream, bool rows_of_requests = false) {
+                   int hs, int n_splits, cudaStream_t stream) {
   CUtensorMap mq, mk, mv;
   const long long rows = (long long)p.num_pages * p.g * p.page_size;
   if (!make_q_map(&mq, q, n_tokens, q_stride, p.nh, hs, p.per, p.tokens_per_tile) ||
       !make_pool_map(&mk, k_pool, rows, hs, p.page_size) || !make_pool_map(&mv, v_pool, rows, hs, p.page_size))
     return YALIS_ERR_LAUNCH;
-  return hs == 64 ? launch<64, GEN>(mq, mk, mv, p, n_splits, n_tokens, rows_of_requests, stream)
-                  : launch<128, GEN>(mq, mk, mv, p, n_splits, n_tokens, rows_of_requests, stream);
+  return hs == 64 ? launch<64, GEN, MARKS>(mq, mk, mv, p, n_splits, n_tokens, stream)
+                  : launch<128, GEN, MARKS>(mq, mk, mv, p, n_splits, n_tokens, stream);
 }
 
 }  // namespace
@@ -954,18 +986,20 @@ YALIS_API int yalis_prefill_attention_tcgen05_general(
   return launch_prefill<true>(p, q, q_stride, k_pool, v_pool, n_tokens, hs, 1, stream);
 }
 
-// For caches in another format, whose visible rows were unpacked into pools of this call (see packed_attention.cu): a window (0:
-// none, else without shares of the keys), rows of no request left alone, and `lse2` [N, nh] or null.  Otherwise as above.
+// For caches in another format, whose visible rows were unpacked into pools of this call (yalis_packed_unpack: pages of 64 keys, a
+// request's pages one after the other, `marks` of their keys): a window (0: none, else without shares of the keys), rows of no request
+// left alone, and `lse2` [N, nh] or null.  Otherwise as above.
 YALIS_API int yalis_prefill_attention_tcgen05_unpacked(
-    const void* q, long long q_stride, void* out, long long out_stride, const void* k_pool, const void* v_pool, const int32_t* positions,
-    const int32_t* q_start, const int32_t* block_table, int table_width, int page_size, int num_pages, int n_tokens, int n_requests,
+    const void* q, long long q_stride, void* out, long long out_stride, const void* k_pool, const void* v_pool, const void* marks, const int32_t* some_marked, int marked_by,
+    const int32_t* positions, const int32_t* q_start, const int32_t* block_table, int table_width, int page_size, int num_pages, int n_tokens, int n_requests,
     int max_q_len, int nh, int g, int hs, float scale, int window, int n_splits, int tiles_per_split, int skip_single, float* lse2,
     float* scratch, int32_t* work, int32_t* error, cudaStream_t stream) {
   if (n_tokens <= 0 || n_requests <= 0) return YALIS_OK;
   if (g <= 0 || nh % g != 0 || max_q_len < 1 || !(scale > 0.f) || n_splits < 1 || n_splits > 64 || tiles_per_split < 1) return YALIS_ERR_SHAPE;
   if (q_stride > 0x7fffffff || out_stride > 0x7fffffff || (window > 0 && n_splits > 1)) return YALIS_ERR_SHAPE;
   if (n_splits > 1 && (scratch == nullptr || ((uintptr_t)scratch & 15))) return YALIS_ERR_ALIGN;
-  if (!yalis_prefill_attention_tcgen05_supports(hs, page_size, nh / g)) return YALIS_ERR_SHAPE;
+  if (page_size != BN || !yalis_prefill_attention_tcgen05_supports(hs, page_size, nh / g)) return YALIS_ERR_SHAPE;
+  if (marks == nullptr || some_marked == nullptr || ((uintptr_t)marks & 3)) return YALIS_ERR_ALIGN;
   if ((((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out) & 15) || (q_stride % 8) || (out_stride % 8)) return YALIS_ERR_ALIGN;
   PrefillParams p = {};
   p.out = (__nv_bfloat16*)out; p.out_stride = (int)out_stride;
@@ -983,9 +1017,10 @@ YALIS_API int yalis_prefill_attention_tcgen05_unpacked(
   p.part_ml = scratch ? scratch + (size_t)n_tokens * nh * n_splits * hs : nullptr;
   p.lse2 = lse2;
   p.error = error;
+  p.marks = static_cast<const unsigned char*>(marks); p.some_marked = some_marked; p.marked_by = marked_by;
   p.window = window; p.out_scale = 1.f;
-  return window > 0 ? launch_prefill<true>(p, q, (int)q_stride, k_pool, v_pool, n_tokens, hs, 1, stream, true)
-                    : launch_prefill<false>(p, q, (int)q_stride, k_pool, v_pool, n_tokens, hs, n_splits, stream, true);
+  return window > 0 ? launch_prefill<true, true>(p, q, (int)q_stride, k_pool, v_pool, n_tokens, hs, 1, stream)
+                    : launch_prefill<false, true>(p, q, (int)q_stride, k_pool, v_pool, n_tokens, hs, n_splits, stream);
 }
 
 YALIS_SLOTS(yalis_prefill_attention_tcgen05_unpacked)

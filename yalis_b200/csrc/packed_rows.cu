@@ -224,7 +224,8 @@ int launch_rows(const RowParams<T>& p, int n_tokens, cudaStream_t stream) {
 
 // The visible rows of requests' caches into bfloat16 pools of one call, for kernels that read such pools: pages of kUnpackPage
 // keys, request after request (page r * width + i holds keys i * kUnpackPage ... of request r), with the block table that says so
-// and the counters of the kernels behind it at zero.  Exact: every value is a bfloat16 number.
+// and the counters of the kernels behind it at zero.  Exact: every value is a bfloat16 number.  A value row without numbers goes in
+// as zeros and is marked instead: rows that do not see it give it the weight 0, and 0 times what is no number is none either.
 // An item is a page of one KV head; a resident grid walks the items that some request needs, which every block counts for itself
 // from the step's lengths (a block for every page that a request could have took 75 us of 64 requests, one of them a portion of
 // 4,033 tokens behind 3,967 and the others single tokens behind 8,000 that need none; now 12).  A thread takes eight codes of a row at
@@ -235,6 +236,9 @@ constexpr int kUnpackPage = 64, kUnpackThreads = 256;
 struct UnpackParams {
   __nv_bfloat16* k_out;        // [R * width, g, kUnpackPage, dim]
   __nv_bfloat16* v_out;
+  unsigned char* marks;        // [R * width, g, kUnpackPage] of each key: 1 where its value holds no numbers, else 0
+  int32_t* some_marked;        // becomes `marked_by`, a number of this launch's own, if any key is marked
+  int marked_by;
   int32_t* table_out;          // [R, width]
   int32_t* zeroed;             // [n_zeroed] counters
   int n_zeroed;
@@ -262,7 +266,8 @@ __global__ void __launch_bounds__(kUnpackThreads, 4) packed_unpack_kernel(const 
     if (r0 + tid < p.n_requests) {
       const int t0 = p.q_start[r0 + tid], n = p.q_start[r0 + tid + 1] - t0;
       if (n > 1 || (n == 1 && !p.skip_single)) {
-        const int last = min(p.positions[t0 + n - 1], p.width * kUnpackPage - 1);
+        const int place = p.positions[t0 + n - 1], last = min(place, p.width * kUnpackPage - 1);
+        if (place > last && blockIdx.x == 0 && p.error) atomicOr(p.error, YALIS_FLAG_BAD_PAGE);       // (it sees places that no pool has)
         const int first = p.window > 0 ? max(0, p.positions[t0] - p.window + 1) : 0;
         first_key[tid] = first;
         last_key[tid] = last;
@@ -317,8 +322,11 @@ __global__ void __launch_bounds__(kUnpackThreads, 4) packed_unpack_kernel(const 
         for (int j = 0; j < 4; ++j) {
           const int r = q + j * per_round;
           if (r >= rows) break;
+          const bool none = (word[j] >> 16 & 0x7F80u) == 0x7F80u;
           reinterpret_cast<uint4*>(p.k_out)[(to + r) * words + w] = unpack_bf16(kc[j], word[j] & 0xFFFFu);
-          reinterpret_cast<uint4*>(p.v_out)[(to + r) * words + w] = unpack_bf16(vc[j], word[j] >> 16);
+          reinterpret_cast<uint4*>(p.v_out)[(to + r) * words + w] = unpack_bf16(vc[j], none ? 0u : word[j] >> 16);
+          if (w == 0) p.marks[to + r] = none ? 1 : 0;
+          if (none) *p.some_marked = p.marked_by;
         }
       }
     }
@@ -350,13 +358,14 @@ YALIS_API int yalis_packed_rows(int write, void* k, void* v, long long k_stride,
 
 YALIS_API int yalis_packed_unpack(void* k_codes, void* v_codes, void* words, int num_pages, int page_size, int g, int dim, const int32_t* positions,
                                   const int32_t* q_start, const int32_t* block_table, int table_width, int n_requests, int width, int window,
-                                  int skip_single, void* k_out, void* v_out, int32_t* table_out, int32_t* zeroed, int n_zeroed, int32_t* error,
-                                  cudaStream_t stream) {
+                                  int skip_single, void* k_out, void* v_out, void* marks, int32_t* some_marked, int marked_by,
+                                  int32_t* table_out, int32_t* zeroed, int n_zeroed, int32_t* error, cudaStream_t stream) {
   if (dim < 8 || dim > 256 || dim % 8 || page_size < 1 || g < 1 || width < 1) return YALIS_ERR_SHAPE;
   if (n_requests <= 0) return YALIS_OK;
   UnpackParams p = {};
   p.n_zeroed = n_zeroed;
-  p.k_out = static_cast<__nv_bfloat16*>(k_out); p.v_out = static_cast<__nv_bfloat16*>(v_out); p.table_out = table_out; p.zeroed = zeroed;
+  p.k_out = static_cast<__nv_bfloat16*>(k_out); p.v_out = static_cast<__nv_bfloat16*>(v_out); p.marks = static_cast<unsigned char*>(marks);
+  p.some_marked = some_marked; p.marked_by = marked_by; p.table_out = table_out; p.zeroed = zeroed;
   p.positions = positions; p.q_start = q_start; p.block_table = block_table; p.table_width = table_width; p.n_requests = n_requests;
   p.width = width; p.window = window; p.skip_single = skip_single; p.error = error;
   p.pages = packed_pages(k_codes, v_codes, words, num_pages, page_size, g, dim);

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import itertools
 import math
 import struct
 from dataclasses import dataclass
@@ -211,6 +212,7 @@ _LONGEST = (1 << 31) - 1   # places are 32-bit numbers
 UNPACK_ROWS, UNPACK_FEW = 64, 1 << 21
 UNPACK_PAGE = 64          # keys of a page of the unpacked pools
 UNPACK_BYTES = 2 << 30    # of unpacked keys and values at a time
+_unpackings = itertools.count(1)       # numbers by which a launch tells its own note that keys are marked from what the memory held before
 SCORE_BYTES = 1 << 30     # of scores that a step of few rows may leave for its sums; beyond, the products are taken once more
 
 
@@ -238,23 +240,28 @@ def _attend_unpacked(name, device, rows, held, at, n, max_q_len, max_kv_len, num
     tiles = -(-max_q_len // (128 // per))               # tiles of rows that see an item, at most; about half of them on average
     each = max(16, items * tiles // (8 * sms))
     parts = -(-tiles // each)
-    # pools, counters (two of the prompt kernel's, one and four an item of the sums'), block table, shares of outputs and of sums
+    # pools; shares of outputs and of sums, counters (two of the prompt kernel's, one and four an item of the sums'), block table, marks of
+    # keys and whether there are any
     floats = n * num_heads * splits * (dim + 2) if splits > 1 else 0
     pools = torch.empty(2 * group * size, dtype=torch.bfloat16, device=device)
     n_counters = (3 + 4 * items + 3) // 4 * 4
-    work = torch.empty(floats + items * parts * 384 + n_counters + group * width, dtype=torch.int32, device=device)
+    pages = group * width
+    work = torch.empty(floats + items * parts * 384 + n_counters + pages * (1 + g * UNPACK_PAGE // 4) + 1, dtype=torch.int32, device=device)
     k_at, scratch = pools.data_ptr(), work.data_ptr()
     v_at, partial = k_at + 2 * group * size, scratch + 4 * floats
     counters = partial + 4 * items * parts * 384
     table_at = counters + 4 * n_counters
+    marks_at = table_at + 4 * pages
+    some_marked_at, marked_by = marks_at + pages * g * UNPACK_PAGE, next(_unpackings) & 0x7FFFFFFF
     for first in range(0, r, group):
         m = min(group, r - first)
         starts, row = q_start + 4 * first, table + 4 * first * table_width
-        check(_entry("yalis_packed_unpack", "pppiiii" + "pppii" + "iii" + "ppppipp")(
-            *held, positions, starts, row, table_width, m, width, window, skip_single, k_at, v_at, table_at, counters, 3 + 4 * items, flag, raw), name)
-        check(_entry("yalis_prefill_attention_tcgen05_unpacked", "plplpp" + "pppiii" + "iiiiii" + "fiiiippppp")(
-            *rows, k_at, v_at, positions, starts, table_at, width, UNPACK_PAGE, m * width, n, m, max_q_len, num_heads, g, dim, scale, window, splits,
-            share, skip_single, _address(lse2), scratch, counters, flag, raw), name)
+        check(_entry("yalis_packed_unpack", "pppiiii" + "pppii" + "iii" + "ppppip" + "pipp")(
+            *held, positions, starts, row, table_width, m, width, window, skip_single, k_at, v_at, marks_at, some_marked_at, marked_by, table_at,
+            counters, 3 + 4 * items, flag, raw), name)
+        check(_entry("yalis_prefill_attention_tcgen05_unpacked", "plpl" + "ppppi" + "pppiii" + "iiiiii" + "fiiiippppp")(
+            *rows, k_at, v_at, marks_at, some_marked_at, marked_by, positions, starts, table_at, width, UNPACK_PAGE, m * width, n, m, max_q_len,
+            num_heads, g, dim, scale, window, splits, share, skip_single, _address(lse2), scratch, counters, flag, raw), name)
         if lse2 is not None:
             check(_entry("yalis_packed_sums_tcgen05", "plpiiiii" + "pppiiiiifii" + "ppiipppp")(
                 *rows[:2], k_at, width, held[3], held[4], g, dim, positions, starts, row, table_width, m, n, max_kv_len, num_heads, scale, window,

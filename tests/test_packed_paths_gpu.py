@@ -113,3 +113,23 @@ def test_sums_where_a_value_without_numbers_is_seen(dtype, dim, n):
         c.words[at, 0, j % 16, 0] = torch.tensor(2.0 ** -2).bfloat16().view(torch.int16) | 7
     q, pos, q_start = step_of(c, [n, n], dtype=dtype, heads=4)
     check(c, q, pos, q_start, 4)
+
+# ---- keys without a page --------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,g,dim", [(4, 2, 64), (8, 1, 128), (4, 2, 24)])
+@pytest.mark.parametrize("page,window", [(16, None), (64, None), (16, 90), (5, None)])
+@pytest.mark.parametrize("brought", [[1, 1, 1, 1], [5, 1, 3, 2], [100, 40, 150, 1]])
+def test_keys_without_a_page_are_left_out(both_forms, dtype, heads, g, dim, page, window, brought):
+    """At the start, in the middle (of keys that every row sees), at the end, and all of a request's: neither rows nor normaliser
+    nor sums know them, and the error word tells."""
+    c = Cache([333, 200, 150, 70], g, dim, page, seed=dim + page)
+    at = lambda r, *places: [c.table[r, j // page].fill_(w) for j, w in places]
+    at(0, (100, -1), (210, c.k.shape[0]), (332, -5))
+    at(1, (0, -1), (10, c.k.shape[0] + 7))
+    c.table[2] = -1
+    q, pos, q_start = step_of(c, brought, dtype=dtype, heads=heads)
+    got = check(c, q, pos, q_start, heads, window, flag=BAD_PAGE)
+    assert bool((got[q_start[2]:q_start[3]] == 0).all())
+    both_forms += ["expects_unpacking"] * (dtype == torch.bfloat16 and dim != 24)
+    check(c, q, pos, q_start, heads, window, sums=False, flag=BAD_PAGE)

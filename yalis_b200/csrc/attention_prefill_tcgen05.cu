@@ -78,7 +78,7 @@ struct PrefillParams {
   float* part_o;               // [N, nh, n_splits, HS]
   float* part_ml;              // [N, nh, n_splits, 2]
   float* lse2;                 // [N, nh] the logarithm to base two of a row's sum of exponentials, or null
-  const unsigned char* marks;  // [pages, g, 64] of unpacked keys (packed_rows.cu), else null: 1 where a value holds no numbers
+  const unsigned char* marks;  // [pages, g, 64] of unpacked keys (packed_rows.cu), else null: bit 0 where a value holds no numbers, 1 without a page
   const int32_t* some_marked;  // `marked_by` if any key is marked (if none is, anything else, as a rule)
   int marked_by;
   int32_t* error;
@@ -146,7 +146,7 @@ __device__ __forceinline__ int first_visible(const PrefillParams& p, int pos) {
 //
 // MARKS: pools unpacked for this launch, in pages of BN keys that follow one another, whose values without numbers lie there as zeros.
 // A row that sees such a value has no result; the others never meet it.  (A key is hidden by the weight 0, which is not enough where
-// the value is none.)  Marks are looked at only where the unpacking says that there are some: a load
+// the value is none.)  Keys without a page are zeros as well and hidden from every row.  Marks are looked at only where the unpacking says that there are some: a load
 // and a vote for every tile, or a look at its pages' marks for every item, took 2 us of 40 to 74.
 template <int HS, bool GEN, bool MARKS>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -558,7 +558,10 @@ prefill_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, cons
               for (int c = 0; c < BN; c += 4) {
                 const uint32_t four = mark[c / 4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sees_none |= (four >> (8 * i) & 1u) && sv[c + i] != -INFINITY;
+                for (int i = 0; i < 4; ++i) {
+                  if (four >> (8 * i) & 2u) sv[c + i] = -INFINITY;
+                  sees_none |= (four >> (8 * i) & 1u) && sv[c + i] != -INFINITY;
+                }
               }
             }
           }

@@ -643,7 +643,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
               sc[nt][half][i] = MASK && v == -INFINITY ? 0.f : e * term[half][i >> 1].z;         // a row that is not seen may hold anything
             }
       };
-      if (__any_sync(0xffffffffu, key0 + kChunk - 1 > all_hi || key0 < all_lo)) weigh(std::true_type());
+      // (a key without a page is hidden from every column)
+      if (__any_sync(0xffffffffu, key0 + kChunk - 1 > all_hi || key0 < all_lo || own.z == 0.f)) weigh(std::true_type());
       else weigh(std::false_type());
       uint32_t wf[NT][2][2][PARTS];              // [half][keys g, g + 8 of the half]: the weights as the second product's operand
 #pragma unroll

@@ -225,7 +225,8 @@ int launch_rows(const RowParams<T>& p, int n_tokens, cudaStream_t stream) {
 // The visible rows of requests' caches into bfloat16 pools of one call, for kernels that read such pools: pages of kUnpackPage
 // keys, request after request (page r * width + i holds keys i * kUnpackPage ... of request r), with the block table that says so
 // and the counters of the kernels behind it at zero.  Exact: every value is a bfloat16 number.  A value row without numbers goes in
-// as zeros and is marked instead: rows that do not see it give it the weight 0, and 0 times what is no number is none either.
+// as zeros and is marked instead: rows that do not see it give it the weight 0, and 0 times what is no number is none either.  A key
+// without a page is zeros and marked too (it would count as a score of 0).
 // An item is a page of one KV head; a resident grid walks the items that some request needs, which every block counts for itself
 // from the step's lengths (a block for every page that a request could have took 75 us of 64 requests, one of them a portion of
 // 4,033 tokens behind 3,967 and the others single tokens behind 8,000 that need none; now 12).  A thread takes eight codes of a row at
@@ -236,7 +237,7 @@ constexpr int kUnpackPage = 64, kUnpackThreads = 256;
 struct UnpackParams {
   __nv_bfloat16* k_out;        // [R * width, g, kUnpackPage, dim]
   __nv_bfloat16* v_out;
-  unsigned char* marks;        // [R * width, g, kUnpackPage] of each key: 1 where its value holds no numbers, else 0
+  unsigned char* marks;        // [R * width, g, kUnpackPage] of each key: bit 0 where its value holds no numbers, bit 1 where it has no page
   int32_t* some_marked;        // becomes `marked_by`, a number of this launch's own, if any key is marked
   int marked_by;
   int32_t* table_out;          // [R, width]
@@ -312,7 +313,7 @@ __global__ void __launch_bounds__(kUnpackThreads, 4) packed_unpack_kernel(const 
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          word[j] = kc[j] = vc[j] = 0u;                       // (a key without a page: zeros)
+          word[j] = kc[j] = vc[j] = 0u;
           if (at[j] < 0) continue;
           word[j] = p.pages.words[at[j]];
           kc[j] = p.pages.k[at[j] * words + w];
@@ -325,8 +326,8 @@ __global__ void __launch_bounds__(kUnpackThreads, 4) packed_unpack_kernel(const 
           const bool none = (word[j] >> 16 & 0x7F80u) == 0x7F80u;
           reinterpret_cast<uint4*>(p.k_out)[(to + r) * words + w] = unpack_bf16(kc[j], word[j] & 0xFFFFu);
           reinterpret_cast<uint4*>(p.v_out)[(to + r) * words + w] = unpack_bf16(vc[j], none ? 0u : word[j] >> 16);
-          if (w == 0) p.marks[to + r] = none ? 1 : 0;
-          if (none) *p.some_marked = p.marked_by;
+          if (w == 0) p.marks[to + r] = (none ? 1 : 0) | (at[j] < 0 ? 2 : 0);
+          if (none || at[j] < 0) *p.some_marked = p.marked_by;
         }
       }
     }

@@ -281,7 +281,8 @@ def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tenso
     rows of a request, ``max_kv_len`` the places seen (the block table's width bounds them otherwise).  ``weight_sums`` float32
     [pages, kv_heads, page_size]: the softmax weight that a token received, summed over the step's rows and the heads of the KV
     head, is added to it (pages of different requests must differ then).  The result is [N, heads * head_dim] in q's dtype
-    (``out`` may be a column block of a wider matrix); rows that see nothing are zeros, rows of no request stay as they are.
+    (``out`` may be a column block of a wider matrix); rows that see nothing are zeros, rows of no request stay as they are.  Places
+    without a page are left out, as if the row did not see them, and raise the error word's bit.
     Scores, weights and sums are float32, and with float32 queries so is every product."""
     name = "packed_attention"
     device = _need_here(name, q, pages.k, pages.v, pages.words, positions, q_start, block_table, weight_sums, out, error_flag)

@@ -40,7 +40,7 @@ def plain_attention(cache, q, q_start, positions, heads, window=None):
     for r in range(len(q_start) - 1):
         for t in range(q_start[r], q_start[r + 1]):
             last = min(int(positions[t]), columns * cache.page - 1)
-            j = torch.arange(0 if window is None else max(0, int(positions[t]) - window + 1), last + 1)
+            j = torch.arange(min(0 if window is None else max(0, int(positions[t]) - window + 1), last + 1), last + 1)
             j = j[(cache.table[r, j // cache.page] >= 0) & (cache.table[r, j // cache.page] < pages)]
             if not len(j):
                 continue
@@ -133,3 +133,24 @@ def test_keys_without_a_page_are_left_out(both_forms, dtype, heads, g, dim, page
     assert bool((got[q_start[2]:q_start[3]] == 0).all())
     both_forms += ["expects_unpacking"] * (dtype == torch.bfloat16 and dim != 24)
     check(c, q, pos, q_start, heads, window, sums=False, flag=BAD_PAGE)
+
+
+# ---- places outside the table ---------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim,n", [(64, 1), (128, 1), (24, 1), (64, 7), (24, 5), (64, 90), (128, 70)])
+@pytest.mark.parametrize("window", [None, 50])
+def test_places_outside_the_table(both_forms, dtype, dim, n, window):
+    """Rows at places that the table has no columns for, at the last place that there is and far before the first: what the table has
+    of their places is seen, the error word tells, and every walk ends with the table."""
+    c = Cache([112, 100, 60, 64, 112, 90], 2, dim, 16, seed=n)       # places 112 .. 127 have no page, 128 and on no column
+    ends = [140, 100, -150, 3, 2 ** 31, 90]
+    pos = torch.cat([torch.arange(end - n, end) for end in ends]).int()
+    q, q_start = torch.randn(6 * n, 4 * dim, generator=torch.Generator().manual_seed(dim)).to(dtype), [n * i for i in range(7)]
+    got = check(c, q, pos, q_start, 4, window, flag=BAD_PAGE)
+    assert bool((got[2 * n:3 * n] == 0).all())
+    check(c, q, pos, q_start, 4, window, sums=False, flag=BAD_PAGE)
+    both_forms += ["expects_unpacking"] * (dtype == torch.bfloat16 and dim != 24)
+    keep = torch.cat([torch.arange(n, 4 * n), torch.arange(5 * n, 6 * n)])       # without them no word is raised
+    c.table[[0, 4]] = c.table[[4, 0]]
+    check(c, q[keep], pos[keep], [0, 0, n, 2 * n, 3 * n, 3 * n, 4 * n], 4, window)

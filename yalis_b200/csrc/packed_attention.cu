@@ -23,6 +23,7 @@ struct AttentionParams {
   const int32_t* q_start;      // [R + 1]
   const int32_t* block_table;  // [R, table_width]
   int table_width, n_requests, n_tokens, nh, per, window;
+  int reach;                   // places that the table has
   float scale;
   float* lse2;                 // [N, nh] the logarithm to base two of a row's sum of exponentials, or null
   float* sums;                 // [pages, g, page_size] or null
@@ -65,14 +66,15 @@ __global__ void __launch_bounds__(kThreads) packed_attention_general_kernel(cons
   float part = 0.f;
   for (int i = tid; i < dim; i += kThreads) part += q[i] = to_f32<T>(src[i]);
   const float q_sum = block_sum(part, scratch);
-  const int last = p.positions[token], first = p.window > 0 ? max(0, last - p.window + 1) : 0;
+  const int place = p.positions[token], first = p.window > 0 ? max(0, place - p.window + 1) : 0, last = min(place, p.reach - 1);
+  if (place > last && tid == 0 && p.error) atomicOr(p.error, YALIS_FLAG_BAD_PAGE);       // (places behind the table have no page)
   const int32_t* table_row = p.block_table + (size_t)req * p.table_width;
   float m = -INFINITY, l = 0.f, acc[2] = {0.f, 0.f};
-  for (int j0 = first; j0 <= last; j0 += kThreads) {
-    const int j = j0 + tid;
+  for (long long j0 = first; j0 <= last; j0 += kThreads) {
+    const int j = (int)(j0 + tid), n = (int)min((long long)kThreads, last - j0 + 1);
     float score = -INFINITY, step = 0.f, z = 0.f;
     long long at = -1;
-    if (j <= last) {
+    if (tid < n) {
       int row;
       const int page = page_of(p.pages, table_row, p.table_width, j, row);
       if (page < 0) {
@@ -94,7 +96,6 @@ __global__ void __launch_bounds__(kThreads) packed_attention_general_kernel(cons
     zero[tid] = z;
     row_at[tid] = at;
     __syncthreads();
-    const int n = min(kThreads, last - j0 + 1);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int d = tid + h * kThreads;
@@ -167,6 +168,7 @@ bool params_of(AttentionParams& p, const void* q, long long q_stride, void* k_co
   p.q = q; p.q_stride = q_stride;
   p.positions = positions; p.q_start = q_start; p.block_table = block_table; p.table_width = table_width;
   p.n_requests = n_requests; p.nh = nh; p.per = nh / g; p.window = window; p.scale = scale;
+  p.reach = (int)min((long long)table_width * page_size, 0x7fffffffll);
   p.pages = packed_pages(k_codes, v_codes, words, num_pages, page_size, g, dim);
   return true;
 }

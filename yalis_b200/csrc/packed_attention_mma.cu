@@ -56,6 +56,7 @@ struct MmaParams {
   const int32_t* q_start;      // [R + 1]
   const int32_t* block_table;  // [R, table_width]
   int table_width, n_requests, nh, per, window;
+  int reach;                   // places that the table has
   int together;                // 2: a chunk never lies in two pages; 1: the rows that one copy instruction of a warp covers do not
   int q_vector;                // 1: rows of q start on 16-byte boundaries
   int only_single;             // 1: requests that bring more than one token are left to another kernel
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
     n_rows = 0;
     if (n <= 0 || (p.only_single && n > 1)) return 0;
     n_rows = n * p.per;
-    const int last = p.positions[t0 + n - 1], begin = p.positions[t0];
+    const int last = min(p.positions[t0 + n - 1], p.reach - 1), begin = p.positions[t0];
     first_key = p.window > 0 ? max(0, begin - p.window + 1) / kChunk * kChunk : 0;
     return max(1, last < first_key ? 1 : (last - first_key) / kChunk + 1);       // (rows that see nothing are written too)
   };
@@ -229,6 +230,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
     const int chunks = span_of(r, first_key, n_rows);
     cum_pairs[r + 1] = (n_rows + COLS - 1) / COLS * p.pages.g;
     cum[r + 1] = chunks;
+    // (places behind the table have no page)
+    if (n_rows > 0 && blockIdx.x == 0 && p.error && p.positions[p.q_start[r + 1] - 1] >= p.reach) atomicOr(p.error, YALIS_FLAG_BAD_PAGE);
   }
   if (threadIdx.x == 0) cum[0] = cum_pairs[0] = 0;
   __syncthreads();
@@ -333,6 +336,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
       any_hi = max(any_hi, __shfl_xor_sync(0xffffffffu, any_hi, o));
       any_lo = min(any_lo, __shfl_xor_sync(0xffffffffu, any_lo, o));
     }
+
+    any_hi = min(any_hi, p.reach - 1);
 
     // Chunks of this warp that any column sees: one in kWarps.
     int c = lo + warp, c_end = hi;
@@ -942,6 +947,7 @@ YALIS_API int yalis_packed_attention_mma(const void* q, long long q_stride, int 
   p.n_requests = n_requests; p.nh = nh; p.per = nh / g; p.window = window; p.q_vector = q_vector; p.only_single = only_single;
   p.together = page_size % kChunk == 0 ? 2 : page_size % (1024 / dim) == 0 ? 1 : 0;
   p.slots = blocks;
+  p.reach = (int)min((long long)table_width * page_size, 0x7fffffffll);
   const long long pairs = (long long)n_requests * g * ((max_rows + columns - 1) / columns), grid = pairs > blocks ? pairs : blocks;
   if (grid > 0x7fffffffll) return YALIS_ERR_SHAPE;
   p.scale_log2 = scale * 1.4426950408889634f; p.lse2 = lse2; p.scores = scores; p.score_stride = score_stride; p.part = scratch; p.tickets = tickets; p.error = error;

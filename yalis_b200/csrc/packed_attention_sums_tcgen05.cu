@@ -241,14 +241,14 @@ packed_sums_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
       bool ok = true;
       for (int i = first_tile; i < it.n_tiles; i += kGroups, ++mine) {
         const int t = it.t_lo + i * p.tokens_per_tile, n_tok = min(p.tokens_per_tile, it.t_hi - t);
+        const int place = it.begin + t, last_place = it.begin + (t + n_tok - 1);
         *reinterpret_cast<float4*>(&lse_s[warp][4 * lane]) = make_float4(lse[0], lse[1], lse[2], lse[3]);
         __syncwarp();
         if (i + kGroups < it.n_tiles) fetch(t + kGroups * p.tokens_per_tile);
         if (!warp_wait(&s_full[group], mine & 1, abort_flag, lane)) { ok = false; break; }
-        if (it.begin + t + n_tok - 1 >= key_lo) {  // (else no row of the tile sees a key of this warp)
+        if (last_place >= key_lo) {                // (else no row of the tile sees a key of this warp)
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const bool masked = n_tok < p.tokens_per_tile || it.begin + t < key_lo + 31 ||
-                              (p.window > 0 && it.begin + t + n_tok - 1 - p.window >= key_lo);
+          const bool masked = n_tok < p.tokens_per_tile || place < key_lo + 31 || (p.window > 0 && last_place - p.window >= key_lo);
           // Row c sees this lane's key if lowest <= token < beyond.
           const int lowest = key - it.begin - t, beyond = p.window > 0 ? (int)min((long long)n_tok, (long long)lowest + p.window) : n_tok;
           auto add = [&](const float (&s)[32], int c0) {

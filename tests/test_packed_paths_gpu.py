@@ -154,3 +154,22 @@ def test_places_outside_the_table(both_forms, dtype, dim, n, window):
     keep = torch.cat([torch.arange(n, 4 * n), torch.arange(5 * n, 6 * n)])       # without them no word is raised
     c.table[[0, 4]] = c.table[[4, 0]]
     check(c, q[keep], pos[keep], [0, 0, n, 2 * n, 3 * n, 3 * n, 4 * n], 4, window)
+
+
+# ---- eviction -------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("pools", [0, 1])
+def test_a_cut_without_rows_to_move(pools):
+    """No pools, or one whose rows have no bytes: the sums move all the same."""
+    from yalis_b200.ops.packed import evict_tokens
+    c = Cache([40, 9, 2000], 2, 8, 16)
+    total = c.sums.to(DEV)
+    kept = evict_tokens([torch.empty(c.k.shape[:3] + (0,), device=DEV)] * pools, total, i32(c.lengths), c.table.to(DEV), 12, 3)
+    for r, n in ((0, 40), (2, 2000)):
+        for h in range(2):
+            score = c.rows(r, n, c.sums)[:, h].clone()
+            score[n - 3:] = 2.0
+            j = torch.sort(torch.topk(score, 12).indices).values
+            assert torch.equal(kept[r, h].cpu().long(), j)
+            assert torch.equal(c.rows(r, 12, total.cpu())[:, h], c.rows(r, n, c.sums)[j, h])
+    assert torch.equal(c.rows(1, 9, total.cpu()), c.rows(1, 9, c.sums)) and kept[1, 0].tolist() == list(range(9)) + [-1] * 3

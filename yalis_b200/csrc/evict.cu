@@ -84,7 +84,7 @@ __device__ __forceinline__ void store_unit(unsigned char* at, int unit, uint4 v)
 template <int NP, int U, typename Kept>
 __device__ __forceinline__ void move_rows(const EvictParams& p, int p0, const Rows& rows, const Kept& kept, int first) {
   const int lane = threadIdx.x & (p.lanes - 1), group = threadIdx.x / p.lanes, groups = kThreads / p.lanes;
-  int widest = 0;                                             // pieces of a row that its lanes take in turn
+  int widest = p0 == 0;                                       // pieces of a row that its lanes take in turn (the sums move with the first)
 #pragma unroll
   for (int i = 0; i < NP; ++i) widest = max(widest, (p.row_bytes[p0 + i] + p.unit[p0 + i] * p.lanes - 1) / (p.unit[p0 + i] * p.lanes));
   for (int j0 = first; j0 < p.keep; j0 += groups * U) {

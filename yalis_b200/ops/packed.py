@@ -365,8 +365,8 @@ def evict_tokens(pools: Sequence[torch.Tensor], weight_sums: torch.Tensor, lengt
     Of a request of ``lengths[r]`` tokens (int32 [R], row r of the block table) that holds more than ``keep``, every KV head keeps
     the last ``recent`` and, of the others, the keep - recent with the largest ``weight_sums`` (float32
     [pages, kv_heads, page_size]; of equal ones the earlier, NaN last).  They move, in their order, to the places 0 .. keep - 1 of
-    the request's pages, in every tensor of ``pools`` (up to four, [pages, kv_heads, page_size, ...]: ``PackedPages.pools()``, or
-    the pools of keys and values of a plain cache) and in ``weight_sums``; what lies behind them stays as it was, and the pages
+    the request's pages, in every tensor of ``pools`` (up to four, or none, [pages, kv_heads, page_size, ...]: ``PackedPages.pools()``,
+    or the pools of keys and values of a plain cache) and in ``weight_sums``; what lies behind them stays as it was, and the pages
     there may be given back.  Requests of at most ``keep`` tokens, and requests with a token without a page (which raise the error
     word's bit), stay as they are.  The pages of the requests must differ.  Returns int32 [R, kv_heads, keep]: the place that each
     token had, ascending, -1 where there is none."""

@@ -173,3 +173,17 @@ def test_a_cut_without_rows_to_move(pools):
             assert torch.equal(kept[r, h].cpu().long(), j)
             assert torch.equal(c.rows(r, 12, total.cpu())[:, h], c.rows(r, n, c.sums)[j, h])
     assert torch.equal(c.rows(1, 9, total.cpu()), c.rows(1, 9, c.sums)) and kept[1, 0].tolist() == list(range(9)) + [-1] * 3
+
+
+# ---- bounds ---------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("brought", [[1, 1], [3, 2], [90, 90], [90, 1]])
+def test_generous_bounds(both_forms, brought):
+    """Bounds far above what a step brings and sees, past 32 bits too, and bounds that fit; none of keys where nothing is seen."""
+    c = Cache([200, 90], 2, 64, 16, seed=4)
+    q, pos, q_start = step_of(c, brought, heads=8)
+    for max_q_len in (max(brought), 5000, 1 << 31, 1 << 40):
+        for max_kv_len in (None, 200, 1 << 31, 1 << 50):
+            check(c, q, pos, q_start, 8, max_q_len=max_q_len, max_kv_len=max_kv_len)
+    both_forms += ["expects_unpacking"]
+    assert bool((check(c, q, torch.full_like(pos, -1), q_start, 8, max_kv_len=0) == 0).all())

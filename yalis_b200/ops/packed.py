@@ -300,8 +300,9 @@ def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tenso
     rows, columns = _check_index(name, n, block_table, positions)
     if q_start.dtype is not torch.int32 or q_start.dim() != 1 or not q_start.is_contiguous() or not 1 <= q_start.shape[0] <= rows + 1:
         raise KernelError(f"{name}: q_start must be int32 [R+1], and block_table have a row for every request")
-    if max_q_len < 0 or (window is not None and window <= 0):
-        raise KernelError(f"{name}: max_q_len and the window must be positive")
+    if max_q_len < 0 or (max_kv_len is not None and max_kv_len < 0) or (window is not None and window <= 0):
+        raise KernelError(f"{name}: max_q_len and max_kv_len must not be negative, and the window must be positive")
+    max_q_len = min(max_q_len, n)                       # (any bound will do)
     if scale is None:
         scale = dim ** -0.5
     elif not math.isfinite(scale):

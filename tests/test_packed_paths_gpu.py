@@ -175,6 +175,22 @@ def test_a_cut_without_rows_to_move(pools):
     assert torch.equal(c.rows(1, 9, total.cpu()), c.rows(1, 9, c.sums)) and kept[1, 0].tolist() == list(range(9)) + [-1] * 3
 
 
+@pytest.mark.parametrize("n,keep,recent", [(24577, 11000, 40), (30000, 25000, 0), (26000, 30, 30)])
+def test_a_cut_of_more_tokens_than_shared_memory_has_keys_for(n, keep, recent):
+    from yalis_b200.ops.packed import evict_tokens
+    c = Cache([n, 0], 1, 8, 64)                                      # (its words are filled row by row: one head)
+    c.sums[torch.rand(c.sums.shape, generator=torch.Generator().manual_seed(1)) < 0.3] = 0.25       # ties
+    pages, table = c.to(DEV)
+    total = c.sums.to(DEV)
+    kept = evict_tokens(pages.pools(), total, i32(c.lengths), table, keep, recent)
+    score = c.rows(0, n, c.sums)[:, 0].clone()
+    score[n - recent:] = 2.0
+    j = torch.sort(torch.sort(score, descending=True, stable=True).indices[:keep]).values
+    assert torch.equal(kept[0, 0].cpu().long(), j)
+    for before, after in zip((c.k, c.v, c.words, c.sums), pages.pools() + (total,)):
+        assert torch.equal(c.rows(0, keep, after.cpu()), c.rows(0, n, before)[j])
+
+
 # ---- bounds ---------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("brought", [[1, 1], [3, 2], [90, 90], [90, 1]])
@@ -187,3 +203,148 @@ def test_generous_bounds(both_forms, brought):
             check(c, q, pos, q_start, 8, max_q_len=max_q_len, max_kv_len=max_kv_len)
     both_forms += ["expects_unpacking"]
     assert bool((check(c, q, torch.full_like(pos, -1), q_start, 8, max_kv_len=0) == 0).all())
+
+
+# ---- how the work is divided ----------------------------------------------------------------------------------------
+
+def deal(slots, pairs, most, total):
+    """What the codes' kernel's ``choose_deal`` answers: pieces of a pair, 0 where chunks go out in equal shares."""
+    if pairs > slots:
+        return 1
+    even = total // min(slots, -(-total // 8)) + 64
+    k = max(1, min(slots // pairs, -(-most // 8)))
+    return k if -(-most // k) + (32 if k > 1 else 0) <= even else 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lengths,g,brought,dim,expected", [
+    ([12000] + [40] * 60, 2, 1, 64, 0),                    # equal shares: one long request among short ones
+    ([9000, 5, 4000, 64] + [33] * 40, 3, 1, 128, 0),
+    ([30, 6000, 31] * 3 + [3] * 30, 2, 4, 64, 0),          # ... with two blocks of columns a pair
+    ([100, 3, 40, 257] * 30, 6, 1, 64, 1),                 # more pairs than blocks: whole pairs
+    ([9, 130] * 45, 4, 5, 128, 1)])
+def test_shares_of_unequal_requests(monkeypatch, dtype, lengths, g, brought, dim, expected):
+    from yalis_b200.ops import packed
+    names = launches(monkeypatch)
+    monkeypatch.setattr(packed, "UNPACK_ROWS", 1 << 20)
+    c, heads = Cache(lengths, g, dim, 64, seed=len(lengths)), 4 * g
+    bring = [min(brought, n) for n in lengths]
+    rows = 4 * max(bring)
+    tile = 8 if dtype == torch.float32 or rows <= 8 else 16
+    pairs = [g * -(-4 * b // tile) for b in bring]
+    chunks = [-(-n // 32) for n in lengths]
+    slots = torch.cuda.get_device_properties(0).multi_processor_count * (4 if dtype == torch.bfloat16 and tile == 8 else 2)
+    assert deal(slots, sum(pairs), max(chunks), sum(a * b for a, b in zip(pairs, chunks))) == expected
+    q, pos, q_start = step_of(c, bring, dtype=dtype, heads=heads)
+    check(c, q, pos, q_start, heads)
+    assert names.count("yalis_packed_attention_mma") == 1 and "yalis_packed_unpack" not in names
+    check(c, q, pos, q_start, heads, sums=False)
+
+
+@pytest.mark.parametrize("heads,g,dim,window", [(8, 2, 64, None), (4, 1, 128, None), (8, 2, 64, 700)])
+@pytest.mark.parametrize("portions", [[600, 1, 1], [600, 0, 300]])
+def test_portions_that_see_thousands_of_keys(monkeypatch, heads, g, dim, window, portions):
+    """Keys of a tile of queries in shares (without a window), several parts of an item's rows in the sums, single tokens beside them."""
+    from yalis_b200.ops import packed
+    names = launches(monkeypatch, forced=True)
+    chosen, splits = [], packed._portion_splits
+    monkeypatch.setattr(packed, "_portion_splits", lambda *a: chosen.append(splits(*a)) or chosen[-1])
+    c = Cache([4500, 900, 3700], g, dim, 64, seed=dim)
+    q, pos, q_start = step_of(c, portions, heads=heads)
+    check(c, q, pos, q_start, heads, window)
+    assert "yalis_packed_unpack" in names and "yalis_packed_sums_tcgen05" in names
+    assert window is not None or chosen[0][0] > 1
+    assert -(-600 // (128 // (heads // g))) > 16           # tiles of the longest portion: more than a part has
+
+
+@pytest.mark.parametrize("heads,g,dim", [(8, 2, 64), (4, 1, 128)])
+def test_marks_where_keys_are_shared_out(monkeypatch, heads, g, dim):
+    """A value without numbers in the last share and missing pages in others, one of them a whole share's."""
+    from yalis_b200.ops import packed
+    launches(monkeypatch, forced=True)
+    chosen, splits = [], packed._portion_splits
+    monkeypatch.setattr(packed, "_portion_splits", lambda *a: chosen.append(splits(*a)) or chosen[-1])
+    c = Cache([4500, 900, 3700], g, dim, 64, seed=dim)
+    c.words[int(c.table[0, 4100 // 64]), 0, 4100 % 64, 1] = NAN_WORD
+    c.table[0, 5], c.table[2, :30], c.table[2, 40] = -1, -1, c.k.shape[0]
+    q, pos, q_start = step_of(c, [600, 1, 300], heads=heads)
+    got = check(c, q, pos, q_start, heads, flag=BAD_PAGE)
+    assert chosen[0][0] > 1
+    assert not bool(got[:200].isnan().any()) and bool(got[200:600, :dim].isnan().all()) and not bool(got[600:].isnan().any())
+
+
+def test_a_replayed_portion_follows_its_values():
+    """A recording made without marks meets a value without numbers, a missing page and neither again."""
+    from yalis_b200.ops.packed import packed_attention
+    c = Cache([300, 80], 2, 64, 16, seed=1)
+    pages, table = c.to(DEV)
+    q, pos, q_start = step_of(c, [300, 80], heads=8)
+    arguments = (q.to(DEV), pages, pos.to(DEV), i32(q_start), table, 300, 8)
+    with pytest.MonkeyPatch.context() as patch:
+        names = launches(patch, forced=True)
+        packed_attention(*arguments)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = packed_attention(*arguments)
+    assert names.count("yalis_packed_unpack") == 2
+    at, word, page = (int(c.table[0, 9]), 1, 5, 1), c.words[int(c.table[0, 9]), 1, 5, 1].clone(), int(c.table[1, 2])
+    whole = None
+    for none, missing in ((False, False), (True, False), (False, True), (True, True), (False, False)):
+        c.words[at] = NAN_WORD if none else word
+        c.table[1, 2] = -1 if missing else page
+        pages.words.copy_(c.words)
+        table.copy_(c.table)
+        graph.replay()
+        torch.cuda.synchronize()
+        ref, _, size, slack, _ = plain_attention(c, q, q_start, pos, 8)
+        y = out.cpu().double()
+        assert torch.equal(y.isnan(), ref.isnan()) and bool(ref.isnan().any()) == none
+        off = (y - ref).abs() / (2.0 ** -8 * ref.abs() + (2.0 ** -8 + 2 * slack + 300 * 2.0 ** -24) * size + 1e-30)
+        assert bool((off[~ref.isnan()] <= 1).all())
+        if not (none or missing):
+            assert whole is None or torch.equal(out, whole)            # the same bits as before there were marks
+            whole = out.clone()
+
+
+def test_groups_of_requests(monkeypatch):
+    """Pools for fewer requests at a time than the step has, sums and single tokens included."""
+    from yalis_b200.ops import packed
+    names = launches(monkeypatch, forced=True)
+    c = Cache([500, 70, 300, 1, 640, 33, 128], 2, 64, 16, seed=3)
+    for brought in ([90, 70, 0, 1, 200, 1, 128], [90, 70, 300, 1, 200, 33, 100]):
+        q, pos, q_start = step_of(c, brought, heads=8)
+        for bytes_held in (1, 3 * 4 * 11 * 2 * 64 * 64):
+            monkeypatch.setattr(packed, "UNPACK_BYTES", bytes_held)
+            del names[:]
+            check(c, q, pos, q_start, 8)
+            check(c, q, pos, q_start, 8, sums=False, max_kv_len=660)
+            assert names.count("yalis_packed_unpack") > 4
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim,window", [(64, None), (128, 90)])
+@pytest.mark.parametrize("brought", [[1, 1, 1], [3, 1, 2], [120, 1, 1]])
+def test_sums_without_room_for_scores(monkeypatch, dtype, dim, window, brought):
+    """Steps of few rows whose scores would take too much memory: their products are taken once more."""
+    from yalis_b200.ops import packed
+    names = launches(monkeypatch, forced=max(brought) > 3)
+    monkeypatch.setattr(packed, "SCORE_BYTES", 1000)
+    c = Cache([700, 90, 257], 2, dim, 16, seed=dim)
+    q, pos, q_start = step_of(c, brought, dtype=dtype, heads=8)
+    check(c, q, pos, q_start, 8, window)
+    assert "yalis_packed_sums_of_scores" not in names and "yalis_packed_weight_sums" in names
+
+
+def test_the_same_bits_however_the_work_is_divided_from_run_to_run(monkeypatch):
+    from yalis_b200.ops.packed import packed_attention
+    launches(monkeypatch, forced=True)
+    for lengths, brought in (([12000] + [40] * 60, [1] * 61), ([4500, 900, 3700], [600, 1, 300])):
+        c = Cache(lengths, 2, 64, 64, seed=9)
+        pages, table = c.to(DEV)
+        q, pos, q_start = step_of(c, brought, heads=8)
+        runs = []
+        for _ in range(3):
+            sums = c.sums.to(DEV)
+            runs.append((packed_attention(q.to(DEV), pages, pos.to(DEV), i32(q_start), table, max(brought), 8, weight_sums=sums), sums))
+        assert all(torch.equal(a, b) for r in runs[1:] for a, b in zip(runs[0], r))

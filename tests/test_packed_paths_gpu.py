@@ -191,6 +191,37 @@ def test_a_cut_of_more_tokens_than_shared_memory_has_keys_for(n, keep, recent):
         assert torch.equal(c.rows(0, keep, after.cpu()), c.rows(0, n, before)[j])
 
 
+def test_tokens_behind_a_cut_start_from_zero_where_the_caller_says_so():
+    """A place that is written again keeps the sum that stood there: set to zero first, its new token is ranked by its own weights."""
+    from yalis_b200.ops.packed import PackedPages, evict_tokens, packed_attention, packed_kv_write
+    heads, g, dim, page, keep = 4, 2, 64, 16, 20
+    gen = torch.Generator().manual_seed(5)
+    pages, table = PackedPages.empty(4, g, page, dim, DEV), i32([[2, 0, 3, 1]])
+    c, sums = Cache([60], g, dim, page, spare=0), torch.zeros(4, g, page, device=DEV)
+    c.table = table.cpu()
+    counted = torch.zeros(4, g, page).double()
+
+    def step(n, at):
+        nonlocal counted
+        qkv = torch.randn(n, (heads + 2 * g) * dim, generator=gen).bfloat16().to(DEV)
+        places = torch.arange(at, at + n, dtype=torch.int32, device=DEV)
+        sums[table[0, places // page].long(), :, (places % page).long()] = 0.0
+        packed_kv_write(qkv[:, heads * dim:(heads + g) * dim], qkv[:, (heads + g) * dim:], pages, places, torch.zeros_like(places), table)
+        packed_attention(qkv, pages, places, i32([0, n]), table, n, heads, weight_sums=sums)
+        c.k, c.v, c.words = (t.cpu() for t in pages.pools())
+        for j in range(at, at + n):
+            counted[int(c.table[0, j // page]), :, j % page] = 0
+        counted += plain_attention(c, qkv.cpu(), [0, n], places.cpu(), heads)[1]
+
+    step(60, 0)
+    evict_tokens(pages.pools(), sums, i32([60]), table, keep, 4)
+    counted = sums.cpu().double()
+    step(7, keep)
+    torch.testing.assert_close(c.rows(0, keep + 7, sums.cpu()).double(), c.rows(0, keep + 7, counted), rtol=1e-4, atol=1e-6)
+    assert bool((c.rows(0, keep + 7, sums.cpu())[keep:].sum(0) <= 7 * heads // g).all())
+
+
+
 # ---- bounds ---------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("brought", [[1, 1], [3, 2], [90, 90], [90, 1]])

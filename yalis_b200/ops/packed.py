@@ -280,10 +280,14 @@ def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tenso
     nothing was evicted: after ``evict_tokens`` a row sees by its place and was rotated by its position.  ``max_q_len`` bounds the
     rows of a request, ``max_kv_len`` the places seen (the block table's width bounds them otherwise).  ``weight_sums`` float32
     [pages, kv_heads, page_size]: the softmax weight that a token received, summed over the step's rows and the heads of the KV
-    head, is added to it (pages of different requests must differ then).  The result is [N, heads * head_dim] in q's dtype
+    head, is added to it (pages of different requests must differ then).  It is never reset: a place that is written anew (in a page
+    taken again, behind a cut) has the sum of the token that stood there until the caller sets it to zero.  The result is [N, heads * head_dim] in q's dtype
     (``out`` may be a column block of a wider matrix); rows that see nothing are zeros, rows of no request stay as they are.  Places
     without a page are left out, as if the row did not see them, and raise the error word's bit.
-    Scores, weights and sums are float32, and with float32 queries so is every product."""
+    Scores, exponentials, normalisers and sums are float32, and with float32 queries so is every product.  With bfloat16 queries a weight
+    is rounded where it meets the value: times the value's step to float16's eleven bits, relative to the row's largest such product,
+    where codes are multiplied as they are (there, of a query what lies below 2^-28 of its row's largest is lost, and one of 2^119 or
+    more gives NaN); to bfloat16 in portions whose rows are unpacked, or with a window to two bfloat16 parts."""
     name = "packed_attention"
     device = _need_here(name, q, pages.k, pages.v, pages.words, positions, q_start, block_table, weight_sums, out, error_flag)
     held = _pages_arguments(name, pages)
@@ -368,9 +372,11 @@ def evict_tokens(pools: Sequence[torch.Tensor], weight_sums: torch.Tensor, lengt
     [pages, kv_heads, page_size]; of equal ones the earlier, NaN last).  They move, in their order, to the places 0 .. keep - 1 of
     the request's pages, in every tensor of ``pools`` (up to four, or none, [pages, kv_heads, page_size, ...]: ``PackedPages.pools()``,
     or the pools of keys and values of a plain cache) and in ``weight_sums``; what lies behind them stays as it was, and the pages
-    there may be given back.  Requests of at most ``keep`` tokens, and requests with a token without a page (which raise the error
-    word's bit), stay as they are.  The pages of the requests must differ.  Returns int32 [R, kv_heads, keep]: the place that each
-    token had, ascending, -1 where there is none."""
+    there may be given back.  That holds for the sums as well: before the weights of tokens behind the cut are counted, the caller sets
+    the sums of their places to zero (``weight_sums[block_table[r, place // page_size], :, place % page_size] = 0``), or they start
+    with those of the tokens that stood there.  Requests of at most ``keep`` tokens, and requests with a token without a page (which
+    raise the error word's bit), stay as they are.  The pages of the requests must differ.  Returns int32 [R, kv_heads, keep]: the
+    place that each token had, ascending, -1 where there is none."""
     name = "evict_tokens"
     pools = tuple(pools)
     device = _need_here(name, *pools, weight_sums, lengths, block_table, error_flag)

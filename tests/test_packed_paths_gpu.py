@@ -367,6 +367,20 @@ def test_sums_without_room_for_scores(monkeypatch, dtype, dim, window, brought):
     assert "yalis_packed_sums_of_scores" not in names and "yalis_packed_weight_sums" in names
 
 
+@pytest.mark.parametrize("heads,g,dim,window", [(8, 2, 64, None), (12, 1, 128, 60)])
+def test_scores_of_single_tokens_beside_a_portion(monkeypatch, heads, g, dim, window):
+    """Room for the single tokens' scores is enough, however many rows the portion has."""
+    from yalis_b200.ops import packed
+    names = launches(monkeypatch, forced=True)
+    c = Cache([70, 400, 1, 257, 300], g, dim, 16, seed=dim)
+    monkeypatch.setattr(packed, "SCORE_BYTES", 4 * 5 * heads * 401)
+    for brought in ([1, 350, 1, 0, 1], [1, 1, 1, 257, 300]):
+        q, pos, q_start = step_of(c, brought, heads=heads)
+        del names[:]
+        check(c, q, pos, q_start, heads, window, max_kv_len=400)
+        assert "yalis_packed_unpack" in names and "yalis_packed_sums_of_scores" in names and "yalis_packed_weight_sums" not in names
+
+
 def test_the_same_bits_however_the_work_is_divided_from_run_to_run(monkeypatch):
     from yalis_b200.ops.packed import packed_attention
     launches(monkeypatch, forced=True)

@@ -63,7 +63,8 @@ struct MmaParams {
   int slots;                   // blocks resident at once; the launch has as many, or one for every pair
   float scale_log2;
   float* lse2;                 // [N, nh] the logarithm to base two of a row's sum of exponentials, or null
-  float* scores;               // [N, nh, score_stride] every score in powers of two, by place (those that some row of the pair sees), or null
+  float* scores;               // [N, nh, score_stride] every score in powers of two, by place (those that some row of the pair sees), or
+                               // null; with only_single [R, nh, score_stride], a request's row
   long long score_stride;
   float* part;                 // [blocks, 2, MT * 32 * 4 + 16 NT * 2]
   int32_t* tickets;            // one per pair, zero before and after
@@ -309,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
     }
 
     // ---- columns: the keys that each sees ----
-    const int tok0 = p.q_start[req];
+    const int tok0 = p.q_start[req], score_row0 = p.only_single ? req : tok0;
     const int32_t* table_row = p.block_table + (size_t)req * p.table_width;
     int see_hi[NT][2], see_lo[NT][2], all_hi = 0x7fffffff, all_lo = 0, any_hi = -1, any_lo = 0x7fffffff;
 #pragma unroll
@@ -573,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && PARTS == 1 ? 4 : 2) packe
             for (int x = 0; x < 2; ++x) {
               const int column = column0 + nt * 8 + 2 * t + x;
               if (column >= n_rows) continue;
-              float* to = p.scores + ((size_t)(tok0 + column / p.per) * p.nh + kvh * p.per + column % p.per) * p.score_stride + key0;
+              float* to = p.scores + ((size_t)(score_row0 + column / p.per) * p.nh + kvh * p.per + column % p.per) * p.score_stride + key0;
 #pragma unroll
               for (int half = 0; half < 2; ++half)
 #pragma unroll

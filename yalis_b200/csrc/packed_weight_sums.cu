@@ -251,18 +251,21 @@ int launch_sums(const SumsParams& p, int n_requests, int max_kv_len, cudaStream_
   return yalis_launch(packed_weight_sums_kernel<T, DIM, PARTS, 2, 4, 64 / (PARTS == 1 ? 1 : 2)>, grid, dim3(kThreads), 0, stream, p);
 }
 
-// From scores: a thread per key of a KV head, over the rows that see it in their order.
+// From scores: a thread per key of a KV head, over the rows that see it in their order.  SINGLE: only of requests that bring one token, with a
+// row of scores a request.
+template <bool SINGLE>
 __global__ void __launch_bounds__(256) packed_sums_of_scores_kernel(const SumsParams p, const float* scores, long long stride) {
   pdl_launch_dependents();
   pdl_wait();
   const int key = blockIdx.x * 256 + threadIdx.x, kvh = blockIdx.y, req = blockIdx.z;
   const int tok0 = p.q_start[req], n = p.q_start[req + 1] - tok0;
-  if (n <= 0 || (p.only_single && n > 1)) return;
+  if (n <= 0 || (SINGLE && n > 1)) return;
   const int last = p.positions[tok0 + n - 1], begin = p.positions[tok0];
   if (key >= stride || key > last || (p.window > 0 && key <= begin - p.window)) return;
-  int row;
-  const int page = page_of(p.pages, p.block_table + (size_t)req * p.table_width, p.table_width, key, row);
+  int in_page;
+  const int page = page_of(p.pages, p.block_table + (size_t)req * p.table_width, p.table_width, key, in_page);
   if (page < 0) return;
+  if constexpr (SINGLE) scores += ((long long)req - tok0) * p.nh * stride;
   float total = 0.f;
   for (int t = 0; t < n; ++t) {
     const int place = p.positions[tok0 + t];
@@ -276,7 +279,7 @@ __global__ void __launch_bounds__(256) packed_sums_of_scores_kernel(const SumsPa
       for (int i = 0; i < 4; ++i) total += exp2f(x[i]);
     }
   }
-  atomicAdd(p.sums + row_index(p.pages, page, kvh, row), total);
+  atomicAdd(p.sums + row_index(p.pages, page, kvh, in_page), total);
 }
 
 }  // namespace
@@ -314,7 +317,8 @@ YALIS_API int yalis_packed_weight_sums(const void* q, long long q_stride, int dt
   return YALIS_ERR_DTYPE;
 }
 
-// The same from scores [N, nh, score_stride] that the attention of the step left (yalis_packed_attention_mma).
+// The same from scores [N, nh, score_stride] ([R, nh, score_stride] of single tokens beside others) that the attention of the step left
+// (yalis_packed_attention_mma).
 YALIS_API int yalis_packed_sums_of_scores(float* scores, long long score_stride, int num_pages, int page_size, int g, int dim,
                                           const int32_t* positions, const int32_t* q_start, const int32_t* block_table, int table_width,
                                           int n_requests, int max_kv_len, int nh, int window, int only_single, float* lse2, float* sums,
@@ -323,8 +327,8 @@ YALIS_API int yalis_packed_sums_of_scores(float* scores, long long score_stride,
   if (n_requests <= 0 || max_kv_len <= 0) return YALIS_OK;
   const SumsParams p = params_of(nullptr, 0, num_pages, page_size, g, dim, positions, q_start, block_table, table_width, nh, 1.f, window, only_single,
                                  lse2, sums);
-  return yalis_launch(packed_sums_of_scores_kernel, dim3((unsigned)((max_kv_len + 255LL) / 256), g, n_requests), dim3(256), 0, stream, p, (const float*)scores,
-                      score_stride);
+  return yalis_launch(only_single ? packed_sums_of_scores_kernel<true> : packed_sums_of_scores_kernel<false>,
+                      dim3((unsigned)((max_kv_len + 255LL) / 256), g, n_requests), dim3(256), 0, stream, p, (const float*)scores, score_stride);
 }
 
 YALIS_SLOTS(yalis_packed_weight_sums)

@@ -211,7 +211,7 @@ _LONGEST = (1 << 31) - 1   # places are 32-bit numbers
 # heads: 64 rows 150 / 160, 128 rows 284 / 150; of 1,000: 64 rows 34 / 40, 128 rows 65 / 39; one of 1,000: 256 rows 18 / 28.
 UNPACK_ROWS, UNPACK_FEW = 64, 1 << 21
 UNPACK_PAGE = 64          # keys of a page of the unpacked pools
-UNPACK_BYTES = 2 << 30    # of unpacked keys and values at a time
+UNPACK_BYTES = 2 << 30    # of unpacked keys and values at a time (one request may take more)
 _unpackings = itertools.count(1)       # numbers by which a launch tells its own note that keys are marked from what the memory held before
 SCORE_BYTES = 1 << 30     # of scores that a step of few rows may leave for its sums; beyond, the products are taken once more
 
@@ -338,8 +338,9 @@ def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tenso
     if mma and (single or not unpack):
         q_rows = per if single else max_q_len * per
         tile = 8 if code == F32 or q_rows <= 8 else 16
-        if lse2 is not None and q_rows <= 16 and 4 * n * num_heads * max_kv_len <= SCORE_BYTES:
-            scores = torch.empty(n * num_heads * max_kv_len, dtype=torch.float32, device=device)
+        n_scores = (r if single else n) * num_heads * max_kv_len               # (of the rows that this launch takes)
+        if lse2 is not None and q_rows <= 16 and 4 * n_scores <= SCORE_BYTES:
+            scores = torch.empty(n_scores, dtype=torch.float32, device=device)
         blocks, floats = _mma_launch(device, code, dim, tile)
         counters, scratch = _workspace(device, raw, blocks, floats)
         check(_entry("yalis_packed_attention_mma", "plipl" + "pppiiii" + "pppii" + "iiiifippliipppp")(

@@ -78,7 +78,8 @@ struct PrefillParams {
   float* part_o;               // [N, nh, n_splits, HS]
   float* part_ml;              // [N, nh, n_splits, 2]
   float* lse2;                 // [N, nh] the logarithm to base two of a row's sum of exponentials, or null
-  const unsigned char* marks;  // [pages, g, 64] of unpacked keys (packed_rows.cu), else null: bit 0 where a value holds no numbers, 1 without a page
+  const uint32_t* marks;       // [pages, g, 2048 / HS] of unpacked keys (packed_rows.cu), else null: bit 0 where a value holds no numbers,
+                               // bit 1 where there is no page
   const int32_t* some_marked;  // `marked_by` if any key is marked (if none is, anything else, as a rule)
   int marked_by;
   int32_t* error;
@@ -553,14 +554,15 @@ prefill_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, cons
             for (int c = 0; c < BN; ++c)
               if (!valid || key0 + c > pos_row || (GEN && key0 + c < lo_row)) sv[c] = -INFINITY;
             if constexpr (MARKED) {
-              const uint32_t* mark = reinterpret_cast<const uint32_t*>(p.marks + ((size_t)(descs[d].page_first + j) * p.g + kvh) * BN);
+              constexpr int kWords = 2048 / HS;               // key i + kWords j has byte j of word i
+              const uint32_t* mark = p.marks + ((size_t)(descs[d].page_first + j) * p.g + kvh) * kWords;
 #pragma unroll
-              for (int c = 0; c < BN; c += 4) {
-                const uint32_t four = mark[c / 4];
+              for (int i = 0; i < kWords; ++i) {
+                const uint32_t word = mark[i];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  if (four >> (8 * i) & 2u) sv[c + i] = -INFINITY;
-                  sees_none |= (four >> (8 * i) & 1u) && sv[c + i] != -INFINITY;
+                for (int c = i; c < BN; c += kWords) {
+                  if (word >> (8 * (c / kWords)) & 2u) sv[c] = -INFINITY;
+                  sees_none |= (word >> (8 * (c / kWords)) & 1u) && sv[c] != -INFINITY;
                 }
               }
             }
@@ -993,8 +995,8 @@ YALIS_API int yalis_prefill_attention_tcgen05_general(
 // request's pages one after the other, `marks` of their keys): a window (0: none, else without shares of the keys), rows of no request
 // left alone, and `lse2` [N, nh] or null.  Otherwise as above.
 YALIS_API int yalis_prefill_attention_tcgen05_unpacked(
-    const void* q, long long q_stride, void* out, long long out_stride, const void* k_pool, const void* v_pool, const void* marks, const int32_t* some_marked, int marked_by,
-    const int32_t* positions, const int32_t* q_start, const int32_t* block_table, int table_width, int page_size, int num_pages, int n_tokens, int n_requests,
+    const void* q, long long q_stride, void* out, long long out_stride, const void* k_pool, const void* v_pool, const void* marks,
+    const int32_t* some_marked, int marked_by, const int32_t* positions, const int32_t* q_start, const int32_t* block_table, int table_width, int page_size, int num_pages, int n_tokens, int n_requests,
     int max_q_len, int nh, int g, int hs, float scale, int window, int n_splits, int tiles_per_split, int skip_single, float* lse2,
     float* scratch, int32_t* work, int32_t* error, cudaStream_t stream) {
   if (n_tokens <= 0 || n_requests <= 0) return YALIS_OK;
@@ -1020,7 +1022,7 @@ YALIS_API int yalis_prefill_attention_tcgen05_unpacked(
   p.part_ml = scratch ? scratch + (size_t)n_tokens * nh * n_splits * hs : nullptr;
   p.lse2 = lse2;
   p.error = error;
-  p.marks = static_cast<const unsigned char*>(marks); p.some_marked = some_marked; p.marked_by = marked_by;
+  p.marks = static_cast<const uint32_t*>(marks); p.some_marked = some_marked; p.marked_by = marked_by;
   p.window = window; p.out_scale = 1.f;
   return window > 0 ? launch_prefill<true, true>(p, q, (int)q_stride, k_pool, v_pool, n_tokens, hs, 1, stream)
                     : launch_prefill<false, true>(p, q, (int)q_stride, k_pool, v_pool, n_tokens, hs, n_splits, stream);

@@ -237,7 +237,8 @@ constexpr int kUnpackPage = 64, kUnpackThreads = 256;
 struct UnpackParams {
   __nv_bfloat16* k_out;        // [R * width, g, kUnpackPage, dim]
   __nv_bfloat16* v_out;
-  unsigned char* marks;        // [R * width, g, kUnpackPage] of each key: bit 0 where its value holds no numbers, bit 1 where it has no page
+  uint32_t* marks;             // [R * width, g, 2048 / dim]: of key i + (2048 / dim) j of a page in byte j of word i; bit 0 where its
+                               // value holds no numbers, bit 1 where it has no page
   int32_t* some_marked;        // becomes `marked_by`, a number of this launch's own, if any key is marked
   int marked_by;
   int32_t* table_out;          // [R, width]
@@ -297,8 +298,8 @@ __global__ void __launch_bounds__(kUnpackThreads, 4) packed_unpack_kernel(const 
       const int index = first / kUnpackPage + local / p.pages.g, kvh = local % p.pages.g, key0 = index * kUnpackPage;
       const size_t to = (((size_t)req * p.width + index) * p.pages.g + kvh) * kUnpackPage;
       const int32_t* table_row = p.block_table + (size_t)req * p.table_width;
-      const int rows = own < per_round ? min(kUnpackPage, last - key0 + 1) : 0;
-      for (int q = own; q < rows; q += 4 * per_round) {
+      const int rows = min(kUnpackPage, last - key0 + 1), q = own;        // (four rounds are a page, or two)
+      if (q < rows) {
         long long at[4];
         uint32_t word[4], kc[4], vc[4];
 #pragma unroll
@@ -319,6 +320,7 @@ __global__ void __launch_bounds__(kUnpackThreads, 4) packed_unpack_kernel(const 
           kc[j] = p.pages.k[at[j] * words + w];
           vc[j] = p.pages.v[at[j] * words + w];
         }
+        uint32_t marked = 0u;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int r = q + j * per_round;
@@ -326,8 +328,11 @@ __global__ void __launch_bounds__(kUnpackThreads, 4) packed_unpack_kernel(const 
           const bool none = (word[j] >> 16 & 0x7F80u) == 0x7F80u;
           reinterpret_cast<uint4*>(p.k_out)[(to + r) * words + w] = unpack_bf16(kc[j], word[j] & 0xFFFFu);
           reinterpret_cast<uint4*>(p.v_out)[(to + r) * words + w] = unpack_bf16(vc[j], none ? 0u : word[j] >> 16);
-          if (w == 0) p.marks[to + r] = (none ? 1 : 0) | (at[j] < 0 ? 2 : 0);
-          if (none || at[j] < 0) *p.some_marked = p.marked_by;
+          marked |= ((none ? 1u : 0u) | (at[j] < 0 ? 2u : 0u)) << (8 * j);
+        }
+        if (w == 0) {
+          p.marks[to / kUnpackPage * per_round + q] = marked;
+          if (marked) *p.some_marked = p.marked_by;
         }
       }
     }
@@ -361,11 +366,11 @@ YALIS_API int yalis_packed_unpack(void* k_codes, void* v_codes, void* words, int
                                   const int32_t* q_start, const int32_t* block_table, int table_width, int n_requests, int width, int window,
                                   int skip_single, void* k_out, void* v_out, void* marks, int32_t* some_marked, int marked_by,
                                   int32_t* table_out, int32_t* zeroed, int n_zeroed, int32_t* error, cudaStream_t stream) {
-  if (dim < 8 || dim > 256 || dim % 8 || page_size < 1 || g < 1 || width < 1) return YALIS_ERR_SHAPE;
+  if ((dim != 64 && dim != 128) || page_size < 1 || g < 1 || width < 1) return YALIS_ERR_SHAPE;
   if (n_requests <= 0) return YALIS_OK;
   UnpackParams p = {};
   p.n_zeroed = n_zeroed;
-  p.k_out = static_cast<__nv_bfloat16*>(k_out); p.v_out = static_cast<__nv_bfloat16*>(v_out); p.marks = static_cast<unsigned char*>(marks);
+  p.k_out = static_cast<__nv_bfloat16*>(k_out); p.v_out = static_cast<__nv_bfloat16*>(v_out); p.marks = static_cast<uint32_t*>(marks);
   p.some_marked = some_marked; p.marked_by = marked_by; p.table_out = table_out; p.zeroed = zeroed;
   p.positions = positions; p.q_start = q_start; p.block_table = block_table; p.table_width = table_width; p.n_requests = n_requests;
   p.width = width; p.window = window; p.skip_single = skip_single; p.error = error;

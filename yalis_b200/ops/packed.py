@@ -246,13 +246,13 @@ def _attend_unpacked(name, device, rows, held, at, n, max_q_len, max_kv_len, num
     pools = torch.empty(2 * group * size, dtype=torch.bfloat16, device=device)
     n_counters = (3 + 4 * items + 3) // 4 * 4
     pages = group * width
-    work = torch.empty(floats + items * parts * 384 + n_counters + pages * (1 + g * UNPACK_PAGE // 4) + 1, dtype=torch.int32, device=device)
+    work = torch.empty(floats + items * parts * 384 + n_counters + pages * (1 + g * 2048 // dim) + 1, dtype=torch.int32, device=device)
     k_at, scratch = pools.data_ptr(), work.data_ptr()
     v_at, partial = k_at + 2 * group * size, scratch + 4 * floats
     counters = partial + 4 * items * parts * 384
     table_at = counters + 4 * n_counters
     marks_at = table_at + 4 * pages
-    some_marked_at, marked_by = marks_at + pages * g * UNPACK_PAGE, next(_unpackings) & 0x7FFFFFFF
+    some_marked_at, marked_by = marks_at + pages * g * 8192 // dim, next(_unpackings) & 0x7FFFFFFF
     for first in range(0, r, group):
         m = min(group, r - first)
         starts, row = q_start + 4 * first, table + 4 * first * table_width

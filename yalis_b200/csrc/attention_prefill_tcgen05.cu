@@ -996,9 +996,9 @@ YALIS_API int yalis_prefill_attention_tcgen05_general(
 // left alone, and `lse2` [N, nh] or null.  Otherwise as above.
 YALIS_API int yalis_prefill_attention_tcgen05_unpacked(
     const void* q, long long q_stride, void* out, long long out_stride, const void* k_pool, const void* v_pool, const void* marks,
-    const int32_t* some_marked, int marked_by, const int32_t* positions, const int32_t* q_start, const int32_t* block_table, int table_width, int page_size, int num_pages, int n_tokens, int n_requests,
-    int max_q_len, int nh, int g, int hs, float scale, int window, int n_splits, int tiles_per_split, int skip_single, float* lse2,
-    float* scratch, int32_t* work, int32_t* error, cudaStream_t stream) {
+    const int32_t* some_marked, int marked_by, const int32_t* positions, const int32_t* q_start, const int32_t* block_table, int table_width,
+    int page_size, int num_pages, int n_tokens, int n_requests, int max_q_len, int nh, int g, int hs, float scale, int window, int n_splits,
+    int tiles_per_split, int skip_single, float* lse2, float* scratch, int32_t* work, int32_t* error, cudaStream_t stream) {
   if (n_tokens <= 0 || n_requests <= 0) return YALIS_OK;
   if (g <= 0 || nh % g != 0 || max_q_len < 1 || !(scale > 0.f) || n_splits < 1 || n_splits > 64 || tiles_per_split < 1) return YALIS_ERR_SHAPE;
   if (q_stride > 0x7fffffff || out_stride > 0x7fffffff || (window > 0 && n_splits > 1)) return YALIS_ERR_SHAPE;

@@ -167,8 +167,11 @@ __device__ __forceinline__ float4 terms_of(uint32_t word, float scale_log2) {
 //   once: the rest follow as blocks end);
 //   0: all chunks of all pairs, laid end to end, in equal shares; a block's share begins and ends inside pairs that others share.
 // A piece is at least kLeast chunks; to come together with other blocks takes about kJoin chunks' time (64 requests of 520 to 1,040
-// tokens, 8 KV heads of 128: 25 us whole, 36 in equal shares; 8 of 16,000 to 32,000: 66 in nine pieces, 69 in equal shares; 96 of 450
-// to 900, 16 heads over 8: 41 in equal shares).
+// tokens, 8 KV heads of 128: 25 us whole, 36 in equal shares; 8 of 16,000 to 32,000: 66 in nine pieces, 69 in equal shares).
+// More pairs than blocks go out whole, whatever their lengths, which is right where they are alike and short (whole / equal shares, us, heads
+// of 128 over 8: 80 requests of 450 to 900 tokens 37 / 43, 128 of them 45 / 53, 200 of 100 to 300 43 / 53), not where they are long
+// (128 of 2,000 to 8,000: 192 / 174) and least where one is (96 requests, one of 30,000, the others of 200 to 1,000: 269 / 60, in float32
+// 327 / 83): one block walks each of its pairs.
 struct Deal {
   int pieces, blocks;
 };

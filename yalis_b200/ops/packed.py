@@ -207,13 +207,18 @@ def packed_kv_read(pages: PackedPages, positions: torch.Tensor, req_of_token: to
 
 _LONGEST = (1 << 31) - 1   # places are 32-bit numbers
 # Query rows of a pair (tokens * heads of a KV head) beyond which portions are unpacked for the prompt kernel: 64, and more where there
-# are few keys, since that way is two launches and 28 us at least.  By codes / unpacked, us, heads of 64: 16 requests of 8,000 tokens, 8 KV
+# are few keys (of a KV head of a request), since that way is two launches and 28 us at least.  By codes / unpacked, us, heads of 64: 16 requests of 8,000 tokens, 8 KV
 # heads: 64 rows 150 / 160, 128 rows 284 / 150; of 1,000: 64 rows 34 / 40, 128 rows 65 / 39; one of 1,000: 256 rows 18 / 28.
 UNPACK_ROWS, UNPACK_FEW = 64, 1 << 21
 UNPACK_PAGE = 64          # keys of a page of the unpacked pools
 UNPACK_BYTES = 2 << 30    # of unpacked keys and values at a time (one request may take more)
 _unpackings = itertools.count(1)       # numbers by which a launch tells its own note that keys are marked from what the memory held before
 SCORE_BYTES = 1 << 30     # of scores that a step of few rows may leave for its sums; beyond, the products are taken once more
+
+
+def _unpacking_pays(rows: int, keys: int) -> bool:
+    """Whether portions of up to ``rows`` query rows a pair, over up to ``keys`` keys in all, go by unpacked rows."""
+    return rows > UNPACK_ROWS + UNPACK_FEW // max(1, keys)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -328,8 +333,8 @@ def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tenso
     at = (positions.data_ptr(), q_start.data_ptr(), block_table.data_ptr(), columns, r)
     aligned = (q_at | step * (4 if code == F32 else 2)) % 16 == 0
     mma = (dim == 64 or dim == 128) and r <= 4096
-    unpack = (max_q_len * per > UNPACK_ROWS + UNPACK_FEW // max(1, r * g * max_kv_len) and code == BF16 and (dim == 64 or dim == 128) and per <= 128 and scale > 0 and aligned
-              and (out_at | out_step * 2) % 16 == 0)
+    unpack = (code == BF16 and (dim == 64 or dim == 128) and per <= 128 and scale > 0 and aligned and (out_at | out_step * 2) % 16 == 0
+              and _unpacking_pays(max_q_len * per, r * g * max_kv_len))
     # Single tokens beside the portions get a kernel of their own where there may be any: with one, the others have all rows but it.
     single = unpack and mma and max_q_len < n <= (r - 1) * max_q_len + 1
     if unpack:

@@ -27,7 +27,7 @@
 // blocks is added up, in the blocks' order, by whichever of them comes last (a counter per pair, left at zero).  Nothing waits for
 // another block.
 // Bound by instructions, about 490 a chunk and warp (620 and 9 % more time with shifts and subtractions for every pair): 8 requests of
-// 16,000 to 32,000 keys, 24 heads of 128 over 8: 58 us, 212 MB at 3.7 TB/s; 64 requests of 520 to 1,040, 32 heads: 23 us (the general
+// 18,000 to 32,000 keys, 24 heads of 128 over 8: 58 us, 212 MB at 3.7 TB/s; 64 requests of 540 to 1,040, 32 heads: 23 us (the general
 // form: 4,640 and 280).
 #include <cuda_fp16.h>
 
@@ -166,8 +166,8 @@ __device__ __forceinline__ float4 terms_of(uint32_t word, float scale_log2) {
 //   pieces k > 0: every pair to k blocks in equal pieces, one piece a block (one, where there are more pairs than blocks resident at
 //   once: the rest follow as blocks end);
 //   0: all chunks of all pairs, laid end to end, in equal shares; a block's share begins and ends inside pairs that others share.
-// A piece is at least kLeast chunks; to come together with other blocks takes about kJoin chunks' time (64 requests of 520 to 1,040
-// tokens, 8 KV heads of 128: 25 us whole, 36 in equal shares; 8 of 16,000 to 32,000: 66 in nine pieces, 69 in equal shares).
+// A piece is at least kLeast chunks; to come together with other blocks takes about kJoin chunks' time (64 requests of 540 to 1,040
+// tokens, 8 KV heads of 128: 25 us whole, 36 in equal shares; 8 of 18,000 to 32,000: 66 in nine pieces, 69 in equal shares).
 // More pairs than blocks go out whole, whatever their lengths, which is right where they are alike and short (whole / equal shares, us, heads
 // of 128 over 8: 80 requests of 450 to 900 tokens 37 / 43, 128 of them 45 / 53, 200 of 100 to 300 43 / 53), not where they are long
 // (128 of 2,000 to 8,000: 192 / 174) and least where one is (96 requests, one of 30,000, the others of 200 to 1,000: 269 / 60, in float32

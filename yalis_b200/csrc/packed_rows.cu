@@ -4,8 +4,8 @@
 // row's extremes by shuffles, then every lane its word of eight codes.  A block takes rows of one token (keys and values are rows
 // of one list), so that the token's place is looked up without a division a thread; of many tokens it takes TOKENS side by side, whose
 // look-ups (token, page, row: three trips to memory one after the other) overlap.
-// 2 dim values read and dim + 4 bytes written a token and KV head (bfloat16: 512 -> 132 B at 128).  Bound by instructions: 12,003 tokens,
-// 8 KV heads of 128 (62 MB): 25 us to write (2.4 TB/s, issue slots busy 0.78), 14 to read back (4.4 TB/s, 0.70).
+// 2 dim values read and dim + 4 bytes written a token and KV head (bfloat16: 512 -> 132 B at 128).  Bound by instructions: 10,002 tokens,
+// 8 KV heads of 128 (51.5 MB): 25 us to write (2.1 TB/s, issue slots busy 0.78), 14 to read back (3.7 TB/s, 0.70).
 #include "packed.cuh"
 #include "slots.cuh"
 

@@ -393,3 +393,25 @@ def test_the_same_bits_however_the_work_is_divided_from_run_to_run(monkeypatch):
             sums = c.sums.to(DEV)
             runs.append((packed_attention(q.to(DEV), pages, pos.to(DEV), i32(q_start), table, max(brought), 8, weight_sums=sums), sums))
         assert all(torch.equal(a, b) for r in runs[1:] for a, b in zip(runs[0], r))
+
+
+# ---- masks by unpacked rows -----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_masks_and_extremes_by_unpacked_rows(monkeypatch, dim):
+    """Steps of so few rows that the rule of sizes computes them from the codes: rows that see nothing, keys without numbers, scores far
+    apart, rows of one value, values of another size, scales and windows at their limits."""
+    import test_packed_cache_gpu as steps
+    names = launches(monkeypatch, forced=True)
+    for run in (lambda: steps.test_rows_that_see_nothing(torch.bfloat16),
+                lambda: steps.test_large_scores_and_rows_of_one_value(torch.bfloat16, dim),
+                lambda: steps.test_a_row_without_numbers_is_seen_only_by_those_that_see_it(64),
+                lambda: steps.test_values_of_another_size_that_have_no_weight(torch.bfloat16, dim, 9, None),
+                lambda: steps.test_values_of_another_size_that_have_no_weight(torch.bfloat16, dim, 5, 40),
+                lambda: steps.test_queries_of_other_sizes(torch.bfloat16, dim, 9),
+                lambda: steps.test_scales_and_windows_at_their_limits(torch.bfloat16, dim, 7),
+                lambda: steps.test_portions(torch.bfloat16, 4, 2, dim),
+                steps.test_attention_without_a_page):
+        del names[:]
+        run()
+        assert "yalis_packed_unpack" in names

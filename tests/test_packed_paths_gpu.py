@@ -135,6 +135,20 @@ def test_keys_without_a_page_are_left_out(both_forms, dtype, heads, g, dim, page
     check(c, q, pos, q_start, heads, window, sums=False, flag=BAD_PAGE)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,g,dim,page", [(4, 2, 64, 16), (8, 1, 128, 5), (4, 2, 24, 16)])
+@pytest.mark.parametrize("brought", [[1, 1, 1], [9, 3, 1], [100, 130, 1]])
+def test_pages_given_back_behind_windows(both_forms, dtype, heads, g, dim, page, brought):
+    """Pages that lie behind the first row's window may be gone, or another request's: nobody is told."""
+    c, window = Cache([333, 200, 170], g, dim, page, seed=dim), 37
+    for r, n in enumerate(brought):
+        gone = (c.lengths[r] - n - window + 1) // page
+        c.table[r, :gone] = torch.arange(gone).int() % 3 - 1
+    q, pos, q_start = step_of(c, brought, dtype=dtype, heads=heads)
+    check(c, q, pos, q_start, heads, window)
+    both_forms += ["expects_unpacking"] * (dtype == torch.bfloat16 and dim != 24)
+
+
 # ---- places outside the table ---------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])

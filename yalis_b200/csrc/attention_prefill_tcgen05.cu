@@ -147,8 +147,8 @@ __device__ __forceinline__ int first_visible(const PrefillParams& p, int pos) {
 //
 // MARKS: pools unpacked for this launch, in pages of BN keys that follow one another, whose values without numbers lie there as zeros.
 // A row that sees such a value has no result; the others never meet it.  (A key is hidden by the weight 0, which is not enough where
-// the value is none.)  Keys without a page are zeros as well and hidden from every row.  Marks are looked at only where the unpacking says that there are some: a load
-// and a vote for every tile, or a look at its pages' marks for every item, took 2 us of 40 to 74.
+// the value is none.)  Keys without a page are zeros as well and hidden from every row.  Marks are looked at only where the unpacking
+// says that there are some: a load and a vote for every tile, or a look at its pages' marks for every item, took 2 us of 40 to 74.
 template <int HS, bool GEN, bool MARKS>
 __global__ void __launch_bounds__(kThreads, 2)
 prefill_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,

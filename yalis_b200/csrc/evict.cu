@@ -8,10 +8,10 @@
 // histograms of eleven bits and ten, then one walk that numbers what stays, four tokens a thread.  Move: the j-th row that stays lies
 // at or behind place j, so in rounds of consecutive rows (all of them read, the block meets, all written) no row is overwritten before
 // it was read; a group of lanes takes a row of all pools at once, several rows under way.
-// Bound by memory: the sums are read once, a row that moves is read and written once (32 requests of 2,176 to 4,160 tokens to 2,048, 8 KV heads of
-// 128 in bfloat16: 101 us, 495 MB at 4.9 TB/s; with nothing to move 27; one request of 700 tokens: 12 us).  A request alone has a block
-// for each of its KV heads and nothing for the other SMs: 32,000 tokens to 16,000, 8 KV heads of 128: 710 us in bfloat16 and 308 in
-// 4 bits, for 20 and 5.5 at the copy's rate; 128,000 to 64,000: 2,850 and 1,240.
+// Bound by memory: the sums are read once, a row that moves is read and written once (32 requests of 2,176 to 4,160 tokens to 2,048, 8 KV
+// heads of 128 in bfloat16: 101 us, 495 MB at 4.9 TB/s; with nothing to move 27; one request of 700 tokens: 12 us).  A request alone has a
+// block for each of its KV heads and nothing for the other SMs: 32,000 tokens to 16,000, 8 KV heads of 128: 710 us in bfloat16 and 308
+// in 4 bits, for 20 and 5.5 at the copy's rate; 128,000 to 64,000: 2,850 and 1,240.
 #include "common.cuh"
 #include "slots.cuh"
 

@@ -45,7 +45,7 @@ constexpr float kNone = -1e30f;  // the maximum of no scores
 constexpr float kUnset = -3e38f; // limit of a column that has seen no score yet: any will do
 constexpr float kLazy = 8.f;   // how far (log2) scores may rise above the maximum in use before the output is rescaled
 constexpr float kTarget = 6.f; // where (log2) the largest weight times its value's step lies in float16 after that: below 2^15 with kLazy more
-constexpr float kSmall = -80.f;  // steps of less (log2) count as this, which keeps the weights themselves within float32; so do steps that are no numbers
+constexpr float kSmall = -80.f;  // steps of less (log2) count as this, which keeps the weights themselves within float32; so do those that are none
 
 struct MmaParams {
   const void* q;               // [N, q_stride]

@@ -237,8 +237,8 @@ constexpr int kUnpackPage = 64, kUnpackThreads = 256;
 struct UnpackParams {
   __nv_bfloat16* k_out;        // [R * width, g, kUnpackPage, dim]
   __nv_bfloat16* v_out;
-  uint32_t* marks;             // [R * width, g, 2048 / dim]: of key i + (2048 / dim) j of a page in byte j of word i; bit 0 where its
-                               // value holds no numbers, bit 1 where it has no page
+  uint32_t* marks;             // [R * width, g, 2048 / dim]: of key i + (2048 / dim) j of a page in byte j of word i; of keys that some
+                               // row sees, bit 0 where the value holds no numbers, bit 1 where there is no page
   int32_t* some_marked;        // becomes `marked_by`, a number of this launch's own, if any key is marked
   int marked_by;
   int32_t* table_out;          // [R, width]
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kUnpackThreads, 4) packed_unpack_kernel(const 
           const bool none = (word[j] >> 16 & 0x7F80u) == 0x7F80u;
           reinterpret_cast<uint4*>(p.k_out)[(to + r) * words + w] = unpack_bf16(kc[j], word[j] & 0xFFFFu);
           reinterpret_cast<uint4*>(p.v_out)[(to + r) * words + w] = unpack_bf16(vc[j], none ? 0u : word[j] >> 16);
-          marked |= ((none ? 1u : 0u) | (at[j] < 0 ? 2u : 0u)) << (8 * j);
+          if (key0 + r >= first) marked |= ((none ? 1u : 0u) | (at[j] < 0 ? 2u : 0u)) << (8 * j);       // (pages behind a window may be gone)
         }
         if (w == 0) {
           p.marks[to / kUnpackPage * per_round + q] = marked;

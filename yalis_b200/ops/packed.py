@@ -207,8 +207,9 @@ def packed_kv_read(pages: PackedPages, positions: torch.Tensor, req_of_token: to
 
 _LONGEST = (1 << 31) - 1   # places are 32-bit numbers
 # Query rows of a pair (tokens * heads of a KV head) beyond which portions are unpacked for the prompt kernel: 64, and more where there
-# are few keys (of a KV head of a request), since that way is two launches and 28 us at least.  By codes / unpacked, us, heads of 64: 16 requests of 8,000 tokens, 8 KV
-# heads: 64 rows 150 / 160, 128 rows 284 / 150; of 1,000: 64 rows 34 / 40, 128 rows 65 / 39; one of 1,000: 256 rows 18 / 28.
+# are few keys (of all KV heads and requests), since that way is two launches and 28 us at least.  By codes / unpacked, us, heads of
+# 64: 16 requests of 8,000 tokens, 8 KV heads: 64 rows 150 / 160, 128 rows 284 / 150; of 1,000: 64 rows 34 / 40, 128 rows 65 / 39; one
+# of 1,000: 256 rows 18 / 28.
 UNPACK_ROWS, UNPACK_FEW = 64, 1 << 21
 UNPACK_PAGE = 64          # keys of a page of the unpacked pools
 UNPACK_BYTES = 2 << 30    # of unpacked keys and values at a time (one request may take more)
@@ -286,9 +287,12 @@ def packed_attention(q: torch.Tensor, pages: PackedPages, positions: torch.Tenso
     rows of a request, ``max_kv_len`` the places seen (the block table's width bounds them otherwise).  ``weight_sums`` float32
     [pages, kv_heads, page_size]: the softmax weight that a token received, summed over the step's rows and the heads of the KV
     head, is added to it (pages of different requests must differ then).  It is never reset: a place that is written anew (in a page
-    taken again, behind a cut) has the sum of the token that stood there until the caller sets it to zero.  The result is [N, heads * head_dim] in q's dtype
-    (``out`` may be a column block of a wider matrix); rows that see nothing are zeros, rows of no request stay as they are.  Places
-    without a page are left out, as if the row did not see them, and raise the error word's bit.
+    taken again, behind a cut) has the sum of the token that stood there until the caller sets it to zero.
+
+    The result is [N, heads * head_dim] in q's dtype (``out`` may be a column block of a wider matrix); rows that see nothing are
+    zeros, rows of no request stay as they are.  Places without a page are left out, as if the row did not see them, and raise the
+    error word's bit.  A row that sees a key or a value without numbers is NaN; the weights' sums go by the keys alone.
+
     Scores, exponentials, normalisers and sums are float32, and with float32 queries so is every product.  With bfloat16 queries a weight
     is rounded where it meets the value: times the value's step to float16's eleven bits, relative to the row's largest such product,
     where codes are multiplied as they are (there, of a query what lies below 2^-28 of its row's largest is lost, and one of 2^119 or
